@@ -107,6 +107,33 @@ class Activation(ctypes.Structure):
     _fields_ = [("d", P), ("B", I), ("T", I), ("C", I), ("rowmax", P), ("gnst", P)]
 
 
+class _Fields(ctypes.Structure):
+    def __init__(self, **kw):
+        super().__init__()
+        for k, v in kw.items():
+            setattr(self, k, v)
+
+
+class W4(_Fields):
+    """VgemmW4 (include/vgemm_lm.h): `count` matrices of packed 4-bit weights."""
+
+    _fields_ = [("N", I), ("K", I), ("group", I), ("count", I), ("q", P), ("cst", P)]
+
+
+class MoeRoute(_Fields):
+    """VgemmMoeRoute (include/vgemm_lm.h)."""
+
+    _fields_ = [("W", P), ("ldw", I), ("cst", P), ("experts", I), ("topk", I), ("renorm", I), ("Lexp", P), ("idx", P), ("p", P),
+                ("logits", P)]
+
+
+class Moe(_Fields):
+    """VgemmMoe (include/vgemm_lm.h)."""
+
+    _fields_ = [("up", W4), ("down", W4), ("topk", I), ("idx", P), ("p", P), ("Lphi", P), ("Y", P), ("ldy", I), ("residual", P),
+                ("ws", P), ("ws_bytes", SZ)]
+
+
 # (name, restype, argtypes) of every entry point declared in include/vgemm.h, include/vgemm_model.h and
 # include/vgemm_engine.h
 SIGNATURES = [
@@ -180,6 +207,17 @@ SIGNATURES = [
     ("vgemm_engine_transformer", I, [P, P, ctypes.POINTER(Activation), ctypes.c_char_p, I, ctypes.POINTER(Activation)]),
 ]
 
+# the entry points declared in include/vgemm_lm.h
+LM_SIGNATURES = [
+    ("vgemm_rmsnorm_q", I, [P, P, P, I, I, P, LL, P, P, P, P, I]),
+    ("vgemm_w4_bytes", SZ, [I, I, I]),
+    ("vgemm_w4_pack", I, [P, ctypes.POINTER(W4), I, I, P, I, P, P, I, P]),
+    ("vgemm_w4", I, [P, ctypes.POINTER(ASrc), I, ctypes.POINTER(W4), ctypes.POINTER(AEpi)]),
+    ("vgemm_moe_route", I, [P, ctypes.POINTER(ASrc), I, ctypes.POINTER(MoeRoute)]),
+    ("vgemm_moe_workspace_bytes", SZ, [I, I, I]),
+    ("vgemm_moe", I, [P, ctypes.POINTER(ASrc), I, ctypes.POINTER(Moe)]),
+]
+
 _lib = None
 
 
@@ -190,7 +228,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH} is not built: run `python -m vela_amd.build` (there is no fallback path)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, res, args in SIGNATURES:
+        for name, res, args in SIGNATURES + LM_SIGNATURES:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

@@ -2,13 +2,14 @@
 meow::k_gn_stats1 / k_gn_fin1 / k_gn_stats2 / k_gn_apply / k_gn_apply_row / k_lnorm / k_lnorm_q
 (src/kernels.h:21-24,59-63,66-67), same argument order and meaning. Records are GnStat (48 bytes,
 vela_amd.gemm.gn_stats_alloc); a failed check raises VgemmError where the reference throws.
+k_rmsnorm_q (include/vgemm_lm.h) has no counterpart in the reference.
 """
 from __future__ import annotations
 
 from ._lib import check, load
 from .gemm import ptr, stream_ptr
 
-__all__ = ["k_gn_stats1", "k_gn_fin1", "k_gn_stats2", "k_gn_apply", "k_gn_apply_row", "k_lnorm", "k_lnorm_q"]
+__all__ = ["k_gn_stats1", "k_gn_fin1", "k_gn_stats2", "k_gn_apply", "k_gn_apply_row", "k_lnorm", "k_lnorm_q", "k_rmsnorm_q"]
 
 
 def k_gn_stats1(X, B: int, T: int, C: int, groups: int, gs, stream=None) -> None:
@@ -45,3 +46,9 @@ def k_lnorm(X, M: int, C: int, g64, beta64, den: int, Y, stream=None) -> None:
 def k_lnorm_q(X, M: int, C: int, g, beta, den: int, hi, lo, e, Kp: int, stream=None) -> None:
     """meow::k_lnorm_q: the int16 view of the normalised row."""
     check(load().vgemm_lnorm_q(stream_ptr(stream), ptr(X), M, C, ptr(g), ptr(beta), den, ptr(hi), ptr(lo), ptr(e), Kp))
+
+
+def k_rmsnorm_q(X, R, M: int, C: int, g, den: int, H, hi, lo, e, Kp: int, stream=None) -> None:
+    """vgemm_rmsnorm_q: h = sat32(X + R) (R may be None) into H (may be None, X or R), its root-mean-square norm scaled by
+    g as 8-bit rows hi [M, Kp] with shifts e (lo None), or as the int16 view hi / lo / e of k_lnorm_q."""
+    check(load().vgemm_rmsnorm_q(stream_ptr(stream), ptr(X), ptr(R), M, C, ptr(g), den, ptr(H), ptr(hi), ptr(lo), ptr(e), Kp))

@@ -1,0 +1,68 @@
+"""Products of few rows with 4-bit weights over the C ABI of libvgemm.so (include/vgemm_lm.h; no counterpart in the
+reference): w[n, k] = (u[n, k] - z[n, k // group]) * sc[n, k // group] with 4-bit codes u and zero points z and scales
+sc in 0..4095, requantised per column as the W8A16 products are. A failed check raises VgemmError (ValueError for a
+tensor of another shape, type or device).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._lib import W4, AEpi, ASrc, check, load
+from .gemm import ptr, stream_ptr
+
+__all__ = ["W4", "W4Weights", "w4_bytes", "k_gemm_w4"]
+
+
+def w4_bytes(N: int, K: int, group: int) -> int:
+    """Bytes of one packed N x K matrix (0: not supported)."""
+    return int(load().vgemm_w4_bytes(N, K, group))
+
+
+class W4Weights:
+    """Device memory of `count` packed N x K matrices and their column constants; desc is the argument of the calls."""
+
+    def __init__(self, N: int, K: int, group: int, count: int = 1, device="cuda"):
+        nb = w4_bytes(N, K, group)
+        if not nb or count < 1:
+            raise ValueError(f"W4Weights: N >= 1, 1 <= K <= 32768, group 32, 64 or 128 and count >= 1 expected, got {N}, {K}, {group}, {count}")
+        self.N, self.K, self.group, self.count = N, K, group, count
+        self.q = torch.empty(count * nb, dtype=torch.uint8, device=device)
+        self.cst = torch.empty((count, (N + 15) // 16 * 16, 4), dtype=torch.int32, device=device)
+        self.desc = W4(N=N, K=K, group=group, count=count, q=ptr(self.q), cst=ptr(self.cst))
+
+    def pack(self, nib: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, msb: torch.Tensor, first: int = 0, stream=None) -> None:
+        """Lay out matrices first, first + 1, ...: nib uint8 [(n,) N, >= K/2] (column 2i in the low half of byte i), scale
+        int16 or uint16 [(n,) N, groups], zero uint8 alike or None (8 throughout), msb int32 [(n,) N, 4] {m, s, b, unused}. Row
+        strides may be larger than the rows."""
+        N, groups = self.N, (self.K + self.group - 1) // self.group
+        n = nib.shape[0] if nib.dim() == 3 else 1
+
+        def rows(t, dtypes, width, name):
+            shape = (n, N) if nib.dim() == 3 else (N,)
+            if t.dtype not in dtypes or t.dim() != nib.dim() or tuple(t.shape[:-1]) != shape or t.shape[-1] < width or t.device != self.q.device:
+                raise ValueError(f"W4Weights.pack: {name} of shape {tuple(t.shape)}, {t.dtype} on {t.device}")
+            t = t if t.stride(-1) == 1 else t.contiguous()
+            if t.dim() == 3 and n > 1 and t.stride(0) != N * t.stride(1):
+                t = t.contiguous()
+            return t
+
+        nib = rows(nib, (torch.uint8,), (self.K + 1) // 2, "nib")
+        scale = rows(scale, (torch.int16, torch.uint16), groups, "scale")
+        zero = rows(zero, (torch.uint8,), groups, "zero") if zero is not None else None
+        if zero is not None and N > 1 and zero.stride(-2) != scale.stride(-2):
+            scale, zero = scale.contiguous(), zero.contiguous()
+            if zero.shape[-1] != scale.shape[-1]:
+                scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
+        msb = rows(msb, (torch.int32,), 4, "msb")[..., :4].contiguous()
+        ld = lambda t, least: t.stride(-2) if N > 1 else max(t.shape[-1], least)  # noqa: E731
+        check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), ld(nib, 1), ptr(scale), ptr(zero), ld(scale, 1),
+                                   ptr(msb)))
+
+
+def k_gemm_w4(A: ASrc, M: int, W: W4Weights | W4, E: AEpi, stream=None) -> None:
+    """vgemm_w4: M rows (SRC_I8 with or without the low plane, or SRC_X32) times the packed weights; EPI_PLAIN (with a
+    residual) or EPI_GEGLU, row maxima onto the caller's values."""
+    desc = W.desc if isinstance(W, W4Weights) else W
+    check(load().vgemm_w4(stream_ptr(stream), ctypes.byref(A), M, ctypes.byref(desc), ctypes.byref(E)))
