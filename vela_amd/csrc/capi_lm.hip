@@ -53,6 +53,9 @@ vk::W4View w4_view(const VgemmW4& W) {
     return vk::W4View{q, q + size_t(CT) * KT * 1024, reinterpret_cast<const int4*>(W.cst), W.N, W.K, KT, CT};
 }
 
+// strides that keep the rows a kernel addresses with 32-bit offsets below 2^30 bytes: 512 int8 rows, 16 int32 rows
+constexpr int MAX_LD8 = 1 << 21, MAX_LDX = 1 << 23;
+
 int up16(int v) { return (v + 15) / 16 * 16; }
 
 // int8 rows of K values (lo may be null)
@@ -60,6 +63,7 @@ int i8_rows(const char* what, const VgemmASrc* A, int K) {
     if (A->src != VGEMM_SRC_I8) return fail(VGEMM_ERR_ARG, "%s: the rows must be VGEMM_SRC_I8", what);
     if (!A->hi || A->ld8 < up16(K) || A->ld8 % 16 || !aligned(A->hi, 16) || !aligned(A->lo, 16))
         return fail(VGEMM_ERR_ARG, "%s: SRC_I8 planes must be 16-byte aligned with ld8 >= K rounded up to 16, ld8 %% 16 == 0", what);
+    if (A->ld8 > MAX_LD8) return fail(VGEMM_ERR_UNSUPPORTED, "%s: ld8 above %d", what, MAX_LD8);
     return VGEMM_OK;
 }
 
@@ -105,6 +109,7 @@ int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const Vg
     if (A->src == VGEMM_SRC_X32) {
         if (!A->x || !A->rowmax || A->K != W->K || A->K % 4 || A->ldx < A->K || A->ldx % 4 || !aligned(A->x, 16))
             return fail(VGEMM_ERR_ARG, "w4: SRC_X32 needs x, rowmax, K == the weights' K, K %% 4 == 0, ldx >= K, ldx %% 4 == 0, 16-byte alignment");
+        if (A->ldx > MAX_LDX) return fail(VGEMM_ERR_UNSUPPORTED, "w4: ldx above %d", MAX_LDX);
         a.x = A->x; a.ldx = A->ldx; a.xmax = A->rowmax;
     } else {
         if (int rc = i8_rows("w4", A, W->K)) return rc;
@@ -137,12 +142,13 @@ int vgemm_moe_route(void* stream, const VgemmASrc* A, int M, const VgemmMoeRoute
     return hip_status(vk::launch_moe_route(static_cast<hipStream_t>(stream), a, M), "moe_route launch");
 }
 
-// tokens one pass takes, and the floats of its workspace: v, then the column tiles' maxima
+// tokens one pass takes; a pass's workspace holds the plan and for each pair the row of the down product, v and the
+// maxima of v's segments
 static int moe_pass(int M, int topk) { return std::min(M, vk::MOE_PAIRS / topk); }
 
 size_t vgemm_moe_workspace_bytes(int M, int topk, int F) {
     if (M <= 0 || topk < 1 || topk > vk::MOE_TOPK || F < 1) return 0;
-    return size_t(moe_pass(M, topk)) * topk * (size_t(F) + vk::w4_ct(2 * F)) * 4;
+    return sizeof(vk::MoePlan) + size_t(moe_pass(M, topk)) * topk * (size_t(F) + vk::MOE_COLS + vk::w4_ct(2 * F)) * 4;
 }
 
 int vgemm_moe(void* stream, const VgemmASrc* A, int M, const VgemmMoe* P) {
@@ -171,7 +177,9 @@ int vgemm_moe(void* stream, const VgemmASrc* A, int M, const VgemmMoe* P) {
     a.Kp16 = up16(P->up.K);
     a.Lphi = P->Lphi;
     a.ldy = P->ldy;
-    a.v = static_cast<int32_t*>(P->ws);
+    a.plan = static_cast<vk::MoePlan*>(P->ws);
+    a.y = reinterpret_cast<int32_t*>(a.plan + 1);
+    a.v = a.y + size_t(pass) * P->topk * vk::MOE_COLS;
     a.vmax = reinterpret_cast<uint32_t*>(a.v + size_t(pass) * P->topk * F);
     for (int t = 0; t < M; t += pass) {
         a.M = std::min(pass, M - t);

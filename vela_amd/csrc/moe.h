@@ -7,6 +7,7 @@ namespace vk {
 constexpr int MOE_EXPERTS = 512;   // experts a call can have
 constexpr int MOE_TOPK = 16;       // choices a token can have
 constexpr int MOE_PAIRS = 512;     // (token, choice) pairs one pass over the experts takes
+constexpr int MOE_COLS = 8192;     // output columns one pass of the down product takes
 
 struct RouteArgs {
     const int8_t *hi, *lo;
@@ -21,6 +22,16 @@ struct RouteArgs {
     int32_t *idx, *p, *logits;
 };
 
+// The work of a pass (several tokens; of one token the choices themselves are the row tiles)
+struct MoePlan {
+    int tiles;
+    int x[MOE_PAIRS];      // row tiles of at most 16 of an expert's pairs: the expert,
+    int at[MOE_PAIRS];     // first place | rows << 16
+    int pair[MOE_PAIRS];   // the pairs in the order of their experts, those of an expert in their own
+    int pad[3];
+};
+static_assert(sizeof(MoePlan) % 16 == 0, "the workspace's parts begin at multiples of 16 bytes");
+
 struct MoeArgs {
     W4View up, down;             // of expert 0; the others follow at the strides
     size_t up_stride, down_stride;
@@ -33,8 +44,12 @@ struct MoeArgs {
     int32_t* Y;
     int ldy;
     const int32_t* R;
+    MoePlan* plan;
     int32_t* v;                  // [pairs x F]
-    uint32_t* vmax;              // [pairs x up.CT]: max |v| of a column tile
+    uint32_t* vmax;              // [pairs x up_segs]: max |v| of a segment
+    int up_segs;
+    int32_t* y;                  // [pairs x MOE_COLS]: the experts' rows
+    int col0, cols;              // output columns of this pass
 };
 
 hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M);

@@ -1,6 +1,7 @@
 // A mixture-of-experts layer for few tokens: the router (vgemm_moe_route, one kernel) and the chosen experts' feed-forward on
-// 4-bit weights with its combination (vgemm_moe, two kernels: up with GEGLU, down with the sum over a token's choices).
+// 4-bit weights with its combination (vgemm_moe: up with GEGLU, down, and the sum over a token's choices).
 #include <algorithm>
+#include <cmath>
 
 #include "dispatch_rules.h"
 #include "moe.h"
@@ -31,12 +32,13 @@ __device__ __forceinline__ int dot16(const v4i& a, const v4i& b, int c) {
     return c;
 }
 
-constexpr int ROUTE_THREADS = 512;
-constexpr int ROUTE_UNROLL = 4;   // experts a wave reads at once
+constexpr int ROUTE_THREADS = 1024;
 
-// A block per token. Plane sums stay below 16384 * 2^14 = 2^28.
+// A block per token; a wave reads U experts at once. Plane sums stay below 16384 * 2^14 = 2^28.
+template <int U>
 __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
-    __shared__ int s_z[MOE_EXPERTS];
+    __shared__ __align__(16) int s_z[MOE_EXPERTS + 16];
+    __shared__ int s_h[MOE_EXPERTS], s_l[MOE_EXPERTS];
     __shared__ int s_top[MOE_TOPK];
     __shared__ unsigned long long s_sum;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x;
@@ -44,36 +46,52 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     const int8_t* lo = a.lo ? a.lo + size_t(t) * a.ld8 : nullptr;
     const int e = a.e ? a.e[t] : 0;
     if (threadIdx.x == 0) s_sum = 0;
-    for (int x0 = wave * ROUTE_UNROLL; x0 < a.experts; x0 += ROUTE_THREADS / 64 * ROUTE_UNROLL) {
-        int ch[ROUTE_UNROLL], cl[ROUTE_UNROLL];
+    if (threadIdx.x < 16) s_z[a.experts + threadIdx.x] = INT_MIN;
+    for (int x0 = wave * U; x0 < a.experts; x0 += ROUTE_THREADS / 64 * U) {
+        int ch[U], cl[U];
 #pragma unroll
-        for (int i = 0; i < ROUTE_UNROLL; ++i) ch[i] = cl[i] = 0;
+        for (int i = 0; i < U; ++i) ch[i] = cl[i] = 0;
+#pragma unroll 2
         for (int k = lane * 16; k < a.K; k += 1024) {
             const v4i h = *reinterpret_cast<const v4i*>(hi + k);
             const v4i l = lo ? *reinterpret_cast<const v4i*>(lo + k) : v4i{0, 0, 0, 0};
+            v4i w[U];
 #pragma unroll
-            for (int i = 0; i < ROUTE_UNROLL; ++i) {
-                const v4i w = *reinterpret_cast<const v4i*>(a.W + size_t(min(x0 + i, a.experts - 1)) * a.ldw + k);
-                ch[i] = dot16(h, w, ch[i]);
-                if (lo) cl[i] = dot16(l, w, cl[i]);
+            for (int i = 0; i < U; ++i) w[i] = *reinterpret_cast<const v4i*>(a.W + size_t(min(x0 + i, a.experts - 1)) * a.ldw + k);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                ch[i] = dot16(h, w[i], ch[i]);
+                if (lo) cl[i] = dot16(l, w[i], cl[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < ROUTE_UNROLL; ++i) {
+        for (int i = 0; i < U; ++i) {
             const int sh = wave_sum32(ch[i]), sl = lo ? wave_sum32(cl[i]) : 0;
             const int x = x0 + i;
-            if (lane == 0 && x < a.experts) s_z[x] = w4_requant(lo ? 256LL * sh + sl : i64(sh), lo != nullptr, a.cst[x], e);
+            if (lane == 0 && x < a.experts) {
+                s_h[x] = sh;
+                s_l[x] = sl;
+            }
         }
     }
-    __syncthreads();
     const int i = threadIdx.x;
-    const int z = i < a.experts ? s_z[i] : 0;
+    const int4 cst = i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
+    __syncthreads();
+    const int z = i < a.experts ? w4_requant(lo ? 256LL * s_h[i] + s_l[i] : i64(s_h[i]), lo != nullptr, cst, e) : 0;
+    if (i < a.experts) s_z[i] = z;
+    __syncthreads();
     if (i < a.experts) {
         // its place: the logits before it in falling order, equal ones by their index
         int rank = 0;
-        for (int j = 0; j < a.experts; ++j) {
-            const int o = s_z[j];
-            rank += (o > z || (o == z && j < i)) ? 1 : 0;
+        for (int j = 0; j < a.experts; j += 16) {   // INT_MIN behind the last expert counts for nobody
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                const int4 o = *reinterpret_cast<const int4*>(&s_z[j + k]);
+                rank += (o.x > z || (o.x == z && j + k < i)) ? 1 : 0;
+                rank += (o.y > z || (o.y == z && j + k + 1 < i)) ? 1 : 0;
+                rank += (o.z > z || (o.z == z && j + k + 2 < i)) ? 1 : 0;
+                rank += (o.w > z || (o.w == z && j + k + 3 < i)) ? 1 : 0;
+            }
         }
         if (rank < a.topk) {
             a.idx[size_t(t) * a.topk + rank] = i;
@@ -95,286 +113,235 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
 }
 
 hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
-    hipLaunchKernelGGL(moe_route_kernel, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
+    const int waves = ROUTE_THREADS / 64;
+    if (a.experts <= waves) hipLaunchKernelGGL(moe_route_kernel<1>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
+    else if (a.experts <= 4 * waves) hipLaunchKernelGGL(moe_route_kernel<4>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(moe_route_kernel<8>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
-// ---------------------------------------------------------------- up
+// ---------------------------------------------------------------- experts
+//
+// Both products are cut into items (row tile of at most 16 of an expert's pairs, segment of `js` column tiles), a block each,
+// which computes as w4_kernel.h says.
 
-// Block (column tile, s) computes the s-th chosen expert's 16 interleaved columns for all its pairs, 16 rows at a time; waves
-// split K. Blocks past the chosen experts end at once.
-template <int P, int G>
-__global__ void __launch_bounds__(512) moe_up_kernel(MoeArgs a) {
-    constexpr int NG = 128 / G, DEPTH = 2;
-    extern __shared__ uint4 s_dyn[];
-    __shared__ int s_cnt[MOE_EXPERTS];
-    __shared__ int s_list[MOE_PAIRS];
-    __shared__ uint32_t s_max[16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int pairs = a.M * a.topk, ct = blockIdx.x, KT = a.up.KT;
-    for (int i = threadIdx.x; i < a.experts; i += blockDim.x) s_cnt[i] = 0;
+// The pairs sorted by expert and cut into row tiles: one block
+__global__ void __launch_bounds__(256) moe_plan_kernel(MoeArgs a) {
+    __shared__ int s_cnt[MOE_EXPERTS];    // pairs of an expert, then its first place
+    __shared__ int s_rank[MOE_PAIRS];     // a pair's place among its expert's
+    const int pairs = a.M * a.topk, lane = threadIdx.x & 63;
+    MoePlan& T = *a.plan;
+    for (int i = threadIdx.x; i < a.experts; i += 256) s_cnt[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-        const unsigned x = unsigned(a.idx[i]);
-        if (x < unsigned(a.experts)) atomicAdd(&s_cnt[x], 1);
-    }
-    __syncthreads();
-    // every wave finds the expert for itself
-    int x = -1, left = blockIdx.y;
-    for (int c = 0; c < a.experts; c += 64) {
-        u64 m = __builtin_amdgcn_ballot_w64(c + lane < a.experts && s_cnt[c + lane] > 0);
-        const int n = __builtin_popcountll(m);
-        if (left < n) {
-            for (; left; --left) m &= m - 1;
-            x = c + __builtin_ctzll(m);
-            break;
-        }
-        left -= n;
-    }
-    if (x < 0) return;
-    x = __builtin_amdgcn_readfirstlane(x);
-    const int n = __builtin_amdgcn_readfirstlane(s_cnt[x]);
-    for (int c = 0, at = 0; c < pairs && at < n; c += 64) {   // each wave writes the same list
-        const bool hit = c + lane < pairs && a.idx[c + lane] == x;
-        const u64 m = __builtin_amdgcn_ballot_w64(hit);
-        if (hit) s_list[at + __builtin_popcountll(m & ((u64(1) << lane) - 1))] = c + lane;
-        at += __builtin_popcountll(m);
-    }
-    wave_lds_fence();
-    const uint8_t* q = a.up.q + x * a.up_stride + size_t(ct) * KT * 1024;
-    const uint8_t* s = a.up.s + x * a.up_stride + size_t(ct) * KT * 32 * NG;
-    const int4* cst = a.up.cst + size_t(x) * a.up.CT * 16;
-    const int F = a.up.N / 2;
-    for (int r0 = 0; r0 < n; r0 += 16) {
-        const int pr = s_list[min(r0 + (lane & 15), n - 1)];   // the lane's pair
-        const int tok = pr / a.topk;
-        const int8_t* hi = a.hi + size_t(tok) * a.ld8;
-        const int8_t* lo = P == 2 ? a.lo + size_t(tok) * a.ld8 : nullptr;
-        W4Tile<G> t[DEPTH];
-        W4Rows<P> rows[DEPTH][1];
-        double acc[1][4] = {{0.0, 0.0, 0.0, 0.0}};
+    if (threadIdx.x < 64) {
+        const u64 before = (u64(1) << lane) - 1;
+        for (int c = 0; c < pairs; c += 64) {
+            const unsigned x = c + lane < pairs ? unsigned(a.idx[c + lane]) : ~0u;
+            const bool have = x < unsigned(a.experts);
+            u64 same = __builtin_amdgcn_ballot_w64(have);   // lanes with the same expert: nine bits tell 512 apart
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int kt = wave + d * waves;
-            if (kt < KT) {
-                t[d].load(q + size_t(kt) * 1024, s + size_t(kt) * 32 * NG, lane);
-                rows[d][0].template load<G>(hi, lo, kt * 128, a.Kp16, lane);
+            for (int bit = 1; bit < MOE_EXPERTS; bit <<= 1) {
+                const u64 m = __builtin_amdgcn_ballot_w64((x & bit) != 0);
+                same &= (x & bit) ? m : ~m;
             }
+            if (have) {
+                const int n = s_cnt[x];
+                s_rank[c + lane] = n + __builtin_popcountll(same & before);
+                wave_lds_fence();
+                if (!(same & before)) s_cnt[x] = n + __builtin_popcountll(same);
+            }
+            wave_lds_fence();
         }
-        for (int kt = wave; kt < KT; kt += DEPTH * waves) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                const int kd = kt + d * waves;
-                if (kd < KT) {
-                    w4_tile<1, P, G>(t[d], rows[d], acc);
-                    const int kn = kd + DEPTH * waves;
-                    if (kn < KT) {
-                        t[d].load(q + size_t(kn) * 1024, s + size_t(kn) * 32 * NG, lane);
-                        rows[d][0].template load<G>(hi, lo, kn * 128, a.Kp16, lane);
-                    }
-                }
-            }
-        }
-        double2* red = reinterpret_cast<double2*>(s_dyn);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) red[(wave * 2 + h) * 64 + lane] = make_double2(acc[0][2 * h], acc[0][2 * h + 1]);
-        if (threadIdx.x < 16) s_max[threadIdx.x] = 0;
-        __syncthreads();
-        for (int h = wave; h < 2; h += waves) {
-            double2 v = red[h * 64 + lane];
-            for (int w = 1; w < waves; ++w) {
-                const double2 o = red[(w * 2 + h) * 64 + lane];
-                v.x += o.x;
-                v.y += o.y;
-            }
-            const int c = ct * 16 + 4 * (lane >> 4) + 2 * h;
-            const int e = a.e ? a.e[tok] : 0;
-            const int y0 = w4_requant(i64(v.x), P == 2, cst[c], e), y1 = w4_requant(i64(v.y), P == 2, cst[c + 1], e);
-            const int y = geglu_exact(y0, y1, a.Lphi);
-            if (r0 + (lane & 15) < n && c < a.up.N) {
-                a.v[size_t(pr) * F + (c >> 1)] = y;
-                atomicMax(&s_max[lane & 15], uabs(y));
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x < 16 && r0 + int(threadIdx.x) < n) a.vmax[size_t(s_list[r0 + threadIdx.x]) * a.up.CT + ct] = s_max[threadIdx.x];
-        __syncthreads();   // red and s_max are written again
-    }
-}
-
-// ---------------------------------------------------------------- down
-
-// LDS of the down kernel: the pairs' sums, the waves' staging areas and the tables
-constexpr int DOWN_WAVES = 16;
-struct alignas(16) DownTables {   // the staging areas and 64-bit sums follow it in LDS
-    int cnt[MOE_EXPERTS];      // pairs of an expert, then their first place
-    int pos[MOE_PAIRS];        // a pair's place in the order by experts (-1: no expert)
-    int pair[MOE_PAIRS];       // the pair at a place
-    int se[MOE_PAIRS];         // the shift of the row at a place
-    int tile_x[MOE_PAIRS];     // row tiles of at most 16 places: expert,
-    int tile_at[MOE_PAIRS];    // first place | rows << 16
-    int tiles;
-};
-static_assert(sizeof(DownTables) % 16 == 0 && (DOWN_WAVES * 2 * 16 * W4_LDR) % 16 == 0, "alignment of what follows the tables");
-
-// A block owns 16 output columns: for every (row tile of an expert's pairs, K tile) its waves take equal shares, quantise the int32 rows
-// in their own staging area, and add the sums of a pair and column to 64-bit integers in LDS; then each output sums its
-// token's choices. Integer sums: their order does not matter.
-template <int G>
-__global__ void __launch_bounds__(64 * DOWN_WAVES) moe_down_kernel(MoeArgs a) {
-    constexpr int NG = 128 / G, DEPTH = 2;
-    extern __shared__ uint4 s_dyn[];
-    DownTables& T = *reinterpret_cast<DownTables*>(s_dyn);
-    uint8_t* stage_all = reinterpret_cast<uint8_t*>(s_dyn) + sizeof(DownTables);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int pairs = a.M * a.topk, ct = blockIdx.x, KT = a.down.KT, F = a.down.K;
-    unsigned long long* sums = reinterpret_cast<unsigned long long*>(stage_all + DOWN_WAVES * 2 * 16 * W4_LDR);   // [place][16]
-    for (int i = threadIdx.x; i < a.experts; i += blockDim.x) T.cnt[i] = 0;
-    for (int i = threadIdx.x; i < pairs * 16; i += blockDim.x) sums[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-        const unsigned x = unsigned(a.idx[i]);
-        T.pos[i] = x < unsigned(a.experts) ? atomicAdd(&T.cnt[x], 1) : -1;
-    }
-    __syncthreads();
-    if (wave == 0) {   // first places and row tiles
         int at = 0, tiles = 0;
         for (int c = 0; c < a.experts; c += 64) {
-            const int n = c + lane < a.experts ? T.cnt[c + lane] : 0, nt = (n + 15) >> 4;
-            int pn = n, pt = nt;   // inclusive sums over the lanes
+            const int n = c + lane < a.experts ? s_cnt[c + lane] : 0, nt = (n + 15) >> 4;
+            int sum = n | nt << 16;   // inclusive over the lanes, both at once: at most 512 of each
             for (int d = 1; d < 64; d <<= 1) {
-                const int on = __shfl_up(pn, d), ot = __shfl_up(pt, d);
-                if (lane >= d) { pn += on; pt += ot; }
+                const int o = __shfl_up(sum, d);
+                if (lane >= d) sum += o;
             }
-            const int first = at + pn - n, tfirst = tiles + pt - nt;
-            if (c + lane < a.experts) T.cnt[c + lane] = first;
+            const int first = at + (sum & 0xffff) - n, tfirst = tiles + (sum >> 16) - nt;
             for (int i = 0; i < nt; ++i) {
-                T.tile_x[tfirst + i] = c + lane;
-                T.tile_at[tfirst + i] = (first + 16 * i) | min(16, n - 16 * i) << 16;
+                T.x[tfirst + i] = c + lane;
+                T.at[tfirst + i] = (first + 16 * i) | min(16, n - 16 * i) << 16;
             }
-            at += __shfl(pn, 63);
-            tiles += __shfl(pt, 63);
+            if (n > 0) s_cnt[c + lane] = first;
+            const int all = __builtin_amdgcn_readlane(sum, 63);
+            at += all & 0xffff;
+            tiles += all >> 16;
         }
         if (lane == 0) T.tiles = tiles;
     }
     __syncthreads();
-    for (int i = wave; i < pairs; i += DOWN_WAVES) {   // places and the rows' shifts
-        const int x = a.idx[i];
-        if (unsigned(x) >= unsigned(a.experts)) continue;
-        uint32_t m = 0;
-        for (int c = lane; c < a.up.CT; c += 64) m = max(m, a.vmax[size_t(i) * a.up.CT + c]);
-        m = wave_umax32(m);
-        if (lane == 0) {
-            const int at = T.cnt[x] + T.pos[i];
-            T.pos[i] = at;
-            T.pair[at] = i;
-            T.se[at] = rowexp_u32(m);
-        }
+    for (int i = threadIdx.x; i < pairs; i += 256) {
+        const unsigned x = unsigned(a.idx[i]);
+        if (x < unsigned(a.experts)) T.pair[s_cnt[x] + s_rank[i]] = i;
+    }
+}
+
+constexpr int MOE_JS = 8;   // column tiles a segment has at most: 16 KiB of sums
+
+// DOWN = false: rows of the tokens' planes, GEGLU to v [pairs x F], and max |v| of the segment. DOWN = true: rows v, quantised by the
+// largest of their segments' maxima, y [pairs x MOE_COLS].
+template <bool DOWN, int P, int G>
+__global__ void __launch_bounds__(512, 4) moe_kernel(MoeArgs a, int js, int rows_lds) {
+    constexpr int DEPTH = 6;
+    extern __shared__ uint4 s_dyn[];
+    __shared__ uint32_t s_max[16];
+    __shared__ int s_se[16], s_pair[16];
+    int x, first, n;
+    if (a.M == 1) {
+        x = a.idx[blockIdx.y];
+        first = 0;
+        n = unsigned(x) < unsigned(a.experts) ? 1 : 0;
+    } else {
+        if (int(blockIdx.y) >= a.plan->tiles) return;
+        x = a.plan->x[blockIdx.y];
+        first = a.plan->at[blockIdx.y] & 0xffff;
+        n = a.plan->at[blockIdx.y] >> 16;
+    }
+    if (n == 0) return;
+    const W4View& W = DOWN ? a.down : a.up;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
+    const int ctb = DOWN ? a.col0 / 16 : 0, CT = DOWN ? (a.cols + 15) / 16 : W.CT, KT = W.KT, F = a.down.K;
+    const int ct0 = ctb + int(blockIdx.x) * js, tiles = min(js, CT - int(blockIdx.x) * js);
+    uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
+    unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
+    const size_t at = x * (DOWN ? a.down_stride : a.up_stride);
+    const uint8_t* q = W.q + at + size_t(ct0) * KT * 1024;
+    const uint8_t* s = W.s + at + size_t(ct0) * KT * (4096 / G);
+    // as many tiles of K a chunk as the staging area holds of n rows, chunks of even size
+    W4Chunks ch;
+    ch.kc = __builtin_amdgcn_readfirstlane(min(KT, max(1, (w4_div(rows_lds >> 4, n * P) - 1) >> 3)));
+    ch.n = 1;
+    if (ch.kc < KT) {
+        ch.n = __builtin_amdgcn_readfirstlane(w4_div(KT + ch.kc - 1, ch.kc));
+        ch.kc = __builtin_amdgcn_readfirstlane(w4_div(KT + ch.n - 1, ch.n));
+        ch.n = __builtin_amdgcn_readfirstlane(w4_div(KT + ch.kc - 1, ch.kc));
+    }
+    W4Ring<G, DEPTH> ring;
+    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    for (int k = threadIdx.x; k < tiles * 256; k += blockDim.x) sums[k] = 0;
+    if (int(threadIdx.x) < n) {
+        const int pr = a.M == 1 ? int(blockIdx.y) : a.plan->pair[first + threadIdx.x];
+        s_pair[threadIdx.x] = pr;
+        s_max[threadIdx.x] = 0;
+        if constexpr (!DOWN) s_se[threadIdx.x] = a.e ? a.e[w4_div(pr, a.topk)] : 0;
     }
     __syncthreads();
-
-    const int units = T.tiles * KT, u1 = int((long long)units * (wave + 1) / DOWN_WAVES);
-    int u = int((long long)units * wave / DOWN_WAVES);
-    uint8_t* lds = stage_all + wave * 2 * 16 * W4_LDR;
-    if (u < u1) {
-        W4Tile<G> t[DEPTH];
-        W4Quads<16> xq;
-        const auto weights = [&](W4Tile<G>& tile, int ti, int kt) {
-            const int x = __builtin_amdgcn_readfirstlane(T.tile_x[ti]);
-            const size_t at = size_t(ct) * KT + kt;
-            tile.load(a.down.q + x * a.down_stride + at * 1024, a.down.s + x * a.down_stride + at * 32 * NG, lane);
-        };
-        const auto quads = [&](int ti, int kt) {
-            const int w = __builtin_amdgcn_readfirstlane(T.tile_at[ti]);
-            const int* pair = T.pair + (w & 0xffff);
-            xq.load([&](int r) { return a.v + size_t(pair[r]) * F; }, w >> 16, kt * 128, F, lane);
-        };
-        int ti = u / KT, kt = u - ti * KT;      // the unit computed
-        int tl = ti, kl = kt, ul = u;           // the unit whose weights are loaded next
-        const auto next = [&](int& i, int& k) { if (++k == KT) { k = 0; ++i; } };
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d)
-            if (ul < u1) {
-                weights(t[d], tl, kl);
-                next(tl, kl);
-                ++ul;
-            }
-        quads(ti, kt);
-        double acc[1][4] = {{0.0, 0.0, 0.0, 0.0}};
-        for (; u < u1;) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                if (u >= u1) break;
-                const int w = __builtin_amdgcn_readfirstlane(T.tile_at[ti]), first = w & 0xffff, n = w >> 16;
-                wave_lds_fence();
-                xq.stage(lds, T.se + first, n, lane);
-                wave_lds_fence();
-                int tn = ti, kn = kt;
-                next(tn, kn);
-                if (u + 1 < u1) quads(tn, kn);
-                W4Rows<2> rows[1];
-                const int r = min(lane & 15, n - 1);
-                rows[0].template load<G>(reinterpret_cast<const int8_t*>(lds + r * W4_LDR), reinterpret_cast<const int8_t*>(lds + (16 + r) * W4_LDR), 0, 128, lane);
-                w4_tile<1, 2, G>(t[d], rows, acc);
-                if (ul < u1) {
-                    weights(t[d], tl, kl);
-                    next(tl, kl);
-                    ++ul;
-                }
-                if (tn != ti || u + 1 == u1) {   // the last unit of this row tile here
-                    if ((lane & 15) < n) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) atomicAdd(&sums[(first + (lane & 15)) * 16 + 4 * (lane >> 4) + k], (unsigned long long)i64(acc[0][k]));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[0][k] = 0.0;
-                }
-                ti = tn;
-                kt = kn;
-                ++u;
-            }
+    if constexpr (DOWN) {
+        for (int r = wave; r < n; r += waves) {
+            const uint32_t* vm = a.vmax + size_t(s_pair[r]) * a.up_segs;
+            uint32_t m = 0;
+            for (int k = lane; k < a.up_segs; k += 64) m = max(m, vm[k]);
+            m = wave_umax32(m);
+            if (lane == 0) s_se[r] = rowexp_u32(m);
         }
+        __syncthreads();
     }
+    for (int c = 0;;) {
+        const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);
+        if constexpr (DOWN)
+            w4_stage_x32(lds, ch.ld(), n, n, k0, kc, F, a.v, [&](int r) { return unsigned(s_pair[r]) * unsigned(F); }, [&](int r) { return s_se[r]; });
+        else
+            w4_stage<P>(lds, ch.ld(), n, n, k0, kc, a.Kp16, a.hi, a.lo, [&](int r) { return unsigned(w4_div(s_pair[r], a.topk)) * unsigned(a.ld8); });
+        __syncthreads();
+        if (n <= 4) w4_share<1, 1, P, G, DEPTH>(ring, lds, ch.ld(), n, n, sums, lane);
+        else w4_share<1, 4, P, G, DEPTH>(ring, lds, ch.ld(), n, n, sums, lane);
+        if (++c == ch.n) break;
+        ring.start(q, s, KT, tiles, c, ch, lane, wave, waves);
+        __syncthreads();
+    }
+    // two columns a thread; their constants come while the last sums do
+    const int outs = tiles * n * 8, TR = n <= 4 ? 4 : 16;
+    const int4* cst = W.cst + size_t(x) * W.CT * 16;
+    int4 c0, c1;
+    const auto fetch = [&](int k) {
+        const int col = (ct0 + w4_div(k >> 3, n)) * 16 + 2 * (k & 7);
+        c0 = cst[col];
+        c1 = cst[col + 1];
+    };
+    if (int(threadIdx.x) < outs) fetch(threadIdx.x);
     __syncthreads();
-    for (int i = threadIdx.x; i < a.M * 16; i += blockDim.x) {
-        const int tok = i >> 4, c = ct * 16 + (i & 15);
-        if (c >= a.down.N) continue;
-        u64 sum = 0;
-        for (int j = 0; j < a.topk; ++j) {
-            const int at = T.pos[tok * a.topk + j];
-            if (at < 0) continue;
-            const int x = a.idx[tok * a.topk + j];
-            const int y = w4_requant(i64(sums[at * 16 + (i & 15)]), true, a.down.cst[size_t(x) * a.down.CT * 16 + c], T.se[at]);
-            sum += u64(i64(a.p[tok * a.topk + j])) * u64(i64(y));
+    for (int k = threadIdx.x; k < outs; k += blockDim.x) {
+        const int c = w4_div(k >> 3, n), t = (k >> 3) - c * n, col = (ct0 + c) * 16 + 2 * (k & 7), pr = s_pair[t];
+        if (k != int(threadIdx.x)) fetch(k);
+        const longlong2 v = *reinterpret_cast<const longlong2*>(&sums[(c * TR + t) * 16 + 2 * (k & 7)]);
+        const int y0 = w4_requant(v.x, P == 2, c0, s_se[t]), y1 = w4_requant(v.y, P == 2, c1, s_se[t]);
+        if constexpr (DOWN) {
+            *reinterpret_cast<int2*>(a.y + size_t(pr) * MOE_COLS + (col - a.col0)) = make_int2(y0, y1);   // columns past N are not read
+        } else if (col < W.N) {
+            const int y = geglu_exact(y0, y1, a.Lphi);
+            a.v[size_t(pr) * F + (col >> 1)] = y;
+            atomicMax(&s_max[t], uabs(y));
         }
-        const size_t o = size_t(tok) * a.ldy + c;
-        const int y = int(rshr(i64(sum), 15));
-        a.Y[o] = a.R ? add_sat(y, a.R[o]) : y;
+    }
+    if constexpr (!DOWN) {
+        __syncthreads();
+        if (int(threadIdx.x) < n) a.vmax[size_t(s_pair[threadIdx.x]) * a.up_segs + blockIdx.x] = s_max[threadIdx.x];
     }
 }
 
-template <int P, int G>
-static void moe_up(hipStream_t st, const MoeArgs& a) {
-    int waves = 8;
-    while (waves > 1 && waves > a.up.KT) waves /= 2;
-    const dim3 grid(a.up.CT, std::min(a.experts, a.M * a.topk));
-    hipLaunchKernelGGL((moe_up_kernel<P, G>), grid, dim3(64 * waves), size_t(waves) * 2 * 64 * 16, st, a);
-}
-template <int G>
-static void moe_down(hipStream_t st, const MoeArgs& a) {
-    const size_t lds = sizeof(DownTables) + DOWN_WAVES * 2 * 16 * W4_LDR + size_t(a.M) * a.topk * 128;
-    hipLaunchKernelGGL((moe_down_kernel<G>), dim3(a.down.CT), dim3(64 * DOWN_WAVES), lds, st, a);
+// Y[t] = sat32(sat32(rshr(sum_j p y, 15)) + R[t]) over the columns of a pass, eight choices' loads in flight
+__global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
+    const int c = int(blockIdx.x) * 256 + int(threadIdx.x), tok = blockIdx.y;
+    if (c >= a.cols) return;
+    const size_t o = size_t(tok) * a.ldy + a.col0 + c;
+    const int res = a.R ? a.R[o] : 0;
+    u64 sum = 0;
+    for (int j0 = 0; j0 < a.topk; j0 += 8) {
+        int y[8], p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int pr = tok * a.topk + min(j0 + j, a.topk - 1);
+            y[j] = a.y[size_t(pr) * MOE_COLS + c];   // of a pair without an expert: whatever stands there, times 0
+            p[j] = j0 + j < a.topk && unsigned(a.idx[pr]) < unsigned(a.experts) ? a.p[pr] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += u64(i64(p[j])) * u64(i64(y[j]));
+    }
+    a.Y[o] = add_sat(int(rshr(i64(sum), 15)), res);
 }
 
-hipError_t launch_moe(hipStream_t st, const MoeArgs& a) {
-    if (a.group_up == 32) a.lo ? moe_up<2, 32>(st, a) : moe_up<1, 32>(st, a);
-    else if (a.group_up == 64) a.lo ? moe_up<2, 64>(st, a) : moe_up<1, 64>(st, a);
-    else a.lo ? moe_up<2, 128>(st, a) : moe_up<1, 128>(st, a);
+// Column tiles a segment: about one item for each block there can be (two of eight waves a CU), if the tokens chose their experts
+// evenly
+static int moe_js(const MoeArgs& a, int CT) {
+    const double pairs = double(a.M) * a.topk, chosen = a.experts * (1.0 - std::pow(1.0 - 1.0 / a.experts, pairs)), tiles = std::max(chosen, pairs / 16);
+    return std::max(1, std::min(MOE_JS, int(tiles * CT / (2 * NCU))));
+}
+
+template <bool DOWN, int P, int G>
+static void moe_launch(hipStream_t st, const MoeArgs& a, int js) {
+    const int CT = DOWN ? cdiv(a.cols, 16) : a.up.CT, KT = DOWN ? a.down.KT : a.up.KT, pairs = a.M * a.topk;
+    const int tiles = std::min(pairs, std::min(a.experts, pairs) + pairs / 16);   // row tiles at most
+    // two blocks a CU; the 64-bit sums behind the rows begin at a multiple of 16 bytes
+    const int sums = js * 2048, most = (79 << 10) - sums, rows = std::min(16, pairs);
+    const int rows_lds = std::max(rows * P * 144, std::min(most, rows * P * (KT * 128 + 16)));
+    hipLaunchKernelGGL((moe_kernel<DOWN, P, G>), dim3(cdiv(CT, js), tiles), dim3(512), rows_lds + sums, st, a, js, rows_lds);
+}
+template <bool DOWN, int P>
+static void moe_product(hipStream_t st, const MoeArgs& a, int group, int js) {
+    if (group == 32) moe_launch<DOWN, P, 32>(st, a, js);
+    else if (group == 64) moe_launch<DOWN, P, 64>(st, a, js);
+    else moe_launch<DOWN, P, 128>(st, a, js);
+}
+
+hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
+    MoeArgs a = args;
+    const int js = moe_js(a, a.up.CT);
+    a.up_segs = cdiv(a.up.CT, js);
+    if (a.M > 1) hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(256), 0, st, a);
+    if (a.lo) moe_product<false, 2>(st, a, a.group_up, js);
+    else moe_product<false, 1>(st, a, a.group_up, js);
     if (hipError_t e = hipGetLastError()) return e;
-    if (a.group_down == 32) moe_down<32>(st, a);
-    else if (a.group_down == 64) moe_down<64>(st, a);
-    else moe_down<128>(st, a);
-    return hipGetLastError();
+    for (a.col0 = 0; a.col0 < a.down.N; a.col0 += MOE_COLS) {
+        a.cols = std::min(MOE_COLS, a.down.N - a.col0);
+        moe_product<true, 2>(st, a, a.group_down, moe_js(a, cdiv(a.cols, 16)));
+        if (hipError_t e = hipGetLastError()) return e;
+        hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(a.cols, 256), a.M), dim3(256), 0, st, a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace vk

@@ -83,171 +83,129 @@ hipError_t launch_w4_pack(hipStream_t st, int N, int K, int group, uint8_t* q, i
 
 // ---------------------------------------------------------------- products
 
-// A block owns one column tile and 16 MT rows; its waves split K by tiles of 128 (wave w takes tiles w, w + waves, ...), each
-// with DEPTH tiles of weights in flight, and join their sums in LDS. SRC: 0 8-bit rows, 1 planes, 2 int32 rows.
-template <int MT, int SRC, int G>
-__global__ void __launch_bounds__(MT == 1 ? 1024 : (MT == 2 ? 512 : 256)) w4_kernel(W4Args a) {
-    constexpr int P = SRC == 0 ? 1 : 2, RT = 16 * MT, DEPTH = MT == 1 && SRC == 0 && G != 32 ? 4 : 2;
-    constexpr int NG = 128 / G;
+// What two columns' epilogue reads besides the sums: fetched before the products where a thread has one pair of columns
+struct W4Epi {
+    int4 c0, c1;
+    int e, r0, r1;
+};
+
+// A block computes `js` column tiles for up to 4 RR MT rows (see w4_kernel.h). LDS: the rows' chunk, then the sums.
+template <int MT, int RR, int P, int G>
+__global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch, int rows_lds) {
+    constexpr int TR = 4 * RR * MT, DEPTH = MT == 4 ? 4 : 6;
     extern __shared__ uint4 s_dyn[];
-    __shared__ int s_e[SRC == 2 ? RT : 1];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int ct = blockIdx.x, row0 = int(blockIdx.y) * RT, nrows = min(RT, a.M - row0), KT = a.w.KT;
-    const uint8_t* q = a.w.q + size_t(ct) * KT * 1024;
-    const uint8_t* s = a.w.s + size_t(ct) * KT * 32 * NG;
-
-    W4Tile<G> t[DEPTH];
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-        const int kt = wave + d * waves;
-        if (kt < KT) t[d].load(q + size_t(kt) * 1024, s + size_t(kt) * 32 * NG, lane);
+    __shared__ uint32_t s_rm[TR];
+    __shared__ int s_e[TR];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
+    const int ct0 = int(blockIdx.x) * js, tiles = min(js, a.w.CT - ct0), row0 = int(blockIdx.y) * TR, rows = min(TR, a.M - row0), KT = a.w.KT;
+    const int prows = MT == 1 ? rows : TR;
+    uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
+    unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
+    const uint8_t* q = a.w.q + size_t(ct0) * KT * 1024;
+    const uint8_t* s = a.w.s + size_t(ct0) * KT * (4096 / G);
+    const bool x32 = P == 2 && a.x;
+    W4Ring<G, DEPTH> ring;
+    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    for (int i = threadIdx.x; i < tiles * TR * 16; i += blockDim.x) sums[i] = 0;
+    if (int(threadIdx.x) < rows) {
+        s_rm[threadIdx.x] = 0;
+        s_e[threadIdx.x] = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     }
-    double acc[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[mt][r] = 0.0;
-
-    if constexpr (SRC == 2) {
-        if (int(threadIdx.x) < nrows) s_e[threadIdx.x] = rowexp_u32(a.xmax[row0 + threadIdx.x]);
+    if (x32) __syncthreads();
+    for (int c = 0;;) {
+        const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);
+        if (x32)
+            w4_stage_x32(lds, ch.ld(), prows, rows, k0, kc, a.w.K, a.x + size_t(row0) * a.ldx, [&](int r) { return unsigned(r) * unsigned(a.ldx); }, [&](int r) { return s_e[r]; });
+        else
+            w4_stage<P>(lds, ch.ld(), prows, rows, k0, kc, a.Kp16, a.hi + size_t(row0) * a.ld8, P == 2 ? a.lo + size_t(row0) * a.ld8 : nullptr,
+                        [&](int r) { return unsigned(r) * unsigned(a.ld8); });
         __syncthreads();
-        uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn) + wave * (2 * RT * W4_LDR);
-        W4Quads<RT> xq;
-        const int32_t* x0 = a.x + size_t(row0) * a.ldx;
-        const auto rowp = [&](int r) { return x0 + size_t(r) * a.ldx; };
-        if (wave < KT) xq.load(rowp, nrows, wave * 128, a.w.K, lane);
-        for (int kt = wave; kt < KT; kt += DEPTH * waves) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                const int kd = kt + d * waves;
-                if (kd < KT) {
-                    wave_lds_fence();
-                    xq.stage(lds, s_e, nrows, lane);
-                    wave_lds_fence();
-                    if (kd + waves < KT) xq.load(rowp, nrows, (kd + waves) * 128, a.w.K, lane);
-                    W4Rows<2> rows[MT];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const int r = min(16 * mt + (lane & 15), nrows - 1);
-                        rows[mt].template load<G>(reinterpret_cast<const int8_t*>(lds + r * W4_LDR), reinterpret_cast<const int8_t*>(lds + (RT + r) * W4_LDR), 0, 128, lane);
-                    }
-                    w4_tile<MT, 2, G>(t[d], rows, acc);
-                    const int kn = kd + DEPTH * waves;
-                    if (kn < KT) t[d].load(q + size_t(kn) * 1024, s + size_t(kn) * 32 * NG, lane);
-                }
-            }
-        }
-        __syncthreads();   // the staging area is used again below
-    } else {
-        const int8_t *hi[MT], *lo[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const size_t off = size_t(row0 + min(16 * mt + (lane & 15), nrows - 1)) * a.ld8;   // lanes of absent rows compute another row's sums, which nobody reads
-            hi[mt] = a.hi + off;
-            lo[mt] = a.lo + off;
-        }
-        W4Rows<P> rows[DEPTH][MT];
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int kt = wave + d * waves;
-            if (kt < KT) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) rows[d][mt].template load<G>(hi[mt], lo[mt], kt * 128, a.Kp16, lane);
-            }
-        }
-        for (int kt = wave; kt < KT; kt += DEPTH * waves) {
-#pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                const int kd = kt + d * waves;
-                if (kd < KT) {
-                    w4_tile<MT, P, G>(t[d], rows[d], acc);
-                    const int kn = kd + DEPTH * waves;
-                    if (kn < KT) {
-                        t[d].load(q + size_t(kn) * 1024, s + size_t(kn) * 32 * NG, lane);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) rows[d][mt].template load<G>(hi[mt], lo[mt], kn * 128, a.Kp16, lane);
-                    }
-                }
-            }
-        }
+        w4_share<MT, RR, P, G, DEPTH>(ring, lds, ch.ld(), prows, rows, sums, lane);
+        if (++c == ch.n) break;
+        ring.start(q, s, KT, tiles, c, ch, lane, wave, waves);   // on its way while the rows are staged
+        __syncthreads();
     }
-
-    // join the waves' sums: [wave][row tile][column pair][lane] pairs of doubles
-    double2* red = reinterpret_cast<double2*>(s_dyn);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) red[((wave * MT + mt) * 2 + h) * 64 + lane] = make_double2(acc[mt][2 * h], acc[mt][2 * h + 1]);
-    __syncthreads();
-    for (int slot = wave; slot < 2 * MT; slot += waves) {
-        const int mt = slot >> 1, h = slot & 1;
-        double2 v = red[slot * 64 + lane];
-        for (int w = 1; w < waves; ++w) {
-            const double2 o = red[(w * MT * 2 + slot) * 64 + lane];
-            v.x += o.x;
-            v.y += o.y;
+    // two columns a thread
+    const int items = tiles * rows * 8;
+    W4Epi ep;
+    const auto fetch = [&](int i) {
+        const int ctt = w4_div(i >> 3, rows), t = (i >> 3) - ctt * rows, n = (ct0 + ctt) * 16 + 2 * (i & 7);
+        ep.c0 = a.w.cst[n];
+        ep.c1 = a.w.cst[n + 1];
+        ep.r0 = ep.r1 = 0;
+        if (a.R) {
+            const int32_t* R = a.R + size_t(row0 + t) * a.ldy + n;
+            if (n < a.w.N) ep.r0 = R[0];
+            if (n + 1 < a.w.N) ep.r1 = R[1];
         }
-        const int rr = 16 * mt + (lane & 15), n = ct * 16 + 4 * (lane >> 4) + 2 * h;
-        const bool live = rr < nrows && n < a.w.N;
-        const int r = row0 + min(rr, nrows - 1);
-        const int e = SRC == 2 ? s_e[min(rr, nrows - 1)] : (a.e ? a.e[r] : 0);
-        const int4 c0 = a.w.cst[n], c1 = a.w.cst[n + 1];
-        int y0 = w4_requant(i64(v.x), P == 2, c0, e), y1 = w4_requant(i64(v.y), P == 2, c1, e);
-        uint32_t m = 0;
+    };
+    if (int(threadIdx.x) < items) fetch(threadIdx.x);
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += blockDim.x) {
+        const int c = w4_div(i >> 3, rows), t = (i >> 3) - c * rows, n = (ct0 + c) * 16 + 2 * (i & 7), r = row0 + t;
+        if (i != int(threadIdx.x)) fetch(i);
+        if (n >= a.w.N) continue;
+        const longlong2 v = *reinterpret_cast<const longlong2*>(&sums[(c * TR + t) * 16 + 2 * (i & 7)]);
+        int y0 = w4_requant(v.x, P == 2, ep.c0, s_e[t]), y1 = w4_requant(v.y, P == 2, ep.c1, s_e[t]);
+        uint32_t m;
         if (a.geglu) {
             y0 = geglu_exact(y0, y1, a.Lphi);
-            if (live) {
-                a.Y[size_t(r) * a.ldy + (n >> 1)] = y0;
-                m = uabs(y0);
-            }
-        } else if (live) {
+            a.Y[size_t(r) * a.ldy + (n >> 1)] = y0;
+            m = uabs(y0);
+        } else {
             const size_t at = size_t(r) * a.ldy + n;
             const bool two = n + 1 < a.w.N;
-            if (a.R) {
-                y0 = add_sat(y0, a.R[at]);
-                if (two) y1 = add_sat(y1, a.R[at + 1]);
-            }
+            y0 = add_sat(y0, ep.r0);
+            y1 = add_sat(y1, ep.r1);
             a.Y[at] = y0;
             if (two) a.Y[at + 1] = y1;
             m = max(uabs(y0), two ? uabs(y1) : 0u);
         }
-        if (a.rowmax) {
-            m = max(m, uint32_t(__shfl_xor(int(m), 16)));
-            m = max(m, uint32_t(__shfl_xor(int(m), 32)));
-            if (lane < 16 && live && m) atomicMax(a.rowmax + r, m);
+        if (a.rowmax) atomicMax(&s_rm[t], m);
+    }
+    if (a.rowmax) {
+        __syncthreads();
+        // a maximum only grows: a row whose value stands already, even read late, needs no atomic
+        if (int(threadIdx.x) < rows) {
+            uint32_t* to = a.rowmax + row0 + threadIdx.x;
+            const uint32_t m = s_rm[threadIdx.x];
+            if (m > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, m);
         }
     }
 }
 
-template <int MT, int SRC, int G>
-static void w4_launch(hipStream_t st, const W4Args& a, int waves) {
-    constexpr int P = SRC == 0 ? 1 : 2;
-    const size_t red = size_t(waves) * MT * 2 * 64 * 16, stage = SRC == 2 ? size_t(waves) * 2 * 16 * MT * W4_LDR : 0;
-    hipLaunchKernelGGL((w4_kernel<MT, SRC, G>), dim3(a.w.CT, cdiv(a.M, 16 * MT)), dim3(64 * waves), std::max(red, stage), st, a);
+template <int MT, int RR, int P, int G>
+static void w4_launch(hipStream_t st, const W4Args& a) {
+    constexpr int TR = 4 * RR * MT;
+    const int rb = cdiv(a.M, TR), blocks = MT == 1 ? 2 * NCU : NCU;
+    const int js = std::min(8, cdiv((long long)a.w.CT * rb, blocks)), segs = cdiv(a.w.CT, js);
+    const int waves = MT > 1 || (long long)segs * rb <= NCU ? 16 : 8;
+    // the rows whole where they fit in what two blocks (one block) of a CU leave beside the sums
+    const int most = (MT == 1 && waves == 8 ? 78 << 10 : 156 << 10) - js * TR * 128, prows = MT == 1 ? std::min(TR, a.M) : TR;
+    const W4Chunks ch = W4Chunks::of(prows, P, a.w.KT, most);
+    const int rows_lds = prows * P * ch.ld();
+    hipLaunchKernelGGL((w4_kernel<MT, RR, P, G>), dim3(segs, rb), dim3(64 * waves), rows_lds + size_t(js) * TR * 128, st, a, js, ch, rows_lds);
 }
 
-template <int MT, int SRC>
-static void w4_group(hipStream_t st, const W4Args& a, int waves) {
-    if (a.group == 32) w4_launch<MT, SRC, 32>(st, a, waves);
-    else if (a.group == 64) w4_launch<MT, SRC, 64>(st, a, waves);
-    else w4_launch<MT, SRC, 128>(st, a, waves);
+template <int MT, int RR, int P>
+static void w4_group(hipStream_t st, const W4Args& a) {
+    if (a.group == 32) w4_launch<MT, RR, P, 32>(st, a);
+    else if (a.group == 64) w4_launch<MT, RR, P, 64>(st, a);
+    else w4_launch<MT, RR, P, 128>(st, a);
 }
 
-template <int MT>
-static void w4_source(hipStream_t st, const W4Args& a, int waves) {
-    if (a.x) w4_group<1, 2>(st, a, waves);
-    else if (a.lo) w4_group<MT, 1>(st, a, waves);
-    else w4_group<MT, 0>(st, a, waves);
+template <int MT, int RR>
+static void w4_planes(hipStream_t st, const W4Args& a) {
+    if (a.x || a.lo) w4_group<MT, RR, 2>(st, a);
+    else w4_group<MT, RR, 1>(st, a);
 }
 
 hipError_t launch_w4(hipStream_t st, const W4Args& a) {
-    const int MT = a.M <= 16 || a.x ? 1 : (a.M <= 32 ? 2 : 4);
-    const long long blocks = (long long)a.w.CT * cdiv(a.M, 16 * MT);
-    int waves = MT == 1 ? 16 : (MT == 2 ? 8 : 4);
-    while (waves > 1 && (waves > a.w.KT || (waves > 4 && blocks * waves > 8192))) waves /= 2;
-    if (MT == 1) w4_source<1>(st, a, waves);
-    else if (MT == 2) w4_source<2>(st, a, waves);
-    else w4_source<4>(st, a, waves);
+    if (a.M <= 4) w4_planes<1, 1>(st, a);
+    else if (a.M <= 8) w4_planes<1, 2>(st, a);
+    else if (a.M <= 16) w4_planes<1, 4>(st, a);
+    else if (a.M <= 32) w4_planes<2, 4>(st, a);
+    else w4_planes<4, 4>(st, a);
     return hipGetLastError();
 }
 

@@ -2,9 +2,10 @@
 //
 //   acc[r, n] = sum over groups G of sc[n, G] * sum_{k in G} q[r, k] (u[n, k] - z[n, G])
 //
-// The inner sums run on int8 MFMA (16 columns x 64 values of K x 16 rows; 32 values of K where a group has 32): the
+// The inner sums run on int8 MFMA (16 rows x 64 values of K x 16 columns; 32 values of K where a group has 32): the
 // nibbles are spread to bytes and shifted by their zero point in registers, 16-bit rows go through as two planes. A
-// group's sum (below 2^27) is scaled and added in double, which is exact: |acc| <= 2^15 * 15 * 4095 * K < 2^46.
+// group's sum (below 2^27) is scaled and added in 64 bits, one v_mad_i64_i32 a value (6 cycles of a SIMD here; a
+// conversion to double and an fma take 10): |acc| <= 2^15 * 15 * 4095 * K < 2^46.
 //
 // Layout of a matrix: tiles of 16 columns x 128 values of K, [column tile][K tile], 1 KiB of nibbles each, so that a wave
 // streams a tile with one 16-byte load a lane; lane l = 16 j + n holds column n, and nibble half h of its byte b is
@@ -12,6 +13,12 @@
 //   groups of 32:          k = 64 h + 32 (b / 8) + 8 j + b % 8
 // behind all tiles the group words [column tile][K tile][16 columns][128 / group], zero << 12 | scale. Columns past N and
 // values past K have scale 0 and u = z.
+//
+// Work of a block: a segment of column tiles against up to 64 rows. The rows are staged in LDS, as much of K at a time as fits
+// (a chunk): read from memory by every wave, 16 rows of 64 bytes would take 65 cycles of a CU's address unit a load, against
+// 17 for a tile's nibbles and 6 for its words. The chunk's tiles, a column tile's one after the other, are split evenly over the
+// waves, which stream them with DEPTH tiles in flight and add each column tile's sums to 64-bit integers in LDS; the epilogue
+// reads those. Integer sums: their order does not matter.
 #pragma once
 #include "vk_common.h"
 
@@ -31,183 +38,265 @@ __host__ __device__ constexpr size_t w4_bytes(int N, int K, int group) { return 
 typedef unsigned u2v __attribute__((ext_vector_type(2)));
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
-// One tile's words as a lane holds them: its 32 nibbles, the group words of its own column n = lane & 15 (for the zero points)
-// and those of the four columns 4 (lane >> 4) + r whose sums it receives.
+// One tile as a lane holds it: its 32 nibbles and the group words of its column n = lane & 15. Loaded through buffer resources made
+// from scalars, so that the lane offsets never change and no 64-bit address stands in vector registers; where `valid` is
+// not set nothing is fetched and the words are 0.
 template <int G>
 struct W4Tile {
     static constexpr int NG = 128 / G;
     u4v w;
     unsigned own[(NG + 1) / 2];
-    unsigned four[2 * NG];
-    __device__ __forceinline__ void load(const uint8_t* q, const uint8_t* s, int lane) {
-        w = *reinterpret_cast<const u4v*>(q + 16 * lane);
-        const uint8_t* so = s + (lane & 15) * NG * 2;
-        const uint8_t* sf = s + (lane >> 4) * NG * 8;
+    __device__ __forceinline__ void load(const uint8_t* q, const uint8_t* s, bool valid, int lane) {
+        const __amdgpu_buffer_rsrc_t rq = make_rsrc(q, valid ? 1024u : 0u), rs = make_rsrc(s, valid ? 32u * NG : 0u);
+        w = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rq, 16 * lane, 0, 0));
+        const int so = (lane & 15) * NG * 2;
         if constexpr (NG == 1) {
-            own[0] = *reinterpret_cast<const uint16_t*>(so);
-            const u2v f = *reinterpret_cast<const u2v*>(sf);
-            four[0] = f.x; four[1] = f.y;
+            own[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, so, 0, 0);
         } else if constexpr (NG == 2) {
-            own[0] = *reinterpret_cast<const unsigned*>(so);
-            const u4v f = *reinterpret_cast<const u4v*>(sf);
-            four[0] = f.x; four[1] = f.y; four[2] = f.z; four[3] = f.w;
+            own[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0);
         } else {
-            const u2v o = *reinterpret_cast<const u2v*>(so);
+            const u2v o = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rs, so, 0, 0));
             own[0] = o.x; own[1] = o.y;
-            const u4v f = *reinterpret_cast<const u4v*>(sf), f2 = *reinterpret_cast<const u4v*>(sf + 16);
-            four[0] = f.x; four[1] = f.y; four[2] = f.z; four[3] = f.w;
-            four[4] = f2.x; four[5] = f2.y; four[6] = f2.z; four[7] = f2.w;
         }
     }
-    // zero point of the lane's column in group g, in every byte
+    // 0x80 - zero point of group g, in every byte
     __device__ __forceinline__ unsigned zero(int g) const {
         const unsigned z = (g & 1) ? own[g >> 1] >> 28 : (own[g >> 1] >> 12) & 15u;
-        return z * 0x01010101u;
+        return 0x80808080u - z * 0x01010101u;
     }
-    // scale of column 4 (lane >> 4) + r in group g
-    __device__ __forceinline__ double scale(int g, int r) const {
-        const int i = r * NG + g;
-        const unsigned v = (i & 1) ? (four[i >> 1] >> 16) & 0xfffu : four[i >> 1] & 0xfffu;
-        return double(int(v));
-    }
+    __device__ __forceinline__ int scale(int g) const { return int((g & 1) ? (own[g >> 1] >> 16) & 0xfffu : own[g >> 1] & 0xfffu); }
 };
 
-// the low (h = 0) or high nibbles of a word as signed bytes u - z: the bytes 0x80 + u - z borrow nothing from one
-// another, and flipping the top bit leaves u - z in two's complement
-__device__ __forceinline__ int w4_spread(unsigned w, int h, unsigned zz) { return int((((h ? w >> 4 : w) & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ int(0x80808080u); }
-
-// One tile's rows: planes b[p][...] of a lane's row, as the tile's K order needs them (G = 128, 64: values 16 j .. 16 j + 15
-// of each half; G = 32: values 8 j .. 8 j + 7 of each group), 32 bytes a plane.
-template <int P>
-struct W4Rows {
-    v4i b[P][2];
-    template <int G>
-    __device__ __forceinline__ void load(const int8_t* hi, const int8_t* lo, int k0, int Kp16, int lane) {
-        // values past the row's end meet zero weights: any address inside the row will do
-        if constexpr (G == 32) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int k = k0 + 32 * g + 8 * (lane >> 4), kk = k < Kp16 ? k : 0;
-                const u2v h = *reinterpret_cast<const u2v*>(hi + kk);
-                b[0][g >> 1][2 * (g & 1)] = int(h.x); b[0][g >> 1][2 * (g & 1) + 1] = int(h.y);
-                if constexpr (P == 2) {
-                    const u2v l = *reinterpret_cast<const u2v*>(lo + kk);
-                    b[P - 1][g >> 1][2 * (g & 1)] = int(l.x); b[P - 1][g >> 1][2 * (g & 1) + 1] = int(l.y);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = k0 + 64 * h + 16 * (lane >> 4), kk = k < Kp16 ? k : 0;
-                b[0][h] = *reinterpret_cast<const v4i*>(hi + kk);
-                if constexpr (P == 2) b[P - 1][h] = *reinterpret_cast<const v4i*>(lo + kk);
-            }
-        }
-    }
-};
+// the low (h = 0) or high nibbles of a word as signed bytes u - z: no byte of u + (0x80 - z) carries into the next, and
+// flipping the top bit leaves u - z in two's complement
+__device__ __forceinline__ int w4_spread(unsigned w, int h, unsigned zz) { return int((((h ? w >> 4 : w) & 0x0f0f0f0fu) + zz) ^ 0x80808080u); }
 
 __device__ __forceinline__ long w4_pair(int a, int b) { return long((u64(unsigned(b)) << 32) | unsigned(a)); }
 
-// acc[r] += the tile's product for column 4 (lane >> 4) + r and row lane & 15, for MT row tiles
-template <int MT, int P, int G>
-__device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const W4Rows<P> (&rows)[MT], double (&acc)[MT][4]) {
+// Rows in the sums' registers. A lane receives rows 4 (lane >> 4) + r of the 16 of a matrix instruction; with at most 4 RR of
+// them in use they are put where r < RR, so that the others' scaling can be left out: row i of the instruction is row
+// (i / 4) RR + i % RR of the tile.
+template <int RR>
+__device__ __forceinline__ int w4_row(int i) { return (i >> 2) * RR + (i & (RR - 1)); }
+
+// acc[mt][r] += the tile's product for column lane & 15 and the rows above, rows from LDS: a[p] + mt_stride mt is the lane's row of
+// plane p at the tile's first value and the lane's part of it
+template <int MT, int RR, int P, int G>
+__device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const (&a)[P], int mt_stride, i64 (&acc)[MT][RR]) {
     constexpr int NG = 128 / G;
     const v4i zero4 = {0, 0, 0, 0};
     v4i c[MT][P];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        int a[4];
+        int b[4];
         if constexpr (G == 32) {
             const unsigned z0 = t.zero(2 * h), z1 = t.zero(2 * h + 1);
-            a[0] = w4_spread(t.w.x, h, z0); a[1] = w4_spread(t.w.y, h, z0);
-            a[2] = w4_spread(t.w.z, h, z1); a[3] = w4_spread(t.w.w, h, z1);
-        } else {
-            const unsigned z = t.zero(NG == 2 ? h : 0);
-            a[0] = w4_spread(t.w.x, h, z); a[1] = w4_spread(t.w.y, h, z);
-            a[2] = w4_spread(t.w.z, h, z); a[3] = w4_spread(t.w.w, h, z);
-        }
-        if constexpr (G == 32) {
+            b[0] = w4_spread(t.w.x, h, z0); b[1] = w4_spread(t.w.y, h, z0);
+            b[2] = w4_spread(t.w.z, h, z1); b[3] = w4_spread(t.w.w, h, z1);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int g = 2 * h + i;
+                const int g = 2 * h + i, sc = t.scale(g);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        c[mt][p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(w4_pair(a[2 * i], a[2 * i + 1]), w4_pair(rows[mt].b[p][h][2 * i], rows[mt].b[p][h][2 * i + 1]), zero4, 0, 0, 0);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const double sc = t.scale(g, r);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const int v = P == 2 ? c[mt][0][r] * 256 + c[mt][P - 1][r] : c[mt][0][r];
-                        acc[mt][r] = fma(double(v), sc, acc[mt][r]);
+                    for (int p = 0; p < P; ++p) {
+                        const u2v r = *reinterpret_cast<const u2v*>(a[p] + mt * mt_stride + 32 * g);
+                        c[mt][p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(w4_pair(int(r.x), int(r.y)), w4_pair(b[2 * i], b[2 * i + 1]), zero4, 0, 0, 0);
                     }
                 }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < RR; ++r) acc[mt][r] += i64(P == 2 ? c[mt][0][r] * 256 + c[mt][P - 1][r] : c[mt][0][r]) * sc;
             }
         } else {
-            const v4i av = {a[0], a[1], a[2], a[3]};
+            const unsigned z = t.zero(NG == 2 ? h : 0);
+            b[0] = w4_spread(t.w.x, h, z); b[1] = w4_spread(t.w.y, h, z);
+            b[2] = w4_spread(t.w.z, h, z); b[3] = w4_spread(t.w.w, h, z);
+            const v4i bv = {b[0], b[1], b[2], b[3]};
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                 for (int p = 0; p < P; ++p)
-                    c[mt][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, rows[mt].b[p][h], (NG == 1 && h) ? c[mt][p] : zero4, 0, 0, 0);
+                    c[mt][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(a[p] + mt * mt_stride + 64 * h), bv, (NG == 1 && h) ? c[mt][p] : zero4, 0, 0, 0);
             }
             if (NG == 2 || h == 1) {
+                const int sc = t.scale(NG == 2 ? h : 0);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const double sc = t.scale(NG == 2 ? h : 0, r);
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        const int v = P == 2 ? c[mt][0][r] * 256 + c[mt][P - 1][r] : c[mt][0][r];
-                        acc[mt][r] = fma(double(v), sc, acc[mt][r]);
-                    }
-                }
+                    for (int r = 0; r < RR; ++r) acc[mt][r] += i64(P == 2 ? c[mt][0][r] * 256 + c[mt][P - 1][r] : c[mt][0][r]) * sc;
             }
         }
     }
 }
 
-// The quads of int32 rows of one tile, quantised to planes in a wave's own LDS: rows 2 i + (lane >> 5) of `nrows`, 32 lanes a
-// row, [plane][row][W4_LDR]. Row shifts are in se[row].
-constexpr int W4_LDR = 144;   // bytes between rows: 16-byte reads of 16 rows fall on distinct banks
-template <int RT>
-struct W4Quads {
-    int4 v[RT / 2];
-    // rowp(r): address of row r (r < nrows)
-    template <class F>
-    __device__ __forceinline__ void load(F rowp, int nrows, int k0, int K, int lane) {
-        const int k = k0 + 4 * (lane & 31);
-#pragma unroll
-        for (int i = 0; i < RT / 2; ++i) {
-            if (2 * i >= nrows) break;
-            const int r = 2 * i + (lane >> 5);
-            v[i] = make_int4(0, 0, 0, 0);
-            if (r < nrows && k < K) v[i] = *reinterpret_cast<const int4*>(rowp(r) + k);
-        }
-    }
-    __device__ __forceinline__ void stage(uint8_t* lds, const int* se, int nrows, int lane) const {
-#pragma unroll
-        for (int i = 0; i < RT / 2; ++i) {
-            if (2 * i >= nrows) break;
-            const int r = 2 * i + (lane >> 5);
-            if (r < nrows) {
-                const int e = se[r];
-                const int q0 = quant16_32(v[i].x, e), q1 = quant16_32(v[i].y, e), q2 = quant16_32(v[i].z, e), q3 = quant16_32(v[i].w, e);
-                unsigned* h = reinterpret_cast<unsigned*>(lds + r * W4_LDR + 4 * (lane & 31));
-                unsigned* l = reinterpret_cast<unsigned*>(lds + (RT + r) * W4_LDR + 4 * (lane & 31));
-                *h = __builtin_amdgcn_perm(unsigned(q1), unsigned(q0), 0x0c0c0501u) | __builtin_amdgcn_perm(unsigned(q3), unsigned(q2), 0x05010c0cu);
-                *l = (__builtin_amdgcn_perm(unsigned(q1), unsigned(q0), 0x0c0c0400u) | __builtin_amdgcn_perm(unsigned(q3), unsigned(q2), 0x04000c0cu)) ^ 0x80808080u;
-            }
-        }
+// a / b for 0 <= a < 2^22, 0 < b: a quotient of floats is off by less than one
+__device__ __forceinline__ int w4_div(int a, int b) {
+    int q = int(float(a) * __builtin_amdgcn_rcpf(float(b)));
+    const int r = a - q * b;
+    q += r >= b ? 1 : 0;
+    return q - (r < 0 ? 1 : 0);
+}
+
+// The rows of a chunk in LDS, [plane][prows][ld]: ld = the chunk's bytes a row + 16, so that 16 rows' 16-byte reads fall on
+// distinct banks. As many tiles of K a chunk as `lds` bytes hold, chunks of even size.
+struct W4Chunks {
+    int kc, n;   // tiles of K a chunk, chunks
+    __host__ __device__ __forceinline__ int ld() const { return kc * 128 + 16; }
+    static __host__ W4Chunks of(int prows, int P, int KT, int lds) {
+        const int fit = (lds / (prows * P) - 16) / 128, most = fit < 1 ? 1 : fit;
+        W4Chunks c;
+        c.n = (KT + most - 1) / most;
+        c.kc = (KT + c.n - 1) / c.n;
+        c.n = (KT + c.kc - 1) / c.kc;
+        return c;
     }
 };
 
-// orders a wave's LDS writes before its other lanes' reads (and the reverse); LDS operations of a wave run in order
+// orders a wave's LDS accesses for its other lanes (LDS operations of a wave run in order)
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+}
+
+// int8 planes to LDS, 16 bytes a thread and step, four steps in flight. off(r): byte offset of row r in its plane (below 2^30); bytes
+// past Kp16 are not written (they meet zero weights)
+template <int P, class F>
+__device__ __forceinline__ void w4_stage(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int Kp16, const int8_t* hi, const int8_t* lo, F off) {
+    const int per = min(kc * 8, (Kp16 - k0 * 128) >> 4), items = rows * per, step = blockDim.x;
+    for (int i0 = threadIdx.x; i0 < items; i0 += 4 * step) {
+        v4i v[4][P];
+        int at[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int i = min(i0 + b * step, items - 1), r = w4_div(i, per), c = 16 * (i - r * per);
+            at[b] = r * ld + c;
+            const unsigned from = off(r) + unsigned(k0 * 128 + c);
+            v[b][0] = *reinterpret_cast<const v4i*>(hi + from);
+            if constexpr (P == 2) v[b][P - 1] = *reinterpret_cast<const v4i*>(lo + from);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {   // the last item may be written more than once
+            *reinterpret_cast<v4i*>(lds + at[b]) = v[b][0];
+            if constexpr (P == 2) *reinterpret_cast<v4i*>(lds + prows * ld + at[b]) = v[b][P - 1];
+        }
+    }
+}
+
+// int32 rows quantised to planes in LDS, four values a thread and step, eight steps in flight: off(r) the row's offset in values (below
+// 2^28), shift(r) its shift. K % 4 == 0. `tpr` threads work on a row, so that a row's address and shift are found once: about a
+// quarter of its quads, more where the rows are too few for the block.
+template <class F, class S>
+__device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int K, const int32_t* x, F off, S shift) {
+    constexpr int B = 8;
+    const int per = min(kc * 32, (K - k0 * 128) >> 2), threads = blockDim.x;
+    int lg = 31 - __builtin_clz(max(64, per >> 2));
+    while ((1 << lg) < threads && (threads >> lg) > rows) ++lg;
+    const int tpr = min(1 << lg, threads), side = threads / tpr;
+    const s2 lim = {-32767, -32767};
+    for (int r = int(threadIdx.x) / tpr; r < rows; r += side) {
+        const int e = shift(r), one = e ? 1 : 0;
+        const unsigned from = off(r) + unsigned(k0 * 128);
+        // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only -32768 is
+        // left to raise
+        const auto q = [&](int w) { return (w >> e) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e - 1), unsigned(one))); };
+        for (int c0 = int(threadIdx.x) & (tpr - 1); c0 < per; c0 += B * tpr) {
+            v4i v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const v4i*>(x + (from + 4u * unsigned(min(c0 + b * tpr, per - 1))));
+#pragma unroll
+            for (int b = 0; b < B; ++b) {   // the last quad may be written more than once
+                const s2 q0 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][0]), q(v[b][1])), lim);
+                const s2 q1 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][2]), q(v[b][3])), lim);
+                const unsigned u0 = __builtin_bit_cast(unsigned, q0), u1 = __builtin_bit_cast(unsigned, q1);
+                uint8_t* to = lds + r * ld + 4 * min(c0 + b * tpr, per - 1);
+                *reinterpret_cast<unsigned*>(to) = __builtin_amdgcn_perm(u1, u0, 0x07050301u);
+                *reinterpret_cast<unsigned*>(to + prows * ld) = __builtin_amdgcn_perm(u1, u0, 0x06040200u) ^ 0x80808080u;
+            }
+        }
+    }
+}
+
+// A wave's share of a chunk: tiles u of the segment's column tiles c = u / kc, in the order of their addresses
+template <int G, int DEPTH>
+struct W4Ring {
+    W4Tile<G> t[DEPTH];
+    const uint8_t *q, *s;      // of the segment's first column tile
+    int KT, k0, kc;
+    int u0, u1;                // the wave's tiles
+    int u, c, k;               // the tile loaded next
+    __device__ __forceinline__ void fetch(int d, int lane) {
+        const size_t tile = size_t(c) * KT + k0 + k;
+        t[d].load(q + tile * 1024, s + tile * (4096 / G), u < u1, lane);
+        ++u;
+        if (++k == kc) {
+            k = 0;
+            ++c;
+        }
+    }
+    __device__ __forceinline__ void start(const uint8_t* q_, const uint8_t* s_, int KT_, int tiles, int chunk, const W4Chunks& ch, int lane, int wave, int waves) {
+        q = q_;
+        s = s_;
+        KT = KT_;
+        k0 = chunk * ch.kc;
+        kc = min(ch.kc, KT - k0);
+        const int units = tiles * kc;
+        const int sh = __builtin_ctz(waves);   // a power of two
+        u0 = __builtin_amdgcn_readfirstlane((units * wave) >> sh);
+        u1 = __builtin_amdgcn_readfirstlane((units * (wave + 1)) >> sh);
+        u = u0;
+        c = __builtin_amdgcn_readfirstlane(w4_div(u0, kc));
+        k = u0 - c * kc;
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) fetch(d, lane);
+    }
+};
+
+// The wave's share: sums of column tile c, row t and column n are added to sums[(c * TR + t) * 16 + n], TR = 4 RR MT
+template <int MT, int RR, int P, int G, int DEPTH>
+__device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* lds, int ld, int prows, int rows, unsigned long long* sums, int lane) {
+    constexpr int TR = 4 * RR * MT;
+    int u = ring.u0, c = __builtin_amdgcn_readfirstlane(w4_div(u, ring.kc)), k = u - c * ring.kc;
+    if (u >= ring.u1) return;
+    // rows of the instruction past the last one repeat it (in the last row tile of several: what stands there): nobody reads
+    // their sums
+    const uint8_t* base[P];
+    static_assert(MT == 1 || RR == 4, "row tiles are whole");
+    const int lane_off = G == 32 ? 8 * (lane >> 4) : 16 * (lane >> 4);
+#pragma unroll
+    for (int p = 0; p < P; ++p) base[p] = lds + (p * prows + min(w4_row<RR>(lane & 15), rows - 1)) * ld + lane_off;
+    i64 acc[MT][RR];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < RR; ++r) acc[mt][r] = 0;
+    for (;;) {
+        bool more = true;
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const uint8_t* a[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) a[p] = base[p] + k * 128;
+            w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc);
+            __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
+            ring.fetch(d, lane);
+            const bool last = ++u == ring.u1;
+            if (++k == ring.kc || last) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < RR; ++r) {
+                        atomicAdd(&sums[(c * TR + 16 * mt + (lane >> 4) * RR + r) * 16 + (lane & 15)], (unsigned long long)acc[mt][r]);
+                        acc[mt][r] = 0;
+                    }
+                k = 0;
+                ++c;
+            }
+            if (last) { more = false; break; }
+        }
+        if (!more) break;
+    }
 }
 
 // The exact epilogue value of a column: acc the product, planes whether the rows carry the offset low plane
