@@ -12,7 +12,7 @@ namespace vk {
 // ---------------------------------------------------------------- router
 
 // exp table lookup of the attention: 0 from 2^20 on, else linear between entries z >> 10 and (z >> 10) + 1
-__device__ __forceinline__ i64 moe_lutexp(uint32_t z, const i64* __restrict__ L) {
+__device__ __forceinline__ i64 moe_lutexp(uint32_t z, const i64* L) {
     if (z >= (16u << 16)) return 0;
     const i64 a = L[z >> 10], b = L[(z >> 10) + 1];
     return a + (((b - a) * i64(z & 1023)) >> 10);
@@ -33,6 +33,26 @@ __device__ __forceinline__ int dot16(const v4i& a, const v4i& b, int c) {
 }
 
 constexpr int ROUTE_THREADS = 1024;
+constexpr int EXP_N = 1025;
+
+// sum over the wave of values whose total stays below 2^63
+__device__ __forceinline__ i64 wave_sum64(i64 v) {
+    for (int d = 32; d; d >>= 1) v += i64(__shfl_xor((long long)v, d));
+    return v;
+}
+
+// floor(2^62 / s): from a quotient of doubles, whose error is below one for s >= 2^20 (quotients below 2^42)
+__device__ __forceinline__ u64 route_recip(u64 s) {
+    const u64 one = u64(1) << 62;
+    if (s < (1u << 20)) return s ? one / s : 0;
+    u64 q = u64(0x1p62 / double(s));
+    i64 r = i64(one - q * s);
+    if (r < 0) {
+        --q;
+        r += i64(s);
+    }
+    return r >= i64(s) ? q + 1 : q;
+}
 
 // A block per token; a wave reads U experts at once. Plane sums stay below 16384 * 2^14 = 2^28.
 template <int U>
@@ -40,13 +60,11 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     __shared__ __align__(16) int s_z[MOE_EXPERTS + 16];
     __shared__ int s_h[MOE_EXPERTS], s_l[MOE_EXPERTS];
     __shared__ int s_top[MOE_TOPK];
-    __shared__ unsigned long long s_sum;
+    __shared__ i64 s_exp[EXP_N], s_sum[ROUTE_THREADS / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x;
     const int8_t* hi = a.hi + size_t(t) * a.ld8;
     const int8_t* lo = a.lo ? a.lo + size_t(t) * a.ld8 : nullptr;
     const int e = a.e ? a.e[t] : 0;
-    if (threadIdx.x == 0) s_sum = 0;
-    if (threadIdx.x < 16) s_z[a.experts + threadIdx.x] = INT_MIN;
     for (int x0 = wave * U; x0 < a.experts; x0 += ROUTE_THREADS / 64 * U) {
         int ch[U], cl[U];
 #pragma unroll
@@ -76,38 +94,50 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     }
     const int i = threadIdx.x;
     const int4 cst = i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
+    for (int k = i; k < EXP_N; k += ROUTE_THREADS) s_exp[k] = a.Lexp[k];
+    if (i < 16) s_z[a.experts + i] = INT_MIN;
     __syncthreads();
     const int z = i < a.experts ? w4_requant(lo ? 256LL * s_h[i] + s_l[i] : i64(s_h[i]), lo != nullptr, cst, e) : 0;
-    if (i < a.experts) s_z[i] = z;
-    __syncthreads();
     if (i < a.experts) {
-        // its place: the logits before it in falling order, equal ones by their index
-        int rank = 0;
-        for (int j = 0; j < a.experts; j += 16) {   // INT_MIN behind the last expert counts for nobody
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-                const int4 o = *reinterpret_cast<const int4*>(&s_z[j + k]);
-                rank += (o.x > z || (o.x == z && j + k < i)) ? 1 : 0;
-                rank += (o.y > z || (o.y == z && j + k + 1 < i)) ? 1 : 0;
-                rank += (o.z > z || (o.z == z && j + k + 2 < i)) ? 1 : 0;
-                rank += (o.w > z || (o.w == z && j + k + 3 < i)) ? 1 : 0;
-            }
-        }
-        if (rank < a.topk) {
-            a.idx[size_t(t) * a.topk + rank] = i;
-            s_top[rank] = z;
-        }
+        s_z[i] = z;
         if (a.logits) a.logits[size_t(t) * a.experts + i] = z;
     }
     __syncthreads();
-    const uint32_t top = uint32_t(s_top[0]);
-    const i64 mine = i < a.topk ? moe_lutexp(top - uint32_t(s_top[i]), a.Lexp) : 0;   // the i-th choice's
-    const i64 part = a.renorm ? mine : (i < a.experts ? moe_lutexp(top - uint32_t(z), a.Lexp) : 0);
-    if (part) atomicAdd(&s_sum, (unsigned long long)part);
+    // an expert's place: the logits before it in falling order, equal ones by their index; `side` threads an expert, 16 logits a
+    // step (INT_MIN behind the last expert counts for nobody)
+    const int lg = a.experts <= 128 ? 3 : (a.experts <= 256 ? 2 : 1), side = 1 << lg, x = i >> lg;
+    if (x < a.experts) {
+        const int zx = s_z[x];
+        int rank = 0;
+        for (int j = 16 * (i & (side - 1)); j < a.experts; j += 16 * side) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                const int4 o = *reinterpret_cast<const int4*>(&s_z[j + k]);
+                rank += (o.x > zx || (o.x == zx && j + k < x)) ? 1 : 0;
+                rank += (o.y > zx || (o.y == zx && j + k + 1 < x)) ? 1 : 0;
+                rank += (o.z > zx || (o.z == zx && j + k + 2 < x)) ? 1 : 0;
+                rank += (o.w > zx || (o.w == zx && j + k + 3 < x)) ? 1 : 0;
+            }
+        }
+        for (int d = 1; d < side; d <<= 1) rank += __shfl_xor(rank, d);
+        if ((i & (side - 1)) == 0 && rank < a.topk) {
+            a.idx[size_t(t) * a.topk + rank] = x;
+            s_top[rank] = zx;
+        }
+    }
     __syncthreads();
+    const uint32_t top = uint32_t(s_top[0]);
+    const i64 mine = i < a.topk ? moe_lutexp(top - uint32_t(s_top[i]), s_exp) : 0;   // the i-th choice's
+    const int members = a.renorm ? a.topk : a.experts;
+    if (64 * wave < members) {
+        const i64 part = a.renorm ? mine : (i < a.experts ? moe_lutexp(top - uint32_t(z), s_exp) : 0), sum = wave_sum64(part);
+        if (lane == 0) s_sum[wave] = sum;
+    }
+    if (!a.renorm) __syncthreads();   // the chosen are all in the first wave
     if (i < a.topk) {
-        const u64 sum = s_sum, r = sum ? (u64(1) << 62) / sum : 0;
-        const u64 p = (u64(mine) * r + (u64(1) << 46)) >> 47;
+        u64 sum = 0;
+        for (int w = 0; 64 * w < members; ++w) sum += u64(s_sum[w]);
+        const u64 p = (u64(mine) * route_recip(sum) + (u64(1) << 46)) >> 47;
         a.p[size_t(t) * a.topk + i] = int(min(p, u64(32767)));
     }
 }
@@ -179,12 +209,12 @@ __global__ void __launch_bounds__(256) moe_plan_kernel(MoeArgs a) {
     }
 }
 
-constexpr int MOE_JS = 8;   // column tiles a segment has at most: 16 KiB of sums
+constexpr int MOE_JS = 16;   // column tiles a segment has at most: 32 KiB of sums
 
 // DOWN = false: rows of the tokens' planes, GEGLU to v [pairs x F], and max |v| of the segment. DOWN = true: rows v, quantised by the
 // largest of their segments' maxima, y [pairs x MOE_COLS].
 template <bool DOWN, int P, int G>
-__global__ void __launch_bounds__(512, 4) moe_kernel(MoeArgs a, int js, int rows_lds) {
+__global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_lds) {
     constexpr int DEPTH = 6;
     extern __shared__ uint4 s_dyn[];
     __shared__ uint32_t s_max[16];
@@ -195,10 +225,10 @@ __global__ void __launch_bounds__(512, 4) moe_kernel(MoeArgs a, int js, int rows
         first = 0;
         n = unsigned(x) < unsigned(a.experts) ? 1 : 0;
     } else {
-        if (int(blockIdx.y) >= a.plan->tiles) return;
+        const int w = a.plan->at[blockIdx.y];   // beside the number of tiles, not behind it: what stands there past the last is not used
         x = a.plan->x[blockIdx.y];
-        first = a.plan->at[blockIdx.y] & 0xffff;
-        n = a.plan->at[blockIdx.y] >> 16;
+        first = w & 0xffff;
+        n = int(blockIdx.y) < a.plan->tiles ? w >> 16 : 0;
     }
     if (n == 0) return;
     const W4View& W = DOWN ? a.down : a.up;
@@ -207,6 +237,8 @@ __global__ void __launch_bounds__(512, 4) moe_kernel(MoeArgs a, int js, int rows
     const int ct0 = ctb + int(blockIdx.x) * js, tiles = min(js, CT - int(blockIdx.x) * js);
     uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
     unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
+    int32_t* lut = reinterpret_cast<int32_t*>(sums + js * 256);   // of the gate
+    if constexpr (!DOWN) w4_load_lut(lut, a.Lphi);
     const size_t at = x * (DOWN ? a.down_stride : a.up_stride);
     const uint8_t* q = W.q + at + size_t(ct0) * KT * 1024;
     const uint8_t* s = W.s + at + size_t(ct0) * KT * (4096 / G);
@@ -271,7 +303,7 @@ __global__ void __launch_bounds__(512, 4) moe_kernel(MoeArgs a, int js, int rows
         if constexpr (DOWN) {
             *reinterpret_cast<int2*>(a.y + size_t(pr) * MOE_COLS + (col - a.col0)) = make_int2(y0, y1);   // columns past N are not read
         } else if (col < W.N) {
-            const int y = geglu_exact(y0, y1, a.Lphi);
+            const int y = geglu_exact(y0, y1, lut);
             a.v[size_t(pr) * F + (col >> 1)] = y;
             atomicMax(&s_max[t], uabs(y));
         }
@@ -303,40 +335,45 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
     a.Y[o] = add_sat(int(rshr(i64(sum), 15)), res);
 }
 
-// Column tiles a segment: about one item for each block there can be (two of eight waves a CU), if the tokens chose their experts
-// evenly
-static int moe_js(const MoeArgs& a, int CT) {
+// Shape of the items if the tokens choose their experts evenly: sixteen waves, a whole CU, for the down product from four pairs
+// an expert on, where quantising the rows counts, else eight, two items a CU; column tiles a segment for about one item a place,
+// with a margin for more experts chosen than expected (a second round of a few items costs as much as the first).
+struct MoeShape {
+    int waves, js;
+};
+static MoeShape moe_shape(const MoeArgs& a, int CT, bool down) {
     const double pairs = double(a.M) * a.topk, chosen = a.experts * (1.0 - std::pow(1.0 - 1.0 / a.experts, pairs)), tiles = std::max(chosen, pairs / 16);
-    return std::max(1, std::min(MOE_JS, int(tiles * CT / (2 * NCU))));
+    const int waves = down && pairs / chosen >= 4.0 ? 16 : 8;
+    return {waves, std::max(1, std::min(MOE_JS, int(std::ceil(1.1 * tiles * CT / (waves == 16 ? NCU : 2 * NCU)))))};
 }
 
 template <bool DOWN, int P, int G>
-static void moe_launch(hipStream_t st, const MoeArgs& a, int js) {
+static void moe_launch(hipStream_t st, const MoeArgs& a, MoeShape sh) {
     const int CT = DOWN ? cdiv(a.cols, 16) : a.up.CT, KT = DOWN ? a.down.KT : a.up.KT, pairs = a.M * a.topk;
     const int tiles = std::min(pairs, std::min(a.experts, pairs) + pairs / 16);   // row tiles at most
-    // two blocks a CU; the 64-bit sums behind the rows begin at a multiple of 16 bytes
-    const int sums = js * 2048, most = (79 << 10) - sums, rows = std::min(16, pairs);
-    const int rows_lds = std::max(rows * P * 144, std::min(most, rows * P * (KT * 128 + 16)));
-    hipLaunchKernelGGL((moe_kernel<DOWN, P, G>), dim3(cdiv(CT, js), tiles), dim3(512), rows_lds + sums, st, a, js, rows_lds);
+    // the 64-bit sums behind the rows begin at a multiple of 16 bytes
+    const int sums = sh.js * 2048, lut = DOWN ? 0 : W4_LUT_LDS, most = (sh.waves == 16 ? 158 << 10 : 79 << 10) - sums - lut, rows = std::min(16, pairs);
+    const int rows_lds = std::max(rows * P * 144, std::min(most & ~15, rows * P * (KT * 128 + 16)));
+    hipLaunchKernelGGL((moe_kernel<DOWN, P, G>), dim3(cdiv(CT, sh.js), tiles), dim3(64 * sh.waves), rows_lds + sums + lut, st, a, sh.js, rows_lds);
 }
 template <bool DOWN, int P>
-static void moe_product(hipStream_t st, const MoeArgs& a, int group, int js) {
-    if (group == 32) moe_launch<DOWN, P, 32>(st, a, js);
-    else if (group == 64) moe_launch<DOWN, P, 64>(st, a, js);
-    else moe_launch<DOWN, P, 128>(st, a, js);
+static void moe_product(hipStream_t st, const MoeArgs& a, int group, MoeShape sh) {
+    if (group == 32) moe_launch<DOWN, P, 32>(st, a, sh);
+    else if (group == 64) moe_launch<DOWN, P, 64>(st, a, sh);
+    else moe_launch<DOWN, P, 128>(st, a, sh);
 }
 
 hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     MoeArgs a = args;
-    const int js = moe_js(a, a.up.CT);
-    a.up_segs = cdiv(a.up.CT, js);
+    const MoeShape up = moe_shape(a, a.up.CT, false);
+    a.up_segs = cdiv(a.up.CT, up.js);
     if (a.M > 1) hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(256), 0, st, a);
-    if (a.lo) moe_product<false, 2>(st, a, a.group_up, js);
-    else moe_product<false, 1>(st, a, a.group_up, js);
+    if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
+    else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
     for (a.col0 = 0; a.col0 < a.down.N; a.col0 += MOE_COLS) {
         a.cols = std::min(MOE_COLS, a.down.N - a.col0);
-        moe_product<true, 2>(st, a, a.group_down, moe_js(a, cdiv(a.cols, 16)));
+        moe_product<true, 2>(st, a, a.group_down, moe_shape(a, cdiv(a.cols, 16), true));
         if (hipError_t e = hipGetLastError()) return e;
         hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(a.cols, 256), a.M), dim3(256), 0, st, a);
         if (hipError_t e = hipGetLastError()) return e;

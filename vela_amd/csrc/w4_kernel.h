@@ -20,6 +20,8 @@
 // waves, which stream them with DEPTH tiles in flight and add each column tile's sums to 64-bit integers in LDS; the epilogue
 // reads those. Integer sums: their order does not matter.
 #pragma once
+#include <utility>
+
 #include "vk_common.h"
 
 namespace vk {
@@ -160,17 +162,25 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// i / per by a multiplication, for i * per < 2^32
+struct W4Per {
+    unsigned per, m;
+    __device__ __forceinline__ explicit W4Per(int n) : per(n), m(0xffffffffu / unsigned(n) + 1u) {}
+    __device__ __forceinline__ int of(int i) const { return per == 1 ? i : int(__umulhi(unsigned(i), m)); }
+};
+
 // int8 planes to LDS, 16 bytes a thread and step, four steps in flight. off(r): byte offset of row r in its plane (below 2^30); bytes
 // past Kp16 are not written (they meet zero weights)
 template <int P, class F>
 __device__ __forceinline__ void w4_stage(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int Kp16, const int8_t* hi, const int8_t* lo, F off) {
     const int per = min(kc * 8, (Kp16 - k0 * 128) >> 4), items = rows * per, step = blockDim.x;
+    const W4Per div(per);
     for (int i0 = threadIdx.x; i0 < items; i0 += 4 * step) {
         v4i v[4][P];
         int at[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int i = min(i0 + b * step, items - 1), r = w4_div(i, per), c = 16 * (i - r * per);
+            const int i = min(i0 + b * step, items - 1), r = div.of(i), c = 16 * (i - r * per);
             at[b] = r * ld + c;
             const unsigned from = off(r) + unsigned(k0 * 128 + c);
             v[b][0] = *reinterpret_cast<const v4i*>(hi + from);
@@ -185,37 +195,45 @@ __device__ __forceinline__ void w4_stage(uint8_t* lds, int ld, int prows, int ro
 }
 
 // int32 rows quantised to planes in LDS, four values a thread and step, eight steps in flight: off(r) the row's offset in values (below
-// 2^28), shift(r) its shift. K % 4 == 0. `tpr` threads work on a row, so that a row's address and shift are found once: about a
-// quarter of its quads, more where the rows are too few for the block.
+// 2^28), shift(r) its shift. K % 4 == 0.
 template <class F, class S>
 __device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int K, const int32_t* x, F off, S shift) {
     constexpr int B = 8;
-    const int per = min(kc * 32, (K - k0 * 128) >> 2), threads = blockDim.x;
-    int lg = 31 - __builtin_clz(max(64, per >> 2));
-    while ((1 << lg) < threads && (threads >> lg) > rows) ++lg;
-    const int tpr = min(1 << lg, threads), side = threads / tpr;
+    const int per = min(kc * 32, (K - k0 * 128) >> 2), items = rows * per, step = blockDim.x;
+    const W4Per div(per);
     const s2 lim = {-32767, -32767};
-    for (int r = int(threadIdx.x) / tpr; r < rows; r += side) {
-        const int e = shift(r), one = e ? 1 : 0;
-        const unsigned from = off(r) + unsigned(k0 * 128);
-        // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only -32768 is
-        // left to raise
-        const auto q = [&](int w) { return (w >> e) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e - 1), unsigned(one))); };
-        for (int c0 = int(threadIdx.x) & (tpr - 1); c0 < per; c0 += B * tpr) {
-            v4i v[B];
+    for (int i0 = threadIdx.x; i0 < items; i0 += B * step) {
+        v4i v[B];
+        int at[B], e[B];
 #pragma unroll
-            for (int b = 0; b < B; ++b) v[b] = *reinterpret_cast<const v4i*>(x + (from + 4u * unsigned(min(c0 + b * tpr, per - 1))));
-#pragma unroll
-            for (int b = 0; b < B; ++b) {   // the last quad may be written more than once
-                const s2 q0 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][0]), q(v[b][1])), lim);
-                const s2 q1 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][2]), q(v[b][3])), lim);
-                const unsigned u0 = __builtin_bit_cast(unsigned, q0), u1 = __builtin_bit_cast(unsigned, q1);
-                uint8_t* to = lds + r * ld + 4 * min(c0 + b * tpr, per - 1);
-                *reinterpret_cast<unsigned*>(to) = __builtin_amdgcn_perm(u1, u0, 0x07050301u);
-                *reinterpret_cast<unsigned*>(to + prows * ld) = __builtin_amdgcn_perm(u1, u0, 0x06040200u) ^ 0x80808080u;
+        for (int b = 0; b < B; ++b) {
+            const int i = i0 + b * step, r = div.of(i), c = 4 * (i - r * per);
+            at[b] = r * ld + c;
+            if (i < items) {
+                e[b] = shift(r);
+                v[b] = *reinterpret_cast<const v4i*>(x + (off(r) + unsigned(k0 * 128 + c)));
             }
         }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (i0 + b * step >= items) continue;
+            // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only
+            // -32768 is left to raise
+            const int one = e[b] ? 1 : 0;
+            const auto q = [&](int w) { return (w >> e[b]) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e[b] - 1), unsigned(one))); };
+            const s2 q0 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][0]), q(v[b][1])), lim);
+            const s2 q1 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][2]), q(v[b][3])), lim);
+            const unsigned u0 = __builtin_bit_cast(unsigned, q0), u1 = __builtin_bit_cast(unsigned, q1);
+            *reinterpret_cast<unsigned*>(lds + at[b]) = __builtin_amdgcn_perm(u1, u0, 0x07050301u);
+            *reinterpret_cast<unsigned*>(lds + at[b] + prows * ld) = __builtin_amdgcn_perm(u1, u0, 0x06040200u) ^ 0x80808080u;
+        }
     }
+}
+
+// The gate's table in LDS: two dependent reads an output are fast there
+constexpr int W4_LUT = 2049, W4_LUT_LDS = 8208;
+__device__ __forceinline__ void w4_load_lut(int32_t* to, const int32_t* L) {
+    for (int i = threadIdx.x; i < W4_LUT; i += blockDim.x) to[i] = L[i];
 }
 
 // A wave's share of a chunk: tiles u of the segment's column tiles c = u / kc, in the order of their addresses
@@ -253,6 +271,12 @@ struct W4Ring {
     }
 };
 
+// the ring's stages once round, with their numbers known to the compiler
+template <class F, int... D>
+__device__ __forceinline__ bool w4_round(const F& step, std::integer_sequence<int, D...>) {
+    return (step(D) && ...);
+}
+
 // The wave's share: sums of column tile c, row t and column n are added to sums[(c * TR + t) * 16 + n], TR = 4 RR MT
 template <int MT, int RR, int P, int G, int DEPTH>
 __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* lds, int ld, int prows, int rows, unsigned long long* sums, int lane) {
@@ -271,32 +295,29 @@ __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* 
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < RR; ++r) acc[mt][r] = 0;
-    for (;;) {
-        bool more = true;
+    // one tile, from the ring's stage d; false after the last
+    const auto step = [&](int d) {
+        const uint8_t* a[P];
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const uint8_t* a[P];
+        for (int p = 0; p < P; ++p) a[p] = base[p] + k * 128;
+        w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc);
+        __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
+        ring.fetch(d, lane);
+        const bool last = ++u == ring.u1;
+        if (++k == ring.kc || last) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) a[p] = base[p] + k * 128;
-            w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc);
-            __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
-            ring.fetch(d, lane);
-            const bool last = ++u == ring.u1;
-            if (++k == ring.kc || last) {
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int r = 0; r < RR; ++r) {
-                        atomicAdd(&sums[(c * TR + 16 * mt + (lane >> 4) * RR + r) * 16 + (lane & 15)], (unsigned long long)acc[mt][r]);
-                        acc[mt][r] = 0;
-                    }
-                k = 0;
-                ++c;
-            }
-            if (last) { more = false; break; }
+                for (int r = 0; r < RR; ++r) {
+                    atomicAdd(&sums[(c * TR + 16 * mt + (lane >> 4) * RR + r) * 16 + (lane & 15)], (unsigned long long)acc[mt][r]);
+                    acc[mt][r] = 0;
+                }
+            k = 0;
+            ++c;
         }
-        if (!more) break;
-    }
+        return !last;
+    };
+    while (w4_round(step, std::make_integer_sequence<int, DEPTH>{})) {}
 }
 
 // The exact epilogue value of a column: acc the product, planes whether the rows carry the offset low plane
