@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     for (int c = 0;;) {
         const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);
         if constexpr (DOWN)
-            w4_stage_x32(lds, ch.ld(), n, n, k0, kc, F, a.v, [&](int r) { return unsigned(s_pair[r]) * unsigned(F); }, [&](int r) { return s_se[r]; });
+            w4_stage_x32(lds, ch.ld(), n, n, k0, kc, F, a.v, [&](int r) { return unsigned(s_pair[r]) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
         else
             w4_stage<P>(lds, ch.ld(), n, n, k0, kc, a.Kp16, a.hi, a.lo, [&](int r) { return unsigned(w4_div(s_pair[r], a.topk)) * unsigned(a.ld8); });
         __syncthreads();

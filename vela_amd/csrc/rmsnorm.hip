@@ -12,6 +12,7 @@
 // correctly rounded quotient, whose error (below 2^-13) is smaller than the 1 / C gap of a non-integer quotient to the next integer.
 #include <climits>
 
+#include "dispatch_rules.h"
 #include "norm_math.h"
 #include "vk_common.h"
 
@@ -181,12 +182,15 @@ hipError_t launch_rmsnorm_q(hipStream_t st, const int32_t* X, const int32_t* R, 
                             int32_t* e, int Kp) {
     RmsArgs a{X, R, M, C, g, H, hi, lo, e, Kp, {}};
     for (int ex = 0; ex < 13; ++ex) a.eps.v[ex] = ((1LL << (32 - 2 * ex)) + den / 2) / den;
+    // Up to 1024 values a row is a wave's; from there on a block's of 256 threads, of 1024 where wide rows are fewer than CUs (37 x 5120: 7.1 us with
+    // 256, 6.4 with 1024; narrower rows measure the same either way, and from 500 rows on 1024 threads are slower, 9.3 -> 10.6 at 500 x 4096)
     const int Q = C / 4;
     if (Q <= 64) rmsnorm_launch<64, 1>(st, a);
     else if (Q <= 128) rmsnorm_launch<64, 2>(st, a);
     else if (Q <= 256) rmsnorm_launch<64, 4>(st, a);
     else if (Q <= 512) rmsnorm_launch<256, 2>(st, a);
     else if (Q <= 1024) rmsnorm_launch<256, 4>(st, a);
+    else if (M <= NCU) rmsnorm_launch<1024, 2>(st, a);
     else rmsnorm_launch<256, 8>(st, a);
     return hipGetLastError();
 }

@@ -113,11 +113,10 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
         s_rm[threadIdx.x] = 0;
         s_e[threadIdx.x] = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     }
-    if (x32) __syncthreads();
     for (int c = 0;;) {
         const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);
         if (x32)
-            w4_stage_x32(lds, ch.ld(), prows, rows, k0, kc, a.w.K, a.x + size_t(row0) * a.ldx, [&](int r) { return unsigned(r) * unsigned(a.ldx); }, [&](int r) { return s_e[r]; });
+            w4_stage_x32(lds, ch.ld(), prows, rows, k0, kc, a.w.K, a.x + size_t(row0) * a.ldx, [&](int r) { return unsigned(r) * unsigned(a.ldx); }, [&](int r) { return rowexp_u32(a.xmax[row0 + r]); }, lane, wave, waves);
         else
             w4_stage<P>(lds, ch.ld(), prows, rows, k0, kc, a.Kp16, a.hi + size_t(row0) * a.ld8, P == 2 ? a.lo + size_t(row0) * a.ld8 : nullptr,
                         [&](int r) { return unsigned(r) * unsigned(a.ld8); });

@@ -194,38 +194,36 @@ __device__ __forceinline__ void w4_stage(uint8_t* lds, int ld, int prows, int ro
     }
 }
 
-// int32 rows quantised to planes in LDS, four values a thread and step, eight steps in flight: off(r) the row's offset in values (below
-// 2^28), shift(r) its shift. K % 4 == 0.
+// int32 rows quantised to planes in LDS, a wave eight times 64 quads of one row at once, so that the row's address and shift are
+// scalars: off(r) the row's offset in values, shift(r) its shift. K % 4 == 0.
 template <class F, class S>
-__device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int K, const int32_t* x, F off, S shift) {
+__device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int K, const int32_t* x, F off, S shift, int lane, int wave, int waves) {
     constexpr int B = 8;
-    const int per = min(kc * 32, (K - k0 * 128) >> 2), items = rows * per, step = blockDim.x;
-    const W4Per div(per);
+    const int quads = min(kc * 32, (K - k0 * 128) >> 2), blocks = (quads + 63) >> 6, parts = (blocks + B - 1) / B, items = rows * parts;
     const s2 lim = {-32767, -32767};
-    for (int i0 = threadIdx.x; i0 < items; i0 += B * step) {
+    for (int i = wave; i < items; i += waves) {
+        const int r = __builtin_amdgcn_readfirstlane(w4_div(i, parts)), b0 = (i - r * parts) * B, n = min(B, blocks - b0);
+        const int e = __builtin_amdgcn_readfirstlane(shift(r)), one = e ? 1 : 0, from = k0 * 128 + b0 * 256;
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(x + __builtin_amdgcn_readfirstlane(off(r)) + from, unsigned(K - from) * 4u);
         v4i v[B];
-        int at[B], e[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (b < n) v[b] = bload16(rs, unsigned(b * 1024 + 16 * lane));
+        // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only -32768
+        // is left to raise
+        const auto q = [&](int w) { return (w >> e) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e - 1), unsigned(one))); };
+        uint8_t* to = lds + r * ld + b0 * 256 + 4 * lane;
+        const int left = quads - b0 * 64 - lane;   // the lane's quads from here on
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            const int i = i0 + b * step, r = div.of(i), c = 4 * (i - r * per);
-            at[b] = r * ld + c;
-            if (i < items) {
-                e[b] = shift(r);
-                v[b] = *reinterpret_cast<const v4i*>(x + (off(r) + unsigned(k0 * 128 + c)));
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            if (i0 + b * step >= items) continue;
-            // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only
-            // -32768 is left to raise
-            const int one = e[b] ? 1 : 0;
-            const auto q = [&](int w) { return (w >> e[b]) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e[b] - 1), unsigned(one))); };
+            if (b >= n) continue;
             const s2 q0 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][0]), q(v[b][1])), lim);
             const s2 q1 = __builtin_elementwise_max(__builtin_amdgcn_cvt_pk_i16(q(v[b][2]), q(v[b][3])), lim);
             const unsigned u0 = __builtin_bit_cast(unsigned, q0), u1 = __builtin_bit_cast(unsigned, q1);
-            *reinterpret_cast<unsigned*>(lds + at[b]) = __builtin_amdgcn_perm(u1, u0, 0x07050301u);
-            *reinterpret_cast<unsigned*>(lds + at[b] + prows * ld) = __builtin_amdgcn_perm(u1, u0, 0x06040200u) ^ 0x80808080u;
+            if (64 * b < left) {
+                *reinterpret_cast<unsigned*>(to + 256 * b) = __builtin_amdgcn_perm(u1, u0, 0x07050301u);
+                *reinterpret_cast<unsigned*>(to + 256 * b + prows * ld) = __builtin_amdgcn_perm(u1, u0, 0x06040200u) ^ 0x80808080u;
+            }
         }
     }
 }
