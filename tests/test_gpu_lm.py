@@ -220,6 +220,13 @@ def test_w4_columns(gpu, N):
         check_w4(rng, "q16", 4, N, 256, 64, epi="geglu", ldpad=1)
 
 
+@pytest.mark.parametrize("kind,M,K,N", [("q16", 48, 5000, 40), ("q8", 64, 9000, 24), ("x32", 16, 12000, 24), ("q16", 16, 9999, 24), ("q8", 33, 20000, 16),
+                                        ("x32", 64, 4100, 40), ("q8", 7, 64, 40000), ("q16", 30, 128, 35001), ("x32", 3, 192, 33000)])
+def test_w4_chunks_and_segments(gpu, kind, M, K, N):
+    """Rows that pass the staging area in several chunks of K; blocks of several column tiles, the last ones short."""
+    check_w4(np.random.default_rng(K + N), kind, M, N, K, 64, residual=True)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_w4_extremes(gpu, kind, group):
@@ -320,6 +327,30 @@ def test_moe_layer(gpu, M, E, topk, D, F, group, renorm):
     L.run()
     torch.cuda.synchronize()
     L.check(f"{M} tokens {E} experts")
+
+
+@pytest.mark.parametrize("M,E,topk,D,F,kind", [
+    (1, 20, 16, 32, 64, "q8"), (1, 20, 16, 32, 5200, "q16"), (1, 6, 3, 5008, 36, "q8"), (1, 40, 6, 96, 1500, "q8"), (40, 2, 2, 32, 3000, "q8"),
+    (20, 2, 1, 2512, 20, "q16"), (3, 4, 2, 8208, 24, "q8"), (33, 2, 1, 6000, 16, "q8"), (300, 3, 1, 16, 8, "q8")])
+def test_moe_shapes(gpu, M, E, topk, D, F, kind):
+    """One token with many choices, rows that fit in LDS or do not; rows in several chunks; more columns than a pass of the down
+    product; row tiles of sixteen and what is left of them."""
+    L = Layer(np.random.default_rng(D + F), M, E, topk, D, F, 64, kind=kind)
+    L.run()
+    torch.cuda.synchronize()
+    L.check()
+
+
+def test_moe_one_token_given_choices(gpu):
+    rng = np.random.default_rng(15)
+    L = Layer(rng, 1, 6, 5, 48, 40, 32)
+    for idx in ([-1, -1, -1, -1, -1], [3, 3, 0, 3, 5], [7, 2, -5, 2**31 - 1, 1]):
+        di, dp = dev(np.array([idx], np.int32)), dev(np.array([[32767, -32768, 1, 0, 12345]], np.int32))
+        for residual in (True, False):
+            vm.k_moe(L.rows.A, 1, L.moe_args(residual=residual, idx=di, p=dp))
+            want = lm.moe(L.rows.q, L.rows.e, [idx], to_np(dp), L.up, L.down, L.lut, L.res if residual else None)
+            assert_equal(to_np(L.y), want, f"{idx}")
+    check_guard(L.ybuf, 48, "one token")
 
 
 @pytest.mark.parametrize("group,group2", [(32, 128), (128, 64), (64, 32)])

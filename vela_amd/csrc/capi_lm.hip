@@ -142,13 +142,12 @@ int vgemm_moe_route(void* stream, const VgemmASrc* A, int M, const VgemmMoeRoute
     return hip_status(vk::launch_moe_route(static_cast<hipStream_t>(stream), a, M), "moe_route launch");
 }
 
-// tokens one pass takes; a pass's workspace holds the plan and for each pair the row of the down product, v and the
-// maxima of v's segments
+// tokens one pass takes; a pass's workspace holds for each pair the row of the down product, v and the maxima of v's segments
 static int moe_pass(int M, int topk) { return std::min(M, vk::MOE_PAIRS / topk); }
 
 size_t vgemm_moe_workspace_bytes(int M, int topk, int F) {
     if (M <= 0 || topk < 1 || topk > vk::MOE_TOPK || F < 1) return 0;
-    return sizeof(vk::MoePlan) + size_t(moe_pass(M, topk)) * topk * (size_t(F) + vk::MOE_COLS + vk::w4_ct(2 * F)) * 4;
+    return size_t(moe_pass(M, topk)) * topk * (size_t(F) + vk::MOE_COLS + vk::w4_ct(2 * F)) * 4;
 }
 
 int vgemm_moe(void* stream, const VgemmASrc* A, int M, const VgemmMoe* P) {
@@ -177,8 +176,7 @@ int vgemm_moe(void* stream, const VgemmASrc* A, int M, const VgemmMoe* P) {
     a.Kp16 = up16(P->up.K);
     a.Lphi = P->Lphi;
     a.ldy = P->ldy;
-    a.plan = static_cast<vk::MoePlan*>(P->ws);
-    a.y = reinterpret_cast<int32_t*>(a.plan + 1);
+    a.y = static_cast<int32_t*>(P->ws);
     a.v = a.y + size_t(pass) * P->topk * vk::MOE_COLS;
     a.vmax = reinterpret_cast<uint32_t*>(a.v + size_t(pass) * P->topk * F);
     for (int t = 0; t < M; t += pass) {

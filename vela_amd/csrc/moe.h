@@ -22,16 +22,6 @@ struct RouteArgs {
     int32_t *idx, *p, *logits;
 };
 
-// The work of a pass (several tokens; of one token the choices themselves are the row tiles)
-struct MoePlan {
-    int tiles;
-    int x[MOE_PAIRS];      // row tiles of at most 16 of an expert's pairs: the expert,
-    int at[MOE_PAIRS];     // first place | rows << 16
-    int pair[MOE_PAIRS];   // the pairs in the order of their experts, those of an expert in their own
-    int pad[3];
-};
-static_assert(sizeof(MoePlan) % 16 == 0, "the workspace's parts begin at multiples of 16 bytes");
-
 struct MoeArgs {
     W4View up, down;             // of expert 0; the others follow at the strides
     size_t up_stride, down_stride;
@@ -44,7 +34,6 @@ struct MoeArgs {
     int32_t* Y;
     int ldy;
     const int32_t* R;
-    MoePlan* plan;
     int32_t* v;                  // [pairs x F]
     uint32_t* vmax;              // [pairs x up_segs]: max |v| of a segment
     int up_segs;

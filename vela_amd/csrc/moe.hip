@@ -155,61 +155,60 @@ hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
 // Both products are cut into items (row tile of at most 16 of an expert's pairs, segment of `js` column tiles), a block each,
 // which computes as w4_kernel.h says.
 
-// The pairs sorted by expert and cut into row tiles: one block
-__global__ void __launch_bounds__(256) moe_plan_kernel(MoeArgs a) {
-    __shared__ int s_cnt[MOE_EXPERTS];    // pairs of an expert, then its first place
-    __shared__ int s_rank[MOE_PAIRS];     // a pair's place among its expert's
+// Row tile `tile` of the pairs sorted by expert: its expert and rows; n = 0 past the last tile. pair[]: the tile's pairs, the same in every
+// block (in the order of the pairs), written by the first wave. Every block finds its own: a kernel that did it once took 2 to 5 us.
+struct MoeTile {
+    int x, n;
+};
+struct MoeFind {
+    int idx[MOE_PAIRS], cnt[MOE_EXPERTS];
+};
+__device__ __forceinline__ MoeTile moe_find(const MoeArgs& a, int tile, MoeFind& T, int* pair) {
     const int pairs = a.M * a.topk, lane = threadIdx.x & 63;
-    MoePlan& T = *a.plan;
-    for (int i = threadIdx.x; i < a.experts; i += 256) s_cnt[i] = 0;
+    if (a.M == 1) {   // one token: its choices are the tiles
+        const int x = a.idx[tile];
+        if (threadIdx.x == 0) pair[0] = tile;
+        return {x, unsigned(x) < unsigned(a.experts) ? 1 : 0};
+    }
+    for (int i = threadIdx.x; i < a.experts; i += blockDim.x) T.cnt[i] = 0;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        const u64 before = (u64(1) << lane) - 1;
-        for (int c = 0; c < pairs; c += 64) {
-            const unsigned x = c + lane < pairs ? unsigned(a.idx[c + lane]) : ~0u;
-            const bool have = x < unsigned(a.experts);
-            u64 same = __builtin_amdgcn_ballot_w64(have);   // lanes with the same expert: nine bits tell 512 apart
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+        const int x = a.idx[i];
+        T.idx[i] = x;
+        if (unsigned(x) < unsigned(a.experts)) atomicAdd(&T.cnt[x], 1);
+    }
+    __syncthreads();
+    const u64 before = (u64(1) << lane) - 1;
+    for (int c = 0; c < a.experts; c += 64) {
+        const int n = c + lane < a.experts ? T.cnt[c + lane] : 0, nt = (n + 15) >> 4;
+        int first = 0, all = 0;   // tiles of the lanes before, of all: bit by bit of the counts
 #pragma unroll
-            for (int bit = 1; bit < MOE_EXPERTS; bit <<= 1) {
-                const u64 m = __builtin_amdgcn_ballot_w64((x & bit) != 0);
-                same &= (x & bit) ? m : ~m;
-            }
-            if (have) {
-                const int n = s_cnt[x];
-                s_rank[c + lane] = n + __builtin_popcountll(same & before);
-                wave_lds_fence();
-                if (!(same & before)) s_cnt[x] = n + __builtin_popcountll(same);
-            }
-            wave_lds_fence();
+        for (int bit = 0; (1 << bit) <= MOE_PAIRS / 16; ++bit) {
+            const u64 m = __builtin_amdgcn_ballot_w64((nt >> bit) & 1);
+            first += __builtin_popcountll(m & before) << bit;
+            all += __builtin_popcountll(m) << bit;
         }
-        int at = 0, tiles = 0;
-        for (int c = 0; c < a.experts; c += 64) {
-            const int n = c + lane < a.experts ? s_cnt[c + lane] : 0, nt = (n + 15) >> 4;
-            int sum = n | nt << 16;   // inclusive over the lanes, both at once: at most 512 of each
-            for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(sum, d);
-                if (lane >= d) sum += o;
-            }
-            const int first = at + (sum & 0xffff) - n, tfirst = tiles + (sum >> 16) - nt;
-            for (int i = 0; i < nt; ++i) {
-                T.x[tfirst + i] = c + lane;
-                T.at[tfirst + i] = (first + 16 * i) | min(16, n - 16 * i) << 16;
-            }
-            if (n > 0) s_cnt[c + lane] = first;
-            const int all = __builtin_amdgcn_readlane(sum, 63);
-            at += all & 0xffff;
-            tiles += all >> 16;
+        if (tile >= all) {
+            tile -= all;
+            continue;
         }
-        if (lane == 0) T.tiles = tiles;
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tile >= first && tile < first + nt));
+        const int x = c + l, r0 = 16 * (tile - __builtin_amdgcn_readlane(first, l)), rows = min(16, __builtin_amdgcn_readlane(n, l) - r0);
+        if (threadIdx.x < 64) {
+            for (int i = 0, at = -r0; i < pairs; i += 64) {
+                const bool hit = i + lane < pairs && T.idx[i + lane] == x;
+                const u64 m = __builtin_amdgcn_ballot_w64(hit);
+                const int r = at + __builtin_popcountll(m & before);
+                if (hit && r >= 0 && r < rows) pair[r] = i + lane;
+                at += __builtin_popcountll(m);
+            }
+        }
+        return {x, rows};
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += 256) {
-        const unsigned x = unsigned(a.idx[i]);
-        if (x < unsigned(a.experts)) T.pair[s_cnt[x] + s_rank[i]] = i;
-    }
+    return {-1, 0};
 }
 
-constexpr int MOE_JS = 16;   // column tiles a segment has at most: 32 KiB of sums
+constexpr int MOE_JS = 24;   // column tiles a segment has at most: 48 KiB of sums
 
 // DOWN = false: rows of the tokens' planes, GEGLU to v [pairs x F], and max |v| of the segment. DOWN = true: rows v, quantised by the
 // largest of their segments' maxima, y [pairs x MOE_COLS].
@@ -219,17 +218,9 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     extern __shared__ uint4 s_dyn[];
     __shared__ uint32_t s_max[16];
     __shared__ int s_se[16], s_pair[16];
-    int x, first, n;
-    if (a.M == 1) {
-        x = a.idx[blockIdx.y];
-        first = 0;
-        n = unsigned(x) < unsigned(a.experts) ? 1 : 0;
-    } else {
-        const int w = a.plan->at[blockIdx.y];   // beside the number of tiles, not behind it: what stands there past the last is not used
-        x = a.plan->x[blockIdx.y];
-        first = w & 0xffff;
-        n = int(blockIdx.y) < a.plan->tiles ? w >> 16 : 0;
-    }
+    __shared__ MoeFind s_find;
+    const MoeTile mt = moe_find(a, blockIdx.y, s_find, s_pair);
+    const int x = __builtin_amdgcn_readfirstlane(mt.x), n = __builtin_amdgcn_readfirstlane(mt.n);
     if (n == 0) return;
     const W4View& W = DOWN ? a.down : a.up;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
@@ -254,13 +245,10 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     W4Ring<G, DEPTH> ring;
     ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
     for (int k = threadIdx.x; k < tiles * 256; k += blockDim.x) sums[k] = 0;
-    if (int(threadIdx.x) < n) {
-        const int pr = a.M == 1 ? int(blockIdx.y) : a.plan->pair[first + threadIdx.x];
-        s_pair[threadIdx.x] = pr;
-        s_max[threadIdx.x] = 0;
-        if constexpr (!DOWN) s_se[threadIdx.x] = a.e ? a.e[w4_div(pr, a.topk)] : 0;
-    }
+    if (int(threadIdx.x) < n) s_max[threadIdx.x] = 0;
     __syncthreads();
+    if constexpr (!DOWN)
+        if (int(threadIdx.x) < n) s_se[threadIdx.x] = a.e ? a.e[w4_div(s_pair[threadIdx.x], a.topk)] : 0;
     if constexpr (DOWN) {
         for (int r = wave; r < n; r += waves) {
             const uint32_t* vm = a.vmax + size_t(s_pair[r]) * a.up_segs;
@@ -314,6 +302,65 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     }
 }
 
+// Of one token: the down products of all its choices and their sum, a segment of column tiles a block. A choice has `wpc` waves; the rows
+// v stand in LDS whole, [choice][plane].
+template <int G>
+__global__ void __launch_bounds__(1024) moe_down_one_kernel(MoeArgs a, int js, int wpc, int rows_lds) {
+    constexpr int DEPTH = 6;
+    extern __shared__ uint4 s_dyn[];
+    __shared__ int s_se[MOE_TOPK], s_x[MOE_TOPK];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
+    const W4View& W = a.down;
+    const int KT = W.KT, ct0 = int(blockIdx.x) * js, tiles = min(js, W.CT - ct0), F = W.K, ld = KT * 128 + 16, k = a.topk;
+    uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
+    unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);   // [choice][column tile][4][16]: the first of the four rows
+    unsigned long long* out = sums + k * js * 64;                                           // [column]
+    const int j = __builtin_amdgcn_readfirstlane(w4_div(wave, wpc)), part = wave - j * wpc;
+    const int x = j < k ? __builtin_amdgcn_readfirstlane(a.idx[j]) : -1;
+    const bool work = unsigned(x) < unsigned(a.experts);
+    W4Ring<G, DEPTH> ring;
+    if (work) {
+        const size_t at = x * a.down_stride;
+        ring.start(W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT, tiles, 0, W4Chunks{KT, 1}, lane, part, wpc);
+    }
+    for (int i = threadIdx.x; i < k * js * 64 + js * 16; i += blockDim.x) sums[i] = 0;
+    for (int r = wave; r < k; r += waves) {
+        const uint32_t* vm = a.vmax + size_t(r) * a.up_segs;
+        uint32_t m = 0;
+        for (int i = lane; i < a.up_segs; i += 64) m = max(m, vm[i]);
+        m = wave_umax32(m);
+        if (lane == 0) {
+            s_se[r] = rowexp_u32(m);
+            s_x[r] = a.idx[r];
+        }
+    }
+    __syncthreads();
+    w4_stage_x32(lds, ld, k, k, 0, KT, F, a.v, [&](int r) { return unsigned(r) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
+    // the column's constants and the choice's share come while the rows do
+    const int items = k * tiles * 16;
+    int4 c;
+    const auto fetch = [&](int i) {
+        const int jj = w4_div(i >> 4, tiles), col = (ct0 + (i >> 4) - jj * tiles) * 16 + (i & 15);
+        c = unsigned(s_x[jj]) < unsigned(a.experts) ? W.cst[size_t(s_x[jj]) * W.CT * 16 + col] : make_int4(0, 0, 0, 0);
+    };
+    if (int(threadIdx.x) < items) fetch(threadIdx.x);
+    __syncthreads();
+    if (work) w4_share<1, 1, 2, G, DEPTH>(ring, lds + j * ld, ld, k, 1, sums + j * js * 64, lane);
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += blockDim.x) {
+        const int jj = w4_div(i >> 4, tiles), ct = (i >> 4) - jj * tiles;
+        if (i != int(threadIdx.x)) fetch(i);
+        if (unsigned(s_x[jj]) >= unsigned(a.experts)) continue;
+        const int y = w4_requant(i64(sums[(jj * js + ct) * 64 + (i & 15)]), true, c, s_se[jj]);
+        atomicAdd(&out[ct * 16 + (i & 15)], u64(i64(a.p[jj])) * u64(i64(y)));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tiles * 16; i += blockDim.x) {
+        const int col = ct0 * 16 + i;
+        if (col < W.N) a.Y[col] = add_sat(int(rshr(i64(out[i]), 15)), a.R ? a.R[col] : 0);
+    }
+}
+
 // Y[t] = sat32(sat32(rshr(sum_j p y, 15)) + R[t]) over the columns of a pass, eight choices' loads in flight
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
     const int c = int(blockIdx.x) * 256 + int(threadIdx.x), tok = blockIdx.y;
@@ -352,9 +399,14 @@ static void moe_launch(hipStream_t st, const MoeArgs& a, MoeShape sh) {
     const int CT = DOWN ? cdiv(a.cols, 16) : a.up.CT, KT = DOWN ? a.down.KT : a.up.KT, pairs = a.M * a.topk;
     const int tiles = std::min(pairs, std::min(a.experts, pairs) + pairs / 16);   // row tiles at most
     // the 64-bit sums behind the rows begin at a multiple of 16 bytes
-    const int sums = sh.js * 2048, lut = DOWN ? 0 : W4_LUT_LDS, most = (sh.waves == 16 ? 158 << 10 : 79 << 10) - sums - lut, rows = std::min(16, pairs);
+    const int sums = sh.js * 2048, lut = DOWN ? 0 : W4_LUT_LDS, fixed = int(sizeof(MoeFind)) + 256 + sums + lut, rows = std::min(16, pairs);
+    const int most = (sh.waves == 16 ? 160 << 10 : 80 << 10) - fixed;
     const int rows_lds = std::max(rows * P * 144, std::min(most & ~15, rows * P * (KT * 128 + 16)));
     hipLaunchKernelGGL((moe_kernel<DOWN, P, G>), dim3(cdiv(CT, sh.js), tiles), dim3(64 * sh.waves), rows_lds + sums + lut, st, a, sh.js, rows_lds);
+}
+template <int G>
+static void moe_down_one(hipStream_t st, const MoeArgs& a, int js, int rows_lds) {
+    hipLaunchKernelGGL((moe_down_one_kernel<G>), dim3(cdiv(a.down.CT, js)), dim3(1024), rows_lds + a.topk * js * 512 + js * 128, st, a, js, 16 / a.topk, rows_lds);
 }
 template <bool DOWN, int P>
 static void moe_product(hipStream_t st, const MoeArgs& a, int group, MoeShape sh) {
@@ -367,10 +419,17 @@ hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     MoeArgs a = args;
     const MoeShape up = moe_shape(a, a.up.CT, false);
     a.up_segs = cdiv(a.up.CT, up.js);
-    if (a.M > 1) hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(256), 0, st, a);
     if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
     else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
+    // one token, rows that fit in LDS: its choices' products and their sum at once
+    const int js1 = std::min(8, cdiv(a.down.CT, NCU)), rows1 = a.topk * 2 * (a.down.KT * 128 + 16);
+    if (a.M == 1 && rows1 + a.topk * js1 * 512 + js1 * 128 + 256 <= 160 << 10) {
+        if (a.group_down == 32) moe_down_one<32>(st, a, js1, rows1);
+        else if (a.group_down == 64) moe_down_one<64>(st, a, js1, rows1);
+        else moe_down_one<128>(st, a, js1, rows1);
+        return hipGetLastError();
+    }
     for (a.col0 = 0; a.col0 < a.down.N; a.col0 += MOE_COLS) {
         a.cols = std::min(MOE_COLS, a.down.N - a.col0);
         moe_product<true, 2>(st, a, a.group_down, moe_shape(a, cdiv(a.cols, 16), true));

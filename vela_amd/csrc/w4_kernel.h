@@ -258,9 +258,8 @@ struct W4Ring {
         k0 = chunk * ch.kc;
         kc = min(ch.kc, KT - k0);
         const int units = tiles * kc;
-        const int sh = __builtin_ctz(waves);   // a power of two
-        u0 = __builtin_amdgcn_readfirstlane((units * wave) >> sh);
-        u1 = __builtin_amdgcn_readfirstlane((units * (wave + 1)) >> sh);
+        u0 = __builtin_amdgcn_readfirstlane(w4_div(units * wave, waves));
+        u1 = __builtin_amdgcn_readfirstlane(w4_div(units * (wave + 1), waves));
         u = u0;
         c = __builtin_amdgcn_readfirstlane(w4_div(u0, kc));
         k = u0 - c * kc;
