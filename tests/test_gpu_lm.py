@@ -266,6 +266,32 @@ def test_w4_pack_parts_of_a_stack(gpu):
     assert torch.equal(whole.q, parts.q) and torch.equal(whole.cst, parts.cst)
 
 
+@pytest.mark.parametrize("N,count", [(1, 4), (1, 1), (5, 3), (5, 1)])
+def test_w4_pack_strided_sources(gpu, N, count):
+    """Slices of wider tensors, scale and zero points of different pitch, every second matrix of a stack, rows broadcast over
+    the columns, on a stream of its own: as from dense rows."""
+    rng = np.random.default_rng(17 + N)
+    w = lm.Weights(rng, N, 200, 64, count=count)
+    dense = packed(w)
+    wide = lambda a, extra: torch.nn.functional.pad(dev(a), (3, extra))[..., 3:3 + a.shape[-1]]  # noqa: E731
+    second = lambda a: torch.stack([dev(a), torch.zeros_like(dev(a))], 1).flatten(0, 1)[::2]  # noqa: E731
+    same = lambda W: torch.equal(W.q, dense.q) and torch.equal(W.cst, dense.cst)  # noqa: E731
+    st = torch.cuda.Stream()
+    for nib, sc, z, msb in ((wide(w.nib, 7), wide(w.sc, 2), wide(w.z, 5), wide(w.msb, 1)), (second(w.nib), second(w.sc), second(w.z), second(w.msb)),
+                            (wide(w.nib, 0), dev(w.sc), wide(w.z, 0), dev(w.msb))):
+        for stream in (None, st, st.cuda_stream):
+            W = vw.W4Weights(N, 200, 64, count=count)
+            W.q.zero_(), W.cst.zero_()
+            torch.cuda.synchronize()
+            W.pack(nib, sc, z, msb, stream=stream)
+            torch.cuda.synchronize()
+            assert same(W)
+    one = vw.W4Weights(N, 200, 64, count=count)
+    one.pack(dev(w.nib), dev(w.sc[..., :1, :]).expand(*w.sc.shape), None, dev(w.msb))
+    dense.pack(dev(w.nib), dev(np.broadcast_to(w.sc[..., :1, :], w.sc.shape).copy()), dev(np.full_like(w.z, 8)), dev(w.msb))
+    assert same(one)
+
+
 # ---------------------------------------------------------------- mixture of experts
 
 class Layer:
@@ -351,6 +377,42 @@ def test_moe_one_token_given_choices(gpu):
             want = lm.moe(L.rows.q, L.rows.e, [idx], to_np(dp), L.up, L.down, L.lut, L.res if residual else None)
             assert_equal(to_np(L.y), want, f"{idx}")
     check_guard(L.ybuf, 48, "one token")
+
+
+@pytest.mark.parametrize("E,topk,F", [(1, 2, 40), (2, 16, 40), (1, 3, 8208), (3, 16, 5200)])
+@pytest.mark.parametrize("M", [1, 2])
+def test_moe_more_choices_than_experts(gpu, M, E, topk, F):
+    """A caller's choices may name every expert several times."""
+    rng = np.random.default_rng(E + topk)
+    L = Layer(rng, M, E, 1, 48, F, 64)
+    idx, p = rng.integers(0, E, (M, topk)).astype(np.int32), rng.integers(-32768, 32768, (M, topk)).astype(np.int32)
+    L.topk, L.ws = topk, torch.full((vm.moe_workspace_bytes(M, topk, F) // 4,), GUARD, dtype=torch.int32, device="cuda")
+    di, dp = dev(idx), dev(p)
+    vm.k_moe(L.rows.A, M, L.moe_args(idx=di, p=dp))
+    assert_equal(to_np(L.y), lm.moe(L.rows.q, L.rows.e, idx, p, L.up, L.down, L.lut, L.res))
+
+
+@pytest.mark.parametrize("M,E,topk,D,F,group", [
+    (2, 4, 2, 4112, 36, 32), (3, 7, 5, 64, 132, 64), (16, 9, 1, 80, 100, 128), (8, 3, 2, 8208, 20, 64), (5, 64, 3, 96, 2052, 128), (2, 20, 8, 64, 5200, 32)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_moe_few_pairs(gpu, M, E, topk, D, F, group, inplace):
+    """Up to sixteen pairs: column tiles alone or several a block, waves left over, rows of Y further apart than D and Y on top of the
+    residual; rows that do not fit in LDS."""
+    rng = np.random.default_rng(M + D + F)
+    L = Layer(rng, M, E, topk, D, F, group)
+    idx, p = rng.integers(-1, E + 1, (M, topk)).astype(np.int32), rng.integers(-(2**31), 2**31, (M, topk)).astype(np.int32)
+    di, dp, ld = dev(idx), dev(p >> 14), D + 24
+    res = rng.integers(-(10**6), 10**6, (M, ld)).astype(np.int32)
+    buf, y = out32((M, ld))
+    y.copy_(dev(res))
+    apart = dev(res)
+    args = L.moe_args(idx=di, p=dp)
+    args.Y, args.ldy, args.residual = vg.ptr(y), ld, vg.ptr(y if inplace else apart)
+    vm.k_moe(L.rows.A, M, args)
+    got = to_np(y)
+    assert_equal(got[:, :D], lm.moe(L.rows.q, L.rows.e, idx, p >> 14, L.up, L.down, L.lut, res[:, :D]))
+    assert_equal(got[:, D:], res[:, D:], "cells between the rows")
+    check_guard(buf, M * ld, "few pairs")
 
 
 @pytest.mark.parametrize("group,group2", [(32, 128), (128, 64), (64, 32)])

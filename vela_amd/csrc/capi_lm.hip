@@ -53,8 +53,12 @@ vk::W4View w4_view(const VgemmW4& W) {
     return vk::W4View{q, q + size_t(CT) * KT * 1024, reinterpret_cast<const int4*>(W.cst), W.N, W.K, KT, CT};
 }
 
-// strides that keep the rows a kernel addresses with 32-bit offsets below 2^30 bytes: 512 int8 rows, 16 int32 rows
+// strides that keep the rows a kernel addresses with 32-bit offsets within 2^30 bytes: 512 int8 rows, 32 int32 rows
 constexpr int MAX_LD8 = 1 << 21, MAX_LDX = 1 << 23;
+// rows of a call: what a grid holds
+constexpr int MAX_ROWS = 1 << 20, MAX_NORM_ROWS = 1 << 23;
+
+int rows_limit(const char* what, int M, int most) { return M > most ? fail(VGEMM_ERR_UNSUPPORTED, "%s: at most %d rows a call, not %d", what, most, M) : VGEMM_OK; }
 
 int up16(int v) { return (v + 15) / 16 * 16; }
 
@@ -77,6 +81,7 @@ int vgemm_rmsnorm_q(void* stream, const int32_t* X, const int32_t* R, int M, int
     if (!X || M < 0 || !g || !hi || !e || den <= 0) return fail(VGEMM_ERR_ARG, "rmsnorm_q: bad arguments");
     if (C <= 0 || C % 4 || C > 8192) return fail(VGEMM_ERR_ARG, "rmsnorm_q: C must be a multiple of 4 and at most 8192");
     if (!aligned(X, 16) || !aligned(R, 16) || !aligned(H, 16) || !aligned(g, 16)) return fail(VGEMM_ERR_ARG, "rmsnorm_q: X, R, H and g must be 16-byte aligned");
+    if (int rc = rows_limit("rmsnorm_q", M, MAX_NORM_ROWS)) return rc;
     if (Kp < C || Kp % 4 || !aligned(hi, 4) || !aligned(lo, 4)) return fail(VGEMM_ERR_ARG, "rmsnorm_q: Kp >= C, Kp %% 4 == 0 and 4-byte aligned rows required");
     return hip_status(vk::launch_rmsnorm_q(static_cast<hipStream_t>(stream), X, R, M, C, g, den, H, hi, lo, e, Kp), "rmsnorm_q launch");
 }
@@ -101,6 +106,7 @@ int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const Vg
     if (int rc = w4_weights("w4", W)) return rc;
     if (W->count != 1) return fail(VGEMM_ERR_ARG, "w4: one matrix expected, not %d", W->count);
     if (M == 0) return ok();
+    if (int rc = rows_limit("w4", M, MAX_ROWS)) return rc;
     vk::W4Args a{};
     a.w = w4_view(*W);
     a.group = W->group;
@@ -134,6 +140,7 @@ int vgemm_moe_route(void* stream, const VgemmASrc* A, int M, const VgemmMoeRoute
     if (R->experts < 1 || R->experts > vk::MOE_EXPERTS || R->topk < 1 || R->topk > vk::MOE_TOPK || R->topk > R->experts)
         return fail(VGEMM_ERR_ARG, "moe_route: 1 <= topk <= experts, experts <= %d and topk <= %d required", vk::MOE_EXPERTS, vk::MOE_TOPK);
     if (M == 0) return ok();
+    if (int rc = rows_limit("moe_route", M, MAX_ROWS)) return rc;
     if (!R->W || !R->cst || !R->Lexp || !R->idx || !R->p || !aligned(R->W, 16) || !aligned(R->cst, 16)) return fail(VGEMM_ERR_ARG, "moe_route: W, cst (16-byte aligned), Lexp, idx and p required");
     if (A->K < 16 || A->K % 16 || A->K > 16384 || R->ldw < A->K || R->ldw % 16) return fail(VGEMM_ERR_ARG, "moe_route: K %% 16 == 0, K <= 16384, ldw >= K, ldw %% 16 == 0 required");
     if (int rc = i8_rows("moe_route", A, A->K)) return rc;

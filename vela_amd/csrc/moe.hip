@@ -64,37 +64,40 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x;
     const int8_t* hi = a.hi + size_t(t) * a.ld8;
     const int8_t* lo = a.lo ? a.lo + size_t(t) * a.ld8 : nullptr;
-    const int e = a.e ? a.e[t] : 0;
+    const int e = a.e ? a.e[t] : 0, i = threadIdx.x;
+    // on their way while the products run: the constants of expert i, entry i of the table
+    const int4 cst = i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
+    const long long ex = a.Lexp[i], ex_last = a.Lexp[EXP_N - 1];
+    static_assert(EXP_N == ROUTE_THREADS + 1, "an entry a thread, and the last");
     for (int x0 = wave * U; x0 < a.experts; x0 += ROUTE_THREADS / 64 * U) {
         int ch[U], cl[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) ch[i] = cl[i] = 0;
+        for (int u = 0; u < U; ++u) ch[u] = cl[u] = 0;
 #pragma unroll 2
         for (int k = lane * 16; k < a.K; k += 1024) {
             const v4i h = *reinterpret_cast<const v4i*>(hi + k);
             const v4i l = lo ? *reinterpret_cast<const v4i*>(lo + k) : v4i{0, 0, 0, 0};
             v4i w[U];
 #pragma unroll
-            for (int i = 0; i < U; ++i) w[i] = *reinterpret_cast<const v4i*>(a.W + size_t(min(x0 + i, a.experts - 1)) * a.ldw + k);
+            for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const v4i*>(a.W + size_t(min(x0 + u, a.experts - 1)) * a.ldw + k);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                ch[i] = dot16(h, w[i], ch[i]);
-                if (lo) cl[i] = dot16(l, w[i], cl[i]);
+            for (int u = 0; u < U; ++u) {
+                ch[u] = dot16(h, w[u], ch[u]);
+                if (lo) cl[u] = dot16(l, w[u], cl[u]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int sh = wave_sum32(ch[i]), sl = lo ? wave_sum32(cl[i]) : 0;
-            const int x = x0 + i;
+        for (int u = 0; u < U; ++u) {
+            const int sh = wave_sum32(ch[u]), sl = lo ? wave_sum32(cl[u]) : 0;
+            const int x = x0 + u;
             if (lane == 0 && x < a.experts) {
                 s_h[x] = sh;
                 s_l[x] = sl;
             }
         }
     }
-    const int i = threadIdx.x;
-    const int4 cst = i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
-    for (int k = i; k < EXP_N; k += ROUTE_THREADS) s_exp[k] = a.Lexp[k];
+    s_exp[i] = ex;
+    if (i == 0) s_exp[EXP_N - 1] = ex_last;
     if (i < 16) s_z[a.experts + i] = INT_MIN;
     __syncthreads();
     const int z = i < a.experts ? w4_requant(lo ? 256LL * s_h[i] + s_l[i] : i64(s_h[i]), lo != nullptr, cst, e) : 0;
@@ -302,29 +305,30 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     }
 }
 
-// Of one token: the down products of all its choices and their sum, a segment of column tiles a block. A choice has `wpc` waves; the rows
-// v stand in LDS whole, [choice][plane].
+// Of at most MOE_FEW pairs: all their down products and the sums over the tokens' choices, a segment of column tiles a block. A pair has
+// `wpp` waves; the rows v stand in LDS whole, [plane][pair].
+constexpr int MOE_FEW = 16;
 template <int G>
-__global__ void __launch_bounds__(1024) moe_down_one_kernel(MoeArgs a, int js, int wpc, int rows_lds) {
+__global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, int wpp, int rows_lds) {
     constexpr int DEPTH = 6;
     extern __shared__ uint4 s_dyn[];
-    __shared__ int s_se[MOE_TOPK], s_x[MOE_TOPK];
+    __shared__ int s_se[MOE_FEW], s_x[MOE_FEW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
     const W4View& W = a.down;
-    const int KT = W.KT, ct0 = int(blockIdx.x) * js, tiles = min(js, W.CT - ct0), F = W.K, ld = KT * 128 + 16, k = a.topk;
+    const int KT = W.KT, ct0 = int(blockIdx.x) * js, tiles = min(js, W.CT - ct0), F = W.K, ld = KT * 128 + 16, pairs = a.M * a.topk;
     uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
-    unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);   // [choice][column tile][4][16]: the first of the four rows
-    unsigned long long* out = sums + k * js * 64;                                           // [column]
-    const int j = __builtin_amdgcn_readfirstlane(w4_div(wave, wpc)), part = wave - j * wpc;
-    const int x = j < k ? __builtin_amdgcn_readfirstlane(a.idx[j]) : -1;
+    unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);   // [pair][column tile][4][16]: the first of the four rows
+    unsigned long long* out = sums + pairs * js * 64;                                       // [token][column]
+    const int j = __builtin_amdgcn_readfirstlane(w4_div(wave, wpp)), part = wave - j * wpp;
+    const int x = j < pairs ? __builtin_amdgcn_readfirstlane(a.idx[j]) : -1;
     const bool work = unsigned(x) < unsigned(a.experts);
     W4Ring<G, DEPTH> ring;
     if (work) {
         const size_t at = x * a.down_stride;
-        ring.start(W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT, tiles, 0, W4Chunks{KT, 1}, lane, part, wpc);
+        ring.start(W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT, tiles, 0, W4Chunks{KT, 1}, lane, part, wpp);
     }
-    for (int i = threadIdx.x; i < k * js * 64 + js * 16; i += blockDim.x) sums[i] = 0;
-    for (int r = wave; r < k; r += waves) {
+    for (int i = threadIdx.x; i < pairs * js * 64 + a.M * js * 16; i += blockDim.x) sums[i] = 0;
+    for (int r = wave; r < pairs; r += waves) {
         const uint32_t* vm = a.vmax + size_t(r) * a.up_segs;
         uint32_t m = 0;
         for (int i = lane; i < a.up_segs; i += 64) m = max(m, vm[i]);
@@ -335,9 +339,9 @@ __global__ void __launch_bounds__(1024) moe_down_one_kernel(MoeArgs a, int js, i
         }
     }
     __syncthreads();
-    w4_stage_x32(lds, ld, k, k, 0, KT, F, a.v, [&](int r) { return unsigned(r) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
-    // the column's constants and the choice's share come while the rows do
-    const int items = k * tiles * 16;
+    w4_stage_x32(lds, ld, pairs, pairs, 0, KT, F, a.v, [&](int r) { return unsigned(r) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
+    // the columns' constants come while the rows do
+    const int items = pairs * tiles * 16;
     int4 c;
     const auto fetch = [&](int i) {
         const int jj = w4_div(i >> 4, tiles), col = (ct0 + (i >> 4) - jj * tiles) * 16 + (i & 15);
@@ -345,19 +349,20 @@ __global__ void __launch_bounds__(1024) moe_down_one_kernel(MoeArgs a, int js, i
     };
     if (int(threadIdx.x) < items) fetch(threadIdx.x);
     __syncthreads();
-    if (work) w4_share<1, 1, 2, G, DEPTH>(ring, lds + j * ld, ld, k, 1, sums + j * js * 64, lane);
+    if (work) w4_share<1, 1, 2, G, DEPTH>(ring, lds + j * ld, ld, pairs, 1, sums + j * js * 64, lane);
     __syncthreads();
     for (int i = threadIdx.x; i < items; i += blockDim.x) {
         const int jj = w4_div(i >> 4, tiles), ct = (i >> 4) - jj * tiles;
         if (i != int(threadIdx.x)) fetch(i);
         if (unsigned(s_x[jj]) >= unsigned(a.experts)) continue;
         const int y = w4_requant(i64(sums[(jj * js + ct) * 64 + (i & 15)]), true, c, s_se[jj]);
-        atomicAdd(&out[ct * 16 + (i & 15)], u64(i64(a.p[jj])) * u64(i64(y)));
+        atomicAdd(&out[(w4_div(jj, a.topk) * js + ct) * 16 + (i & 15)], u64(i64(a.p[jj])) * u64(i64(y)));
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < tiles * 16; i += blockDim.x) {
-        const int col = ct0 * 16 + i;
-        if (col < W.N) a.Y[col] = add_sat(int(rshr(i64(out[i]), 15)), a.R ? a.R[col] : 0);
+    for (int i = threadIdx.x; i < a.M * js * 16; i += blockDim.x) {
+        const int tok = w4_div(i >> 4, js), ct = (i >> 4) - tok * js, col = (ct0 + ct) * 16 + (i & 15);
+        const size_t o = size_t(tok) * a.ldy + col;
+        if (ct < tiles && col < W.N) a.Y[o] = add_sat(int(rshr(i64(out[i]), 15)), a.R ? a.R[o] : 0);
     }
 }
 
@@ -388,8 +393,9 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
 struct MoeShape {
     int waves, js;
 };
+static double moe_chosen(const MoeArgs& a) { return a.experts * (1.0 - std::pow(1.0 - 1.0 / a.experts, double(a.M) * a.topk)); }   // experts, expected
 static MoeShape moe_shape(const MoeArgs& a, int CT, bool down) {
-    const double pairs = double(a.M) * a.topk, chosen = a.experts * (1.0 - std::pow(1.0 - 1.0 / a.experts, pairs)), tiles = std::max(chosen, pairs / 16);
+    const double pairs = double(a.M) * a.topk, chosen = moe_chosen(a), tiles = std::max(chosen, pairs / 16);
     const int waves = down && pairs / chosen >= 4.0 ? 16 : 8;
     return {waves, std::max(1, std::min(MOE_JS, int(std::ceil(1.1 * tiles * CT / (waves == 16 ? NCU : 2 * NCU)))))};
 }
@@ -397,7 +403,8 @@ static MoeShape moe_shape(const MoeArgs& a, int CT, bool down) {
 template <bool DOWN, int P, int G>
 static void moe_launch(hipStream_t st, const MoeArgs& a, MoeShape sh) {
     const int CT = DOWN ? cdiv(a.cols, 16) : a.up.CT, KT = DOWN ? a.down.KT : a.up.KT, pairs = a.M * a.topk;
-    const int tiles = std::min(pairs, std::min(a.experts, pairs) + pairs / 16);   // row tiles at most
+    // row tiles at most; of one token a tile a choice, also where an expert is chosen twice
+    const int tiles = a.M == 1 ? pairs : std::min(pairs, std::min(a.experts, pairs) + pairs / 16);
     // the 64-bit sums behind the rows begin at a multiple of 16 bytes
     const int sums = sh.js * 2048, lut = DOWN ? 0 : W4_LUT_LDS, fixed = int(sizeof(MoeFind)) + 256 + sums + lut, rows = std::min(16, pairs);
     const int most = (sh.waves == 16 ? 160 << 10 : 80 << 10) - fixed;
@@ -405,8 +412,9 @@ static void moe_launch(hipStream_t st, const MoeArgs& a, MoeShape sh) {
     hipLaunchKernelGGL((moe_kernel<DOWN, P, G>), dim3(cdiv(CT, sh.js), tiles), dim3(64 * sh.waves), rows_lds + sums + lut, st, a, sh.js, rows_lds);
 }
 template <int G>
-static void moe_down_one(hipStream_t st, const MoeArgs& a, int js, int rows_lds) {
-    hipLaunchKernelGGL((moe_down_one_kernel<G>), dim3(cdiv(a.down.CT, js)), dim3(1024), rows_lds + a.topk * js * 512 + js * 128, st, a, js, 16 / a.topk, rows_lds);
+static void moe_down_few(hipStream_t st, const MoeArgs& a, int js, int rows_lds) {
+    const int pairs = a.M * a.topk;
+    hipLaunchKernelGGL((moe_down_few_kernel<G>), dim3(cdiv(a.down.CT, js)), dim3(1024), rows_lds + pairs * js * 512 + a.M * js * 128, st, a, js, 16 / pairs, rows_lds);
 }
 template <bool DOWN, int P>
 static void moe_product(hipStream_t st, const MoeArgs& a, int group, MoeShape sh) {
@@ -422,12 +430,14 @@ hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
     else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
-    // one token, rows that fit in LDS: its choices' products and their sum at once
-    const int js1 = std::min(8, cdiv(a.down.CT, NCU)), rows1 = a.topk * 2 * (a.down.KT * 128 + 16);
-    if (a.M == 1 && rows1 + a.topk * js1 * 512 + js1 * 128 + 256 <= 160 << 10) {
-        if (a.group_down == 32) moe_down_one<32>(st, a, js1, rows1);
-        else if (a.group_down == 64) moe_down_one<64>(st, a, js1, rows1);
-        else moe_down_one<128>(st, a, js1, rows1);
+    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 11.6 against 13.3 + 4.7 us. A pair
+    // reads its expert's matrix by itself: not where that is more than 64 MB beyond a read each of the chosen experts (16 pairs of 2
+    // experts: 4096 x 1536, 44 MB, 14.1 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
+    const int pairs = a.M * a.topk, js = std::min(8, cdiv(a.down.CT, NCU)), rows = pairs * 2 * (a.down.KT * 128 + 16);
+    if (pairs <= MOE_FEW && rows + pairs * js * 512 + a.M * js * 128 + 256 <= 160 << 10 && (pairs - moe_chosen(a)) * double(a.down_stride) <= 64e6) {
+        if (a.group_down == 32) moe_down_few<32>(st, a, js, rows);
+        else if (a.group_down == 64) moe_down_few<64>(st, a, js, rows);
+        else moe_down_few<128>(st, a, js, rows);
         return hipGetLastError();
     }
     for (a.col0 = 0; a.col0 < a.down.N; a.col0 += MOE_COLS) {

@@ -38,27 +38,28 @@ class W4Weights:
         strides may be larger than the rows."""
         N, groups = self.N, (self.K + self.group - 1) // self.group
         n = nib.shape[0] if nib.dim() == 3 else 1
+        # from one row to the next, over all matrices
+        pitch = lambda t: t.stride(-2) if N > 1 else (t.stride(0) if n > 1 else t.shape[-1])  # noqa: E731
 
         def rows(t, dtypes, width, name):
             shape = (n, N) if nib.dim() == 3 else (N,)
             if t.dtype not in dtypes or t.dim() != nib.dim() or tuple(t.shape[:-1]) != shape or t.shape[-1] < width or t.device != self.q.device:
                 raise ValueError(f"W4Weights.pack: {name} of shape {tuple(t.shape)}, {t.dtype} on {t.device}")
-            t = t if t.stride(-1) == 1 else t.contiguous()
-            if t.dim() == 3 and n > 1 and t.stride(0) != N * t.stride(1):
+            if t.stride(-1) != 1 or pitch(t) < t.shape[-1] or (n > 1 and t.stride(0) != N * pitch(t)):
                 t = t.contiguous()
             return t
 
-        nib = rows(nib, (torch.uint8,), (self.K + 1) // 2, "nib")
-        scale = rows(scale, (torch.int16, torch.uint16), groups, "scale")
-        zero = rows(zero, (torch.uint8,), groups, "zero") if zero is not None else None
-        if zero is not None and N > 1 and zero.stride(-2) != scale.stride(-2):
-            scale, zero = scale.contiguous(), zero.contiguous()
-            if zero.shape[-1] != scale.shape[-1]:
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream)
+        with torch.cuda.stream(stream):   # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
+            nib = rows(nib, (torch.uint8,), (self.K + 1) // 2, "nib")
+            scale = rows(scale, (torch.int16, torch.uint16), groups, "scale")
+            zero = rows(zero, (torch.uint8,), groups, "zero") if zero is not None else None
+            if zero is not None and pitch(zero) != pitch(scale):
                 scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
-        msb = rows(msb, (torch.int32,), 4, "msb")[..., :4].contiguous()
-        ld = lambda t, least: t.stride(-2) if N > 1 else max(t.shape[-1], least)  # noqa: E731
-        check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), ld(nib, 1), ptr(scale), ptr(zero), ld(scale, 1),
-                                   ptr(msb)))
+            msb = rows(msb, (torch.int32,), 4, "msb")[..., :4].contiguous()
+            check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
+                                       ptr(msb)))
 
 
 def k_gemm_w4(A: ASrc, M: int, W: W4Weights | W4, E: AEpi, stream=None) -> None:
