@@ -211,6 +211,14 @@ __device__ __forceinline__ MoeTile moe_find(const MoeArgs& a, int tile, MoeFind&
     return {-1, 0};
 }
 
+// the shift of pair pr's row v: of the largest of its segments' maxima
+__device__ __forceinline__ int moe_shift(const MoeArgs& a, int pr, int lane) {
+    const uint32_t* vm = a.vmax + size_t(pr) * a.up_segs;
+    uint32_t m = 0;
+    for (int k = lane; k < a.up_segs; k += 64) m = max(m, vm[k]);
+    return rowexp_u32(wave_umax32(m));
+}
+
 constexpr int MOE_JS = 24;   // column tiles a segment has at most: 48 KiB of sums
 
 // DOWN = false: rows of the tokens' planes, GEGLU to v [pairs x F], and max |v| of the segment. DOWN = true: rows v, quantised by the
@@ -252,20 +260,15 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     __syncthreads();
     if constexpr (!DOWN)
         if (int(threadIdx.x) < n) s_se[threadIdx.x] = a.e ? a.e[w4_div(s_pair[threadIdx.x], a.topk)] : 0;
-    if constexpr (DOWN) {
-        for (int r = wave; r < n; r += waves) {
-            const uint32_t* vm = a.vmax + size_t(s_pair[r]) * a.up_segs;
-            uint32_t m = 0;
-            for (int k = lane; k < a.up_segs; k += 64) m = max(m, vm[k]);
-            m = wave_umax32(m);
-            if (lane == 0) s_se[r] = rowexp_u32(m);
-        }
-        __syncthreads();
-    }
+    [[maybe_unused]] const auto shift = [&](int r) {
+        const int e = moe_shift(a, s_pair[r], lane);
+        if (lane == 0) s_se[r] = e;
+        return e;
+    };
     for (int c = 0;;) {
         const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);
         if constexpr (DOWN)
-            w4_stage_x32(lds, ch.ld(), n, n, k0, kc, F, a.v, [&](int r) { return unsigned(s_pair[r]) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
+            w4_stage_x32(lds, ch.ld(), n, n, k0, kc, F, a.v, [&](int r) { return unsigned(s_pair[r]) * unsigned(F); }, [&](int r) { return c ? s_se[r] : shift(r); }, lane, wave, waves);
         else
             w4_stage<P>(lds, ch.ld(), n, n, k0, kc, a.Kp16, a.hi, a.lo, [&](int r) { return unsigned(w4_div(s_pair[r], a.topk)) * unsigned(a.ld8); });
         __syncthreads();
@@ -328,19 +331,15 @@ __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, i
         ring.start(W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT, tiles, 0, W4Chunks{KT, 1}, lane, part, wpp);
     }
     for (int i = threadIdx.x; i < pairs * js * 64 + a.M * js * 16; i += blockDim.x) sums[i] = 0;
-    for (int r = wave; r < pairs; r += waves) {
-        const uint32_t* vm = a.vmax + size_t(r) * a.up_segs;
-        uint32_t m = 0;
-        for (int i = lane; i < a.up_segs; i += 64) m = max(m, vm[i]);
-        m = wave_umax32(m);
-        if (lane == 0) {
-            s_se[r] = rowexp_u32(m);
-            s_x[r] = a.idx[r];
-        }
-    }
+    if (int(threadIdx.x) < pairs) s_x[threadIdx.x] = a.idx[threadIdx.x];
+    const auto shift = [&](int r) {
+        const int e = moe_shift(a, r, lane);
+        if (lane == 0) s_se[r] = e;
+        return e;
+    };
+    w4_stage_x32(lds, ld, pairs, pairs, 0, KT, F, a.v, [&](int r) { return unsigned(r) * unsigned(F); }, shift, lane, wave, waves);
     __syncthreads();
-    w4_stage_x32(lds, ld, pairs, pairs, 0, KT, F, a.v, [&](int r) { return unsigned(r) * unsigned(F); }, [&](int r) { return s_se[r]; }, lane, wave, waves);
-    // the columns' constants come while the rows do
+    // the columns' constants come while the products run
     const int items = pairs * tiles * 16;
     int4 c;
     const auto fetch = [&](int i) {
@@ -348,7 +347,6 @@ __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, i
         c = unsigned(s_x[jj]) < unsigned(a.experts) ? W.cst[size_t(s_x[jj]) * W.CT * 16 + col] : make_int4(0, 0, 0, 0);
     };
     if (int(threadIdx.x) < items) fetch(threadIdx.x);
-    __syncthreads();
     if (work) w4_share<1, 1, 2, G, DEPTH>(ring, lds + j * ld, ld, pairs, 1, sums + j * js * 64, lane);
     __syncthreads();
     for (int i = threadIdx.x; i < items; i += blockDim.x) {
@@ -430,9 +428,9 @@ hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
     else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
-    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 11.6 against 13.3 + 4.7 us. A pair
+    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 9.8 against 13.3 + 4.7 us. A pair
     // reads its expert's matrix by itself: not where that is more than 64 MB beyond a read each of the chosen experts (16 pairs of 2
-    // experts: 4096 x 1536, 44 MB, 14.1 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
+    // experts: 4096 x 1536, 44 MB, 12.3 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
     const int pairs = a.M * a.topk, js = std::min(8, cdiv(a.down.CT, NCU)), rows = pairs * 2 * (a.down.KT * 128 + 16);
     if (pairs <= MOE_FEW && rows + pairs * js * 512 + a.M * js * 128 + 256 <= 160 << 10 && (pairs - moe_chosen(a)) * double(a.down_stride) <= 64e6) {
         if (a.group_down == 32) moe_down_few<32>(st, a, js, rows);

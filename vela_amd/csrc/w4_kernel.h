@@ -195,7 +195,7 @@ __device__ __forceinline__ void w4_stage(uint8_t* lds, int ld, int prows, int ro
 }
 
 // int32 rows quantised to planes in LDS, a wave eight times 64 quads of one row at once, so that the row's address and shift are
-// scalars: off(r) the row's offset in values, shift(r) its shift. K % 4 == 0.
+// scalars: off(r) the row's offset in values, shift(r) its shift, asked for when the values are on their way. K % 4 == 0.
 template <class F, class S>
 __device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, int rows, int k0, int kc, int K, const int32_t* x, F off, S shift, int lane, int wave, int waves) {
     constexpr int B = 8;
@@ -203,12 +203,14 @@ __device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, in
     const s2 lim = {-32767, -32767};
     for (int i = wave; i < items; i += waves) {
         const int r = __builtin_amdgcn_readfirstlane(w4_div(i, parts)), b0 = (i - r * parts) * B, n = min(B, blocks - b0);
-        const int e = __builtin_amdgcn_readfirstlane(shift(r)), one = e ? 1 : 0, from = k0 * 128 + b0 * 256;
+        const int from = k0 * 128 + b0 * 256;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(x + __builtin_amdgcn_readfirstlane(off(r)) + from, unsigned(K - from) * 4u);
         v4i v[B];
 #pragma unroll
         for (int b = 0; b < B; ++b)
             if (b < n) v[b] = bload16(rs, unsigned(b * 1024 + 16 * lane));
+        __builtin_amdgcn_sched_barrier(0);
+        const int e = __builtin_amdgcn_readfirstlane(shift(r)), one = e ? 1 : 0;
         // quant16_32 of a value: (v >> e) + bit e - 1 of v; the conversion of pairs to 16 bits clamps the upper end, and only -32768
         // is left to raise
         const auto q = [&](int w) { return (w >> e) + int(__builtin_amdgcn_ubfe(unsigned(w), unsigned(e - 1), unsigned(one))); };
