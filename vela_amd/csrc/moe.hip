@@ -240,7 +240,6 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
     unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
     int32_t* lut = reinterpret_cast<int32_t*>(sums + js * 256);   // of the gate
-    if constexpr (!DOWN) w4_load_lut(lut, a.Lphi);
     const size_t at = x * (DOWN ? a.down_stride : a.up_stride);
     const uint8_t* q = W.q + at + size_t(ct0) * KT * 1024;
     const uint8_t* s = W.s + at + size_t(ct0) * KT * (4096 / G);
@@ -257,6 +256,7 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
     for (int k = threadIdx.x; k < tiles * 256; k += blockDim.x) sums[k] = 0;
     if (int(threadIdx.x) < n) s_max[threadIdx.x] = 0;
+    if constexpr (!DOWN) w4_load_lut(lut, a.Lphi, lane, wave, waves);
     __syncthreads();
     if constexpr (!DOWN)
         if (int(threadIdx.x) < n) s_se[threadIdx.x] = a.e ? a.e[w4_div(s_pair[threadIdx.x], a.topk)] : 0;

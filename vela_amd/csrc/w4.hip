@@ -106,12 +106,14 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     const uint8_t* s = a.w.s + size_t(ct0) * KT * (4096 / G);
     const bool x32 = P == 2 && a.x;
     W4Ring<G, DEPTH> ring;
-    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    int e = 0;   // of row threadIdx.x, asked for before the tiles so that nobody waits for those
+    if (int(threadIdx.x) < rows) e = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     for (int i = threadIdx.x; i < tiles * TR * 16; i += blockDim.x) sums[i] = 0;
-    if (a.geglu) w4_load_lut(lut, a.Lphi);
+    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    if (a.geglu) w4_load_lut(lut, a.Lphi, lane, wave, waves);
     if (int(threadIdx.x) < rows) {
         s_rm[threadIdx.x] = 0;
-        s_e[threadIdx.x] = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
+        s_e[threadIdx.x] = e;
     }
     for (int c = 0;;) {
         const int k0 = c * ch.kc, kc = min(ch.kc, KT - k0);

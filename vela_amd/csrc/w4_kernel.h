@@ -20,8 +20,6 @@
 // waves, which stream them with DEPTH tiles in flight and add each column tile's sums to 64-bit integers in LDS; the epilogue
 // reads those. Integer sums: their order does not matter.
 #pragma once
-#include <utility>
-
 #include "vk_common.h"
 
 namespace vk {
@@ -41,19 +39,18 @@ typedef unsigned u2v __attribute__((ext_vector_type(2)));
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
 // One tile as a lane holds it: its 32 nibbles and the group words of its column n = lane & 15. Loaded through buffer resources made
-// from scalars, so that the lane offsets never change and no 64-bit address stands in vector registers; where `valid` is
-// not set nothing is fetched and the words are 0.
+// from scalars, so that the lane offsets never change and no 64-bit address stands in vector registers.
 template <int G>
 struct W4Tile {
     static constexpr int NG = 128 / G;
     u4v w;
     unsigned own[(NG + 1) / 2];
-    __device__ __forceinline__ void load(const uint8_t* q, const uint8_t* s, bool valid, int lane) {
-        const __amdgpu_buffer_rsrc_t rq = make_rsrc(q, valid ? 1024u : 0u), rs = make_rsrc(s, valid ? 32u * NG : 0u);
+    __device__ __forceinline__ void load(const uint8_t* q, const uint8_t* s, int lane) {
+        const __amdgpu_buffer_rsrc_t rq = make_rsrc(q, 1024u), rs = make_rsrc(s, 32u * NG);
         w = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rq, 16 * lane, 0, 0));
         const int so = (lane & 15) * NG * 2;
-        if constexpr (NG == 1) {
-            own[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, so, 0, 0);
+        if constexpr (NG == 1) {   // both columns of a pair: a 16-bit load is widened where it ends, which would wait for the newest of them
+            own[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, so & ~3, 0, 0);
         } else if constexpr (NG == 2) {
             own[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0);
         } else {
@@ -61,12 +58,13 @@ struct W4Tile {
             own[0] = o.x; own[1] = o.y;
         }
     }
-    // 0x80 - zero point of group g, in every byte
-    __device__ __forceinline__ unsigned zero(int g) const {
-        const unsigned z = (g & 1) ? own[g >> 1] >> 28 : (own[g >> 1] >> 12) & 15u;
-        return 0x80808080u - z * 0x01010101u;
+    // the word of group g begins at bit 0 or 16 of own[g / 2]
+    __device__ __forceinline__ unsigned bits(int g, int lane, int from, int n) const {
+        return __builtin_amdgcn_ubfe(own[g >> 1], unsigned((NG == 1 ? 16 * (lane & 1) : 16 * (g & 1)) + from), unsigned(n));
     }
-    __device__ __forceinline__ int scale(int g) const { return int((g & 1) ? (own[g >> 1] >> 16) & 0xfffu : own[g >> 1] & 0xfffu); }
+    // 0x80 - zero point of group g, in every byte
+    __device__ __forceinline__ unsigned zero(int g, int lane) const { return 0x80808080u - bits(g, lane, 12, 4) * 0x01010101u; }
+    __device__ __forceinline__ int scale(int g, int lane) const { return int(bits(g, lane, 0, 12)); }
 };
 
 // the low (h = 0) or high nibbles of a word as signed bytes u - z: no byte of u + (0x80 - z) carries into the next, and
@@ -84,7 +82,7 @@ __device__ __forceinline__ int w4_row(int i) { return (i >> 2) * RR + (i & (RR -
 // acc[mt][r] += the tile's product for column lane & 15 and the rows above, rows from LDS: a[p] + mt_stride mt is the lane's row of
 // plane p at the tile's first value and the lane's part of it
 template <int MT, int RR, int P, int G>
-__device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const (&a)[P], int mt_stride, i64 (&acc)[MT][RR]) {
+__device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const (&a)[P], int mt_stride, i64 (&acc)[MT][RR], int lane) {
     constexpr int NG = 128 / G;
     const v4i zero4 = {0, 0, 0, 0};
     v4i c[MT][P];
@@ -92,12 +90,12 @@ __device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const
     for (int h = 0; h < 2; ++h) {
         int b[4];
         if constexpr (G == 32) {
-            const unsigned z0 = t.zero(2 * h), z1 = t.zero(2 * h + 1);
+            const unsigned z0 = t.zero(2 * h, lane), z1 = t.zero(2 * h + 1, lane);
             b[0] = w4_spread(t.w.x, h, z0); b[1] = w4_spread(t.w.y, h, z0);
             b[2] = w4_spread(t.w.z, h, z1); b[3] = w4_spread(t.w.w, h, z1);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int g = 2 * h + i, sc = t.scale(g);
+                const int g = 2 * h + i, sc = t.scale(g, lane);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -112,7 +110,7 @@ __device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const
                     for (int r = 0; r < RR; ++r) acc[mt][r] += i64(P == 2 ? c[mt][0][r] * 256 + c[mt][P - 1][r] : c[mt][0][r]) * sc;
             }
         } else {
-            const unsigned z = t.zero(NG == 2 ? h : 0);
+            const unsigned z = t.zero(NG == 2 ? h : 0, lane);
             b[0] = w4_spread(t.w.x, h, z); b[1] = w4_spread(t.w.y, h, z);
             b[2] = w4_spread(t.w.z, h, z); b[3] = w4_spread(t.w.w, h, z);
             const v4i bv = {b[0], b[1], b[2], b[3]};
@@ -123,7 +121,7 @@ __device__ __forceinline__ void w4_tile(const W4Tile<G>& t, const uint8_t* const
                     c[mt][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(a[p] + mt * mt_stride + 64 * h), bv, (NG == 1 && h) ? c[mt][p] : zero4, 0, 0, 0);
             }
             if (NG == 2 || h == 1) {
-                const int sc = t.scale(NG == 2 ? h : 0);
+                const int sc = t.scale(NG == 2 ? h : 0, lane);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -230,10 +228,13 @@ __device__ __forceinline__ void w4_stage_x32(uint8_t* lds, int ld, int prows, in
     }
 }
 
-// The gate's table in LDS: two dependent reads an output are fast there
-constexpr int W4_LUT = 2049, W4_LUT_LDS = 8208;
-__device__ __forceinline__ void w4_load_lut(int32_t* to, const int32_t* L) {
-    for (int i = threadIdx.x; i < W4_LUT; i += blockDim.x) to[i] = L[i];
+// The gate's table in LDS, where two dependent reads an output are fast: 64 entries a wave and step straight from memory, with nobody
+// waiting for them (through registers they held the rows' staging up). Zeros behind the last entry.
+constexpr int W4_LUT = 2049, W4_LUT_STEPS = (W4_LUT + 63) / 64, W4_LUT_LDS = W4_LUT_STEPS * 256;
+__device__ __forceinline__ void w4_load_lut(int32_t* to, const int32_t* L, int lane, int wave, int waves) {
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(L, W4_LUT * 4u);
+    for (int i = wave; i < W4_LUT_STEPS; i += waves)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + 64 * i), 4, 4 * lane, 256 * i, 0, 0);
 }
 
 // A wave's share of a chunk: tiles u of the segment's column tiles c = u / kc, in the order of their addresses
@@ -243,11 +244,10 @@ struct W4Ring {
     const uint8_t *q, *s;      // of the segment's first column tile
     int KT, k0, kc;
     int u0, u1;                // the wave's tiles
-    int u, c, k;               // the tile loaded next
+    int c, k;                  // the tile loaded next
     __device__ __forceinline__ void fetch(int d, int lane) {
         const size_t tile = size_t(c) * KT + k0 + k;
-        t[d].load(q + tile * 1024, s + tile * (4096 / G), u < u1, lane);
-        ++u;
+        t[d].load(q + tile * 1024, s + tile * (4096 / G), lane);
         if (++k == kc) {
             k = 0;
             ++c;
@@ -262,19 +262,13 @@ struct W4Ring {
         const int units = tiles * kc;
         u0 = __builtin_amdgcn_readfirstlane(w4_div(units * wave, waves));
         u1 = __builtin_amdgcn_readfirstlane(w4_div(units * (wave + 1), waves));
-        u = u0;
         c = __builtin_amdgcn_readfirstlane(w4_div(u0, kc));
         k = u0 - c * kc;
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) fetch(d, lane);
+        for (int d = 0; d < DEPTH; ++d)
+            if (u0 + d < u1) fetch(d, lane);
     }
 };
-
-// the ring's stages once round, with their numbers known to the compiler
-template <class F, int... D>
-__device__ __forceinline__ bool w4_round(const F& step, std::integer_sequence<int, D...>) {
-    return (step(D) && ...);
-}
 
 // The wave's share: sums of column tile c, row t and column n are added to sums[(c * TR + t) * 16 + n], TR = 4 RR MT
 template <int MT, int RR, int P, int G, int DEPTH>
@@ -294,15 +288,11 @@ __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* 
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < RR; ++r) acc[mt][r] = 0;
-    // one tile, from the ring's stage d; false after the last
-    const auto step = [&](int d) {
+    const auto step = [&](int d, bool last) {
         const uint8_t* a[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) a[p] = base[p] + k * 128;
-        w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc);
-        __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
-        ring.fetch(d, lane);
-        const bool last = ++u == ring.u1;
+        w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc, lane);
         if (++k == ring.kc || last) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -314,9 +304,28 @@ __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* 
             k = 0;
             ++c;
         }
-        return !last;
+        __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
     };
-    while (w4_round(step, std::make_integer_sequence<int, DEPTH>{})) {}
+    // Rounds of the ring that use and refill every stage, so that the compiler counts the loads in flight and waits for one tile at
+    // a time; then the rest, where a load may be left out and it waits for all of a round. (Refilling past the last tile instead, with loads
+    // that fetch nothing, cost 1 us of 4.6 for 1 x 2048 x 2048.)
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the first tiles are here, the rows' staging waited for younger loads
+    for (; u + 2 * DEPTH <= ring.u1; u += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            step(d, false);
+            ring.fetch(d, lane);
+        }
+    }
+    for (; u < ring.u1; u += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (u + d < ring.u1) {
+                step(d, u + d + 1 == ring.u1);
+                if (u + d + DEPTH < ring.u1) ring.fetch(d, lane);
+            }
+        }
+    }
 }
 
 // The exact epilogue value of a column: acc the product, planes whether the rows carry the offset low plane
