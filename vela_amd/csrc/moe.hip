@@ -225,7 +225,7 @@ constexpr int MOE_JS = 24;   // column tiles a segment has at most: 48 KiB of su
 // largest of their segments' maxima, y [pairs x MOE_COLS].
 template <bool DOWN, int P, int G>
 __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_lds) {
-    constexpr int DEPTH = 6;
+    constexpr int DEPTH = DOWN ? 6 : 4;   // 2 experts, 8 tokens, 4096 x 4480: up 13.3 us with 6, 12.6 with 4; down 27.6 against 28.5 for 43 tokens with 6
     extern __shared__ uint4 s_dyn[];
     __shared__ uint32_t s_max[16];
     __shared__ int s_se[16], s_pair[16];
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
 constexpr int MOE_FEW = 16;
 template <int G>
 __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, int wpp, int rows_lds) {
-    constexpr int DEPTH = 6;
+    constexpr int DEPTH = 6;   // one token, 4096 x 1536: 5.8 us, 8.5 with 4
     extern __shared__ uint4 s_dyn[];
     __shared__ int s_se[MOE_FEW], s_x[MOE_FEW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
