@@ -67,7 +67,7 @@ int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const Vg
  * (K = A->K columns, ldw >= K, ldw % 16 == 0) and cst {m, s, b, wsum}; idx [M x topk] = the topk largest, in falling order, equal
  * ones by their index; p [M x topk] their shares in Q15: E_x = lutexp(max z - z[x]) by the attention's exp table Lexp (1025 entries in [0, 2^31)),
  * r = floor(2^62 / sum E) over the chosen (renorm != 0) or all experts, p = min(32767, (E r + 2^46) >> 47). logits [M x experts]
- * may be NULL (p = 0 where sum E = 0). experts <= 512, topk <= 16, topk <= experts, K % 16 == 0, K <= 16384, M <= 2^20. */
+ * may be NULL; given, it lets the logits of a layer above 256 KiB of weights be computed by many CUs (p = 0 where sum E = 0). experts <= 512, topk <= 16, topk <= experts, K % 16 == 0, K <= 16384, M <= 2^20. */
 typedef struct VgemmMoeRoute {
     const int8_t* W; int ldw; const int32_t* cst;
     int experts, topk, renorm;

@@ -355,6 +355,42 @@ def test_moe_layer(gpu, M, E, topk, D, F, group, renorm):
     L.check(f"{M} tokens {E} experts")
 
 
+@pytest.mark.parametrize("kind", ["q8", "q16"])
+@pytest.mark.parametrize("M,E,topk,K", [(1, 1, 1, 16), (2, 16, 16, 48), (1, 65, 3, 4048), (3, 128, 16, 32), (2, 129, 16, 32), (1, 130, 1, 2032), (5, 256, 8, 1040),
+                                        (9, 257, 7, 1024), (1, 384, 16, 5008), (2, 512, 16, 64), (4, 512, 10, 16384), (6, 511, 2, 528)])
+def test_route(gpu, M, E, topk, K, kind):
+    """With the logits and without, ordinary ones, and ones that saturate at either end or are few different values: the lowest
+    indices first."""
+    rng = np.random.default_rng(E * 17 + M)
+    rows = Rows(rng, kind, M, K, pad=16)
+    w = rng.integers(-127, 128, (E, K + 32)).astype(np.int8)
+    lexp = lm.exp_table()
+    for what in ("plain", "saturated", "steps"):
+        cst = np.zeros((E, 4), np.int32)
+        cst[:, 0], cst[:, 1] = rng.integers(1 << 14, 1 << 15, E), 22 + (8 if kind == "q16" else 0)
+        cst[:, 2] = rng.integers(-9000, 9000, E)
+        if what == "saturated":
+            cst[:, 2] = rng.choice(np.array([-(2**31), 2**31 - 1], np.int64), E, p=[0.9, 0.1] if M % 2 else [1.0, 0.0])
+            cst[:, 0] = 0
+        elif what == "steps":
+            cst[:, 0], cst[:, 2] = 0, rng.integers(-2, 3, E) * 30000
+        cst[:, 3] = w[:, :K].sum(1, dtype=np.int64)
+        dw, dc, dl = dev(w), dev(cst), dev(lexp)
+        for renorm in (0, 1):
+            idx, p, z = lm.route(rows.q, rows.e, w[:, :K], cst, topk, bool(renorm), lexp)
+            for logits in (False, True):
+                di, dp = (torch.full((M, topk), -7, dtype=torch.int32, device="cuda") for _ in range(2))
+                buf, dz = out32((M, E))
+                R = vm.MoeRoute(W=vg.ptr(dw), ldw=K + 32, cst=vg.ptr(dc), experts=E, topk=topk, renorm=renorm, Lexp=vg.ptr(dl), idx=vg.ptr(di), p=vg.ptr(dp),
+                                logits=vg.ptr(dz) if logits else None)
+                vm.k_moe_route(rows.A, M, R)
+                assert_equal(to_np(di), idx, what + " idx")
+                assert_equal(to_np(dp), p, what + " p")
+                if logits:
+                    assert_equal(to_np(dz), z, what + " logits")
+                check_guard(buf, M * E, what)
+
+
 @pytest.mark.parametrize("M,E,topk,D,F,kind", [
     (1, 20, 16, 32, 64, "q8"), (1, 20, 16, 32, 5200, "q16"), (1, 6, 3, 5008, 36, "q8"), (1, 40, 6, 96, 1500, "q8"), (40, 2, 2, 32, 3000, "q8"),
     (20, 2, 1, 2512, 20, "q16"), (3, 4, 2, 8208, 24, "q8"), (33, 2, 1, 6000, 16, "q8"), (300, 3, 1, 16, 8, "q8")])

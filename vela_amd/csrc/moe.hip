@@ -34,6 +34,8 @@ __device__ __forceinline__ int dot16(const v4i& a, const v4i& b, int c) {
 
 constexpr int ROUTE_THREADS = 1024;
 constexpr int EXP_N = 1025;
+constexpr int ROUTE_RANK = ROUTE_THREADS / 8;   // experts whose places are counted by all threads: 512 took 12 us so, 16 choices 2
+constexpr int ROUTE_ONE = 1 << 18;   // bytes of weights one block a token reads
 
 // sum over the wave of values whose total stays below 2^63
 __device__ __forceinline__ i64 wave_sum64(i64 v) {
@@ -54,7 +56,46 @@ __device__ __forceinline__ u64 route_recip(u64 s) {
     return r >= i64(s) ? q + 1 : q;
 }
 
-// A block per token; a wave reads U experts at once. Plane sums stay below 16384 * 2^14 = 2^28.
+// Logits of T tokens and eight experts a block, two a wave. Plane sums stay below 16384 * 2^14 = 2^28.
+constexpr int LOGITS_X = 8;
+template <int T>
+__global__ void __launch_bounds__(256) moe_logits_kernel(RouteArgs a, int M) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x0 = int(blockIdx.x) * LOGITS_X + 2 * wave, t0 = int(blockIdx.y) * T;
+    if (x0 >= a.experts) return;
+    int ch[T][2], cl[T][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t) ch[t][0] = ch[t][1] = cl[t][0] = cl[t][1] = 0;
+    const int8_t *w0 = a.W + size_t(x0) * a.ldw, *w1 = a.W + size_t(min(x0 + 1, a.experts - 1)) * a.ldw;
+    const int x = x0 + (lane & 1), t = t0 + (lane >> 1);   // of the logit this lane writes
+    const bool mine = lane < 2 * T && x < a.experts && t < M;
+    const int4 cst = mine ? a.cst[x] : make_int4(0, 0, 0, 0);
+    const int e = mine && a.e ? a.e[t] : 0;
+#pragma unroll 4
+    for (int k = lane * 16; k < a.K; k += 1024) {
+        const v4i u0 = *reinterpret_cast<const v4i*>(w0 + k), u1 = *reinterpret_cast<const v4i*>(w1 + k);
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            const size_t row = size_t(min(t0 + i, M - 1)) * a.ld8 + k;
+            const v4i h = *reinterpret_cast<const v4i*>(a.hi + row);
+            ch[i][0] = dot16(h, u0, ch[i][0]);
+            ch[i][1] = dot16(h, u1, ch[i][1]);
+            if (a.lo) {
+                const v4i l = *reinterpret_cast<const v4i*>(a.lo + row);
+                cl[i][0] = dot16(l, u0, cl[i][0]);
+                cl[i][1] = dot16(l, u1, cl[i][1]);
+            }
+        }
+    }
+    i64 acc = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * T; ++i) {
+        const int sh = wave_sum32(ch[i >> 1][i & 1]), sl = a.lo ? wave_sum32(cl[i >> 1][i & 1]) : 0;
+        if (lane == i) acc = a.lo ? 256LL * sh + sl : i64(sh);
+    }
+    if (mine) a.logits[size_t(t) * a.experts + x] = w4_requant(acc, a.lo != nullptr, cst, e);
+}
+
+// A block per token, which computes the logits, a wave U experts at once, or (U = 0) finds them in a.logits
 template <int U>
 __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     __shared__ __align__(16) int s_z[MOE_EXPERTS + 16];
@@ -66,10 +107,11 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     const int8_t* lo = a.lo ? a.lo + size_t(t) * a.ld8 : nullptr;
     const int e = a.e ? a.e[t] : 0, i = threadIdx.x;
     // on their way while the products run: the constants of expert i, entry i of the table
-    const int4 cst = i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
+    const int4 cst = U && i < a.experts ? a.cst[i] : make_int4(0, 0, 0, 0);
+    const int found = !U && i < a.experts ? a.logits[size_t(t) * a.experts + i] : 0;
     const long long ex = a.Lexp[i], ex_last = a.Lexp[EXP_N - 1];
     static_assert(EXP_N == ROUTE_THREADS + 1, "an entry a thread, and the last");
-    for (int x0 = wave * U; x0 < a.experts; x0 += ROUTE_THREADS / 64 * U) {
+    if constexpr (U > 0) for (int x0 = wave * U; x0 < a.experts; x0 += ROUTE_THREADS / 64 * U) {
         int ch[U], cl[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) ch[u] = cl[u] = 0;
@@ -99,33 +141,62 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     s_exp[i] = ex;
     if (i == 0) s_exp[EXP_N - 1] = ex_last;
     if (i < 16) s_z[a.experts + i] = INT_MIN;
-    __syncthreads();
-    const int z = i < a.experts ? w4_requant(lo ? 256LL * s_h[i] + s_l[i] : i64(s_h[i]), lo != nullptr, cst, e) : 0;
+    if constexpr (U > 0) __syncthreads();
+    const int z = i >= a.experts ? 0 : (U ? w4_requant(lo ? 256LL * s_h[i] + s_l[i] : i64(s_h[i]), lo != nullptr, cst, e) : found);
     if (i < a.experts) {
         s_z[i] = z;
-        if (a.logits) a.logits[size_t(t) * a.experts + i] = z;
+        if (U && a.logits) a.logits[size_t(t) * a.experts + i] = z;
     }
     __syncthreads();
-    // an expert's place: the logits before it in falling order, equal ones by their index; `side` threads an expert, 16 logits a
-    // step (INT_MIN behind the last expert counts for nobody)
-    const int lg = a.experts <= 128 ? 3 : (a.experts <= 256 ? 2 : 1), side = 1 << lg, x = i >> lg;
-    if (x < a.experts) {
-        const int zx = s_z[x];
-        int rank = 0;
-        for (int j = 16 * (i & (side - 1)); j < a.experts; j += 16 * side) {
+    if (a.experts > ROUTE_RANK) {   // choice by choice: the first wave's largest, of equal ones the lowest index
+        if (wave == 0) {
+            uint32_t key[MOE_EXPERTS / 64];
+            unsigned left = 0;          // bit s: expert 64 s + lane is there and not chosen yet
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-                const int4 o = *reinterpret_cast<const int4*>(&s_z[j + k]);
-                rank += (o.x > zx || (o.x == zx && j + k < x)) ? 1 : 0;
-                rank += (o.y > zx || (o.y == zx && j + k + 1 < x)) ? 1 : 0;
-                rank += (o.z > zx || (o.z == zx && j + k + 2 < x)) ? 1 : 0;
-                rank += (o.w > zx || (o.w == zx && j + k + 3 < x)) ? 1 : 0;
+            for (int s = 0; s < MOE_EXPERTS / 64; ++s) {
+                const int x = 64 * s + lane;
+                key[s] = x < a.experts ? uint32_t(s_z[x]) ^ 0x80000000u : 0u;
+                left |= x < a.experts ? 1u << s : 0u;
+            }
+            for (int r = 0; r < a.topk; ++r) {
+                uint32_t best = 0;
+                int at = -1;
+#pragma unroll
+                for (int s = MOE_EXPERTS / 64 - 1; s >= 0; --s) {
+                    const bool take = (left >> s & 1) && key[s] >= best;
+                    best = take ? key[s] : best;
+                    at = take ? s : at;
+                }
+                const uint32_t m = wave_umax32(best);
+                const int x = int(~wave_umax32(best == m && at >= 0 ? ~unsigned(64 * at + lane) : 0u));
+                if (lane == (x & 63)) left &= ~(1u << (x >> 6));
+                if (lane == 0) {
+                    a.idx[size_t(t) * a.topk + r] = x;
+                    s_top[r] = int(m ^ 0x80000000u);
+                }
             }
         }
-        for (int d = 1; d < side; d <<= 1) rank += __shfl_xor(rank, d);
-        if ((i & (side - 1)) == 0 && rank < a.topk) {
-            a.idx[size_t(t) * a.topk + rank] = x;
-            s_top[rank] = zx;
+    } else {   // an expert's place: the logits before it in falling order; eight threads an expert, 16 logits a step (INT_MIN behind the
+               // last expert counts for nobody)
+        const int x = i >> 3;
+        if (x < a.experts) {
+            const int zx = s_z[x];
+            int rank = 0;
+            for (int j = 16 * (i & 7); j < a.experts; j += 128) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const int4 o = *reinterpret_cast<const int4*>(&s_z[j + k]);
+                    rank += (o.x > zx || (o.x == zx && j + k < x)) ? 1 : 0;
+                    rank += (o.y > zx || (o.y == zx && j + k + 1 < x)) ? 1 : 0;
+                    rank += (o.z > zx || (o.z == zx && j + k + 2 < x)) ? 1 : 0;
+                    rank += (o.w > zx || (o.w == zx && j + k + 3 < x)) ? 1 : 0;
+                }
+            }
+            for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor(rank, d);
+            if ((i & 7) == 0 && rank < a.topk) {
+                a.idx[size_t(t) * a.topk + rank] = x;
+                s_top[rank] = zx;
+            }
         }
     }
     __syncthreads();
@@ -147,6 +218,15 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
 
 hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
     const int waves = ROUTE_THREADS / 64;
+    // One block reads 256 x 7168 in 25.8 us, 512 x 16384 in 92: with room for the logits a kernel before computes them on many CUs, 3.8 + 4.9
+    // and 4.9 + 4.7 us (128 x 2048 takes 6.6 us in one)
+    if (a.logits && (long long)a.experts * a.K > ROUTE_ONE) {
+        if (M < 4) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(cdiv(a.experts, LOGITS_X), M), dim3(256), 0, st, a, M);
+        else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(cdiv(a.experts, LOGITS_X), cdiv(M, 4)), dim3(256), 0, st, a, M);
+        if (hipError_t e = hipGetLastError()) return e;
+        hipLaunchKernelGGL(moe_route_kernel<0>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
+        return hipGetLastError();
+    }
     if (a.experts <= waves) hipLaunchKernelGGL(moe_route_kernel<1>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
     else if (a.experts <= 4 * waves) hipLaunchKernelGGL(moe_route_kernel<4>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
     else hipLaunchKernelGGL(moe_route_kernel<8>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
@@ -241,8 +321,7 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
     int32_t* lut = reinterpret_cast<int32_t*>(sums + js * 256);   // of the gate
     const size_t at = x * (DOWN ? a.down_stride : a.up_stride);
-    const uint8_t* q = W.q + at + size_t(ct0) * KT * 1024;
-    const uint8_t* s = W.s + at + size_t(ct0) * KT * (4096 / G);
+    const W4Columns from{W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT};
     // as many tiles of K a chunk as the staging area holds of n rows, chunks of even size
     W4Chunks ch;
     ch.kc = __builtin_amdgcn_readfirstlane(min(KT, max(1, (w4_div(rows_lds >> 4, n * P) - 1) >> 3)));
@@ -253,7 +332,7 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
         ch.n = __builtin_amdgcn_readfirstlane(w4_div(KT + ch.kc - 1, ch.kc));
     }
     W4Ring<G, DEPTH> ring;
-    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    ring.start(from, KT, tiles, 0, ch, lane, wave, waves);
     for (int k = threadIdx.x; k < tiles * 256; k += blockDim.x) sums[k] = 0;
     if (int(threadIdx.x) < n) s_max[threadIdx.x] = 0;
     if constexpr (!DOWN) w4_load_lut(lut, a.Lphi, lane, wave, waves);
@@ -272,10 +351,10 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
         else
             w4_stage<P>(lds, ch.ld(), n, n, k0, kc, a.Kp16, a.hi, a.lo, [&](int r) { return unsigned(w4_div(s_pair[r], a.topk)) * unsigned(a.ld8); });
         __syncthreads();
-        if (n <= 4) w4_share<1, 1, P, G, DEPTH>(ring, lds, ch.ld(), n, n, sums, lane);
-        else w4_share<1, 4, P, G, DEPTH>(ring, lds, ch.ld(), n, n, sums, lane);
+        if (n <= 4) w4_share<1, 1, P, G>(ring, lds, ch.ld(), n, n, [](int) { return 0; }, sums, lane);
+        else w4_share<1, 4, P, G>(ring, lds, ch.ld(), n, n, [](int) { return 0; }, sums, lane);
         if (++c == ch.n) break;
-        ring.start(q, s, KT, tiles, c, ch, lane, wave, waves);
+        ring.start(from, KT, tiles, c, ch, lane, wave, waves);
         __syncthreads();
     }
     // two columns a thread; their constants come while the last sums do
@@ -308,11 +387,28 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     }
 }
 
-// Of at most MOE_FEW pairs: all their down products and the sums over the tokens' choices, a segment of column tiles a block. A pair has
-// `wpp` waves; the rows v stand in LDS whole, [plane][pair].
-constexpr int MOE_FEW = 16;
+// Column tiles c of the down products of several pairs: pair c / tiles, the block's column tile c % tiles
+struct MoeColumns {
+    const uint8_t *q, *s;      // the block's first column tile in expert 0
+    size_t stride;
+    int KT, tiles;
+    int x;                     // lane l: the expert of pair l
+    __device__ __forceinline__ int pair(int c) const { return tiles == 1 ? c : __builtin_amdgcn_readfirstlane(w4_div(c, tiles)); }
+    template <int G>
+    __device__ __forceinline__ void at(int c, int k, const uint8_t*& qc, const uint8_t*& sc) const {
+        const int j = pair(c);
+        const size_t off = __builtin_amdgcn_readlane(x, j) * stride, tile = size_t(c - j * tiles) * KT + k;
+        qc = q + off + tile * 1024;
+        sc = s + off + tile * (4096 / G);
+    }
+};
+
+// Of at most MOE_FEW pairs: all their down products and the sums over the tokens' choices, a segment of column tiles a block, whose
+// waves share the tiles of all the pairs evenly. The rows v stand in LDS whole, [plane][pair]. A pair without an expert goes through
+// expert 0's tiles and is left out of the sums.
+constexpr int MOE_FEW = 24;
 template <int G>
-__global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, int wpp, int rows_lds) {
+__global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, int rows_lds) {
     constexpr int DEPTH = 6;   // one token, 4096 x 1536: 5.8 us, 8.5 with 4
     extern __shared__ uint4 s_dyn[];
     __shared__ int s_se[MOE_FEW], s_x[MOE_FEW];
@@ -322,16 +418,12 @@ __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, i
     uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
     unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);   // [pair][column tile][4][16]: the first of the four rows
     unsigned long long* out = sums + pairs * js * 64;                                       // [token][column]
-    const int j = __builtin_amdgcn_readfirstlane(w4_div(wave, wpp)), part = wave - j * wpp;
-    const int x = j < pairs ? __builtin_amdgcn_readfirstlane(a.idx[j]) : -1;
-    const bool work = unsigned(x) < unsigned(a.experts);
-    W4Ring<G, DEPTH> ring;
-    if (work) {
-        const size_t at = x * a.down_stride;
-        ring.start(W.q + at + size_t(ct0) * KT * 1024, W.s + at + size_t(ct0) * KT * (4096 / G), KT, tiles, 0, W4Chunks{KT, 1}, lane, part, wpp);
-    }
+    const int xl = lane < pairs ? a.idx[lane] : -1;
+    const MoeColumns from{W.q + size_t(ct0) * KT * 1024, W.s + size_t(ct0) * KT * (4096 / G), a.down_stride, KT, tiles, unsigned(xl) < unsigned(a.experts) ? xl : 0};
+    W4Ring<G, DEPTH, MoeColumns> ring;
+    ring.start(from, KT, pairs * tiles, 0, W4Chunks{KT, 1}, lane, wave, waves);
     for (int i = threadIdx.x; i < pairs * js * 64 + a.M * js * 16; i += blockDim.x) sums[i] = 0;
-    if (int(threadIdx.x) < pairs) s_x[threadIdx.x] = a.idx[threadIdx.x];
+    if (int(threadIdx.x) < pairs) s_x[threadIdx.x] = xl;   // the first wave
     const auto shift = [&](int r) {
         const int e = moe_shift(a, r, lane);
         if (lane == 0) s_se[r] = e;
@@ -347,13 +439,13 @@ __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, i
         c = unsigned(s_x[jj]) < unsigned(a.experts) ? W.cst[size_t(s_x[jj]) * W.CT * 16 + col] : make_int4(0, 0, 0, 0);
     };
     if (int(threadIdx.x) < items) fetch(threadIdx.x);
-    if (work) w4_share<1, 1, 2, G, DEPTH>(ring, lds + j * ld, ld, pairs, 1, sums + j * js * 64, lane);
+    w4_share<1, 1, 2, G>(ring, lds, ld, pairs, 1, [&](int c2) { return from.pair(c2); }, sums, lane);
     __syncthreads();
     for (int i = threadIdx.x; i < items; i += blockDim.x) {
         const int jj = w4_div(i >> 4, tiles), ct = (i >> 4) - jj * tiles;
         if (i != int(threadIdx.x)) fetch(i);
         if (unsigned(s_x[jj]) >= unsigned(a.experts)) continue;
-        const int y = w4_requant(i64(sums[(jj * js + ct) * 64 + (i & 15)]), true, c, s_se[jj]);
+        const int y = w4_requant(i64(sums[(i >> 4) * 64 + (i & 15)]), true, c, s_se[jj]);
         atomicAdd(&out[(w4_div(jj, a.topk) * js + ct) * 16 + (i & 15)], u64(i64(a.p[jj])) * u64(i64(y)));
     }
     __syncthreads();
@@ -412,7 +504,7 @@ static void moe_launch(hipStream_t st, const MoeArgs& a, MoeShape sh) {
 template <int G>
 static void moe_down_few(hipStream_t st, const MoeArgs& a, int js, int rows_lds) {
     const int pairs = a.M * a.topk;
-    hipLaunchKernelGGL((moe_down_few_kernel<G>), dim3(cdiv(a.down.CT, js)), dim3(1024), rows_lds + pairs * js * 512 + a.M * js * 128, st, a, js, 16 / pairs, rows_lds);
+    hipLaunchKernelGGL((moe_down_few_kernel<G>), dim3(cdiv(a.down.CT, js)), dim3(1024), rows_lds + pairs * js * 512 + a.M * js * 128, st, a, js, rows_lds);
 }
 template <bool DOWN, int P>
 static void moe_product(hipStream_t st, const MoeArgs& a, int group, MoeShape sh) {
@@ -428,11 +520,12 @@ hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
     else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
-    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 9.8 against 13.3 + 4.7 us. A pair
+    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 8.8 against 13.3 + 4.7 us; 24
+    // pairs of 64 experts, 2048 x 1408, 14.5 against 11.7 + 4.0, 32 pairs 17.2 against 12.5 + 4.0. A pair
     // reads its expert's matrix by itself: not where that is more than 64 MB beyond a read each of the chosen experts (16 pairs of 2
-    // experts: 4096 x 1536, 44 MB, 12.3 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
+    // experts: 4096 x 1536, 44 MB, 11.5 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
     const int pairs = a.M * a.topk, js = std::min(8, cdiv(a.down.CT, NCU)), rows = pairs * 2 * (a.down.KT * 128 + 16);
-    if (pairs <= MOE_FEW && rows + pairs * js * 512 + a.M * js * 128 + 256 <= 160 << 10 && (pairs - moe_chosen(a)) * double(a.down_stride) <= 64e6) {
+    if (pairs <= MOE_FEW && rows + pairs * js * 512 + a.M * js * 128 + 2 * MOE_FEW * 4 <= 160 << 10 && (pairs - moe_chosen(a)) * double(a.down_stride) <= 64e6) {
         if (a.group_down == 32) moe_down_few<32>(st, a, js, rows);
         else if (a.group_down == 64) moe_down_few<64>(st, a, js, rows);
         else moe_down_few<128>(st, a, js, rows);

@@ -104,14 +104,13 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     uint8_t* lds = reinterpret_cast<uint8_t*>(s_dyn);
     unsigned long long* sums = reinterpret_cast<unsigned long long*>(lds + rows_lds);
     int32_t* lut = reinterpret_cast<int32_t*>(sums + js * TR * 16);   // GEGLU
-    const uint8_t* q = a.w.q + size_t(ct0) * KT * 1024;
-    const uint8_t* s = a.w.s + size_t(ct0) * KT * (4096 / G);
+    const W4Columns from{a.w.q + size_t(ct0) * KT * 1024, a.w.s + size_t(ct0) * KT * (4096 / G), KT};
     const bool x32 = P == 2 && a.x;
     W4Ring<G, DEPTH> ring;
     int e = 0;   // of row threadIdx.x, asked for before the tiles so that nobody waits for those
     if (int(threadIdx.x) < rows) e = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     for (int i = threadIdx.x; i < tiles * TR * 16; i += blockDim.x) sums[i] = 0;
-    ring.start(q, s, KT, tiles, 0, ch, lane, wave, waves);
+    ring.start(from, KT, tiles, 0, ch, lane, wave, waves);
     if (a.geglu) w4_load_lut(lut, a.Lphi, lane, wave, waves);
     if (int(threadIdx.x) < rows) {
         s_rm[threadIdx.x] = 0;
@@ -125,9 +124,9 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
             w4_stage<P>(lds, ch.ld(), prows, rows, k0, kc, a.Kp16, a.hi + size_t(row0) * a.ld8, P == 2 ? a.lo + size_t(row0) * a.ld8 : nullptr,
                         [&](int r) { return unsigned(r) * unsigned(a.ld8); });
         __syncthreads();
-        w4_share<MT, RR, P, G, DEPTH>(ring, lds, ch.ld(), prows, rows, sums, lane);
+        w4_share<MT, RR, P, G>(ring, lds, ch.ld(), prows, rows, [](int) { return 0; }, sums, lane);
         if (++c == ch.n) break;
-        ring.start(q, s, KT, tiles, c, ch, lane, wave, waves);   // on its way while the rows are staged
+        ring.start(from, KT, tiles, c, ch, lane, wave, waves);   // on its way while the rows are staged
         __syncthreads();
     }
     // two columns a thread

@@ -237,42 +237,54 @@ __device__ __forceinline__ void w4_load_lut(int32_t* to, const int32_t* L, int l
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + 64 * i), 4, 4 * lane, 256 * i, 0, 0);
 }
 
-// A wave's share of a chunk: tiles u of the segment's column tiles c = u / kc, in the order of their addresses
-template <int G, int DEPTH>
+// Column tiles c = 0, 1, ... of a matrix, one behind the other
+struct W4Columns {
+    const uint8_t *q, *s;      // of the first
+    int KT;
+    template <int G>
+    __device__ __forceinline__ void at(int c, int k, const uint8_t*& qc, const uint8_t*& sc) const {   // tile k of column tile c
+        const size_t tile = size_t(c) * KT + k;
+        qc = q + tile * 1024;
+        sc = s + tile * (4096 / G);
+    }
+};
+
+// A wave's share of a chunk: tiles u of the column tiles c = u / kc, in the order of their addresses
+template <int G, int DEPTH, class Src = W4Columns>
 struct W4Ring {
     W4Tile<G> t[DEPTH];
-    const uint8_t *q, *s;      // of the segment's first column tile
-    int KT, k0, kc;
+    Src src;
+    int k0, kc;                // the chunk's tiles of K
     int u0, u1;                // the wave's tiles
+    const uint8_t *qc, *sc;    // the column tile loaded from
     int c, k;                  // the tile loaded next
     __device__ __forceinline__ void fetch(int d, int lane) {
-        const size_t tile = size_t(c) * KT + k0 + k;
-        t[d].load(q + tile * 1024, s + tile * (4096 / G), lane);
+        t[d].load(qc + size_t(k) * 1024, sc + size_t(k) * (4096 / G), lane);
         if (++k == kc) {
             k = 0;
-            ++c;
+            src.template at<G>(++c, k0, qc, sc);
         }
     }
-    __device__ __forceinline__ void start(const uint8_t* q_, const uint8_t* s_, int KT_, int tiles, int chunk, const W4Chunks& ch, int lane, int wave, int waves) {
-        q = q_;
-        s = s_;
-        KT = KT_;
+    __device__ __forceinline__ void start(const Src& from, int KT, int cols, int chunk, const W4Chunks& ch, int lane, int wave, int waves) {
+        src = from;
         k0 = chunk * ch.kc;
         kc = min(ch.kc, KT - k0);
-        const int units = tiles * kc;
+        const int units = cols * kc;
         u0 = __builtin_amdgcn_readfirstlane(w4_div(units * wave, waves));
         u1 = __builtin_amdgcn_readfirstlane(w4_div(units * (wave + 1), waves));
         c = __builtin_amdgcn_readfirstlane(w4_div(u0, kc));
         k = u0 - c * kc;
+        src.template at<G>(c, k0, qc, sc);
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
             if (u0 + d < u1) fetch(d, lane);
     }
 };
 
-// The wave's share: sums of column tile c, row t and column n are added to sums[(c * TR + t) * 16 + n], TR = 4 RR MT
-template <int MT, int RR, int P, int G, int DEPTH>
-__device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* lds, int ld, int prows, int rows, unsigned long long* sums, int lane) {
+// The wave's share: sums of column tile c, row t and column n are added to sums[(c * TR + t) * 16 + n], TR = 4 RR MT. rows_of(c): the
+// first of the rows column tile c meets
+template <int MT, int RR, int P, int G, int DEPTH, class Src, class F>
+__device__ __forceinline__ void w4_share(W4Ring<G, DEPTH, Src>& ring, const uint8_t* lds, int ld, int prows, int rows, F rows_of, unsigned long long* sums, int lane) {
     constexpr int TR = 4 * RR * MT;
     int u = ring.u0, c = __builtin_amdgcn_readfirstlane(w4_div(u, ring.kc)), k = u - c * ring.kc;
     if (u >= ring.u1) return;
@@ -288,10 +300,11 @@ __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* 
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < RR; ++r) acc[mt][r] = 0;
+    int row = rows_of(c) * ld;
     const auto step = [&](int d, bool last) {
         const uint8_t* a[P];
 #pragma unroll
-        for (int p = 0; p < P; ++p) a[p] = base[p] + k * 128;
+        for (int p = 0; p < P; ++p) a[p] = base[p] + row + k * 128;
         w4_tile<MT, RR, P, G>(ring.t[d], a, 16 * ld, acc, lane);
         if (++k == ring.kc || last) {
 #pragma unroll
@@ -302,7 +315,7 @@ __device__ __forceinline__ void w4_share(W4Ring<G, DEPTH>& ring, const uint8_t* 
                     acc[mt][r] = 0;
                 }
             k = 0;
-            ++c;
+            row = rows_of(++c) * ld;
         }
         __builtin_amdgcn_sched_barrier(0);   // one tile at a time: stages drawn into one another spill
     };
