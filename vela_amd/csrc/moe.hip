@@ -60,7 +60,7 @@ __device__ __forceinline__ u64 route_recip(u64 s) {
 constexpr int LOGITS_X = 8;
 template <int T>
 __global__ void __launch_bounds__(256) moe_logits_kernel(RouteArgs a, int M) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x0 = int(blockIdx.x) * LOGITS_X + 2 * wave, t0 = int(blockIdx.y) * T;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x0 = int(blockIdx.y) * LOGITS_X + 2 * wave, t0 = int(blockIdx.x) * T;
     if (x0 >= a.experts) return;
     int ch[T][2], cl[T][2];
 #pragma unroll
@@ -221,8 +221,8 @@ hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
     // One block reads 256 x 7168 in 25.8 us, 512 x 16384 in 92: with room for the logits a kernel before computes them on many CUs, 3.8 + 4.9
     // and 4.9 + 4.7 us (128 x 2048 takes 6.6 us in one)
     if (a.logits && (long long)a.experts * a.K > ROUTE_ONE) {
-        if (M < 4) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(cdiv(a.experts, LOGITS_X), M), dim3(256), 0, st, a, M);
-        else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(cdiv(a.experts, LOGITS_X), cdiv(M, 4)), dim3(256), 0, st, a, M);
+        if (M < 4) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(M, cdiv(a.experts, LOGITS_X)), dim3(256), 0, st, a, M);
+        else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(cdiv(M, 4), cdiv(a.experts, LOGITS_X)), dim3(256), 0, st, a, M);
         if (hipError_t e = hipGetLastError()) return e;
         hipLaunchKernelGGL(moe_route_kernel<0>, dim3(M), dim3(ROUTE_THREADS), 0, st, a);
         return hipGetLastError();
