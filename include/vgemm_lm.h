@@ -59,7 +59,7 @@ int vgemm_w4_pack(void* stream, const VgemmW4* W, int first, int n, const uint8_
  *                    table it is a * SiLU(g)
  * and rowmax[r] = max(rowmax[r], |y|) when E->rowmax != NULL. A: VGEMM_SRC_I8 (lo may be NULL; ld8 >= K rounded up to 16, ld8 % 16
  * == 0, 16-byte aligned planes; columns past K are not used) or VGEMM_SRC_X32 (K == W->K, K % 4 == 0; row maxima in
- * rowmax). Made for rows up to a few tens: the weights are read once for every 64 8-bit rows, for every 32 of the other kinds.
+ * rowmax). Made for rows up to a few tens: the weights are read once for every 16 or 32 of them.
  * M <= 2^20, ld8 <= 2^21, ldx <= 2^23 (else VGEMM_ERR_UNSUPPORTED). M == 0 is a no-op. */
 int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const VgemmAEpi* E);
 

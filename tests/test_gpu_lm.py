@@ -227,6 +227,13 @@ def test_w4_chunks_and_segments(gpu, kind, M, K, N):
     check_w4(np.random.default_rng(K + N), kind, M, N, K, 64, residual=True)
 
 
+@pytest.mark.parametrize("kind,M,K,N", [("q8", 3, 33, 70001), ("x32", 1, 64, 150000), ("q16", 40, 32, 20002), ("x32", 100, 16, 9000), ("q8", 17, 64, 34000), ("q16", 33, 200, 4096),
+                                        ("q8", 1000, 20, 70), ("q16", 700, 40, 33), ("x32", 4100, 8, 20)])
+def test_w4_many_columns_or_rows(gpu, kind, M, K, N):
+    """Segments of many column tiles, more blocks than CUs, more row tiles than CUs."""
+    check_w4(np.random.default_rng(M + N), kind, M, N, K, 64, residual=True)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_w4_extremes(gpu, kind, group):

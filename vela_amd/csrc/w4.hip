@@ -178,12 +178,15 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     }
 }
 
+// Column tiles a block has, of up to TR rows: what one round of blocks, one a CU, takes; at most 64 KiB of sums
+static int w4_js(const W4Args& a, int TR) { return std::min(512 / TR, cdiv(a.w.CT, std::max(1, NCU / cdiv(a.M, TR)))); }
+
 template <int MT, int RR, int P, int G>
 static void w4_launch(hipStream_t st, const W4Args& a) {
     constexpr int TR = 4 * RR * MT;
     // Sixteen waves a block, a block a CU: halves of that, two a CU, staged the rows twice as often and, with twice as many blocks adding to the row
     // maxima, took 18.1 against 16.0 us for 16 x 4096 x 22016 with GEGLU, 16.1 against 13.2 with 16-bit rows.
-    const int rb = cdiv(a.M, TR), js = std::min(8, cdiv((long long)a.w.CT * rb, NCU));
+    const int rb = cdiv(a.M, TR), js = w4_js(a, TR);
     const int lut = a.geglu ? W4_LUT_LDS : 0, most = (156 << 10) - js * TR * 128 - lut, prows = MT == 1 ? std::min(TR, a.M) : TR;
     const W4Chunks ch = W4Chunks::of(prows, P, a.w.KT, most);   // whole rows where they fit
     const int rows_lds = prows * P * ch.ld();
@@ -199,18 +202,28 @@ static void w4_group(hipStream_t st, const W4Args& a) {
 
 template <int MT, int RR>
 static void w4_planes(hipStream_t st, const W4Args& a) {
-    if constexpr (MT < 4) {   // sixty-four rows in two planes do not fit the registers: 51 x 2600 x 9999 took 28.7 us, 18.8 as two blocks of 32
-        if (a.x || a.lo) return w4_group<MT, RR, 2>(st, a);
-    }
-    w4_group<MT, RR, 1>(st, a);
+    if (a.x || a.lo) w4_group<MT, RR, 2>(st, a);
+    else w4_group<MT, RR, 1>(st, a);
 }
 
+// More than sixteen rows go in blocks of 16 where a block then has few column tiles, so that staging (and quantising) the rows counts
+// more than reading the weights again, else in blocks of 32:
+//                                   16        32 rows a block
+//   int32, 32 x 11008 x 4096        23.0      44.1 us    2 column tiles a block of 16 rows
+//          64 x 4096 x 12288        23.1      24.8      12
+//          64 x 4096 x 22016        38.4      36.2      22
+//   16-bit, 32 x 11008 x 4096       14.7      21.2       2
+//          128 x 4096 x 4096        14.4      14.0       8
+//          64 x 4096 x 12288        20.2      19.2      12
+//   8-bit, 32 x 11008 x 4096        11.5      13.0       2
+//          20 x 4096 x 4096          6.2       6.0       2
+//          128 x 4096 x 4096        11.8      10.0       8
+//          32 x 4096 x 22016        18.2      12.8      11
 hipError_t launch_w4(hipStream_t st, const W4Args& a) {
     if (a.M <= 4) w4_planes<1, 1>(st, a);
     else if (a.M <= 8) w4_planes<1, 2>(st, a);
-    else if (a.M <= 16) w4_planes<1, 4>(st, a);
-    else if (a.M <= 32 || a.x || a.lo) w4_planes<2, 4>(st, a);
-    else w4_planes<4, 4>(st, a);
+    else if (a.M <= 16 || w4_js(a, 16) <= (a.x ? 16 : (a.lo ? 8 : 2))) w4_planes<1, 4>(st, a);
+    else w4_planes<2, 4>(st, a);
     return hipGetLastError();
 }
 

@@ -14,7 +14,7 @@
 // behind all tiles the group words [column tile][K tile][16 columns][128 / group], zero << 12 | scale. Columns past N and
 // values past K have scale 0 and u = z.
 //
-// Work of a block: a segment of column tiles against up to 64 rows. The rows are staged in LDS, as much of K at a time as fits
+// Work of a block: a segment of column tiles against up to 32 rows. The rows are staged in LDS, as much of K at a time as fits
 // (a chunk): read from memory by every wave, 16 rows of 64 bytes would take 65 cycles of a CU's address unit a load, against
 // 17 for a tile's nibbles and 6 for its words. The chunk's tiles, a column tile's one after the other, are split evenly over the
 // waves, which stream them with DEPTH tiles in flight and add each column tile's sums to 64-bit integers in LDS; the epilogue
