@@ -207,7 +207,7 @@ static void w4_planes(hipStream_t st, const W4Args& a) {
 }
 
 // More than sixteen rows go in blocks of 16 where a block then has few column tiles, so that staging (and quantising) the rows counts
-// more than reading the weights again, else in blocks of 32:
+// more than reading the weights again, else in blocks of 32; int32 rows by the same reason in blocks of 8:
 //                                   16        32 rows a block
 //   int32, 32 x 11008 x 4096        23.0      44.1 us    2 column tiles a block of 16 rows
 //          64 x 4096 x 12288        23.1      24.8      12
@@ -219,9 +219,14 @@ static void w4_planes(hipStream_t st, const W4Args& a) {
 //          20 x 4096 x 4096          6.2       6.0       2
 //          128 x 4096 x 4096        11.8      10.0       8
 //          32 x 4096 x 22016        18.2      12.8      11
+//                                    8        16 rows a block
+//   int32, 16 x 11008 x 4096        15.0      20.5 us    2 column tiles a block of 8 rows
+//          32 x 11008 x 4096        20.1      22.9       4
+//          64 x 11008 x 4096        29.3      28.8       8
+//          16 x 4096 x 22016        20.3      15.8      11
 hipError_t launch_w4(hipStream_t st, const W4Args& a) {
     if (a.M <= 4) w4_planes<1, 1>(st, a);
-    else if (a.M <= 8) w4_planes<1, 2>(st, a);
+    else if (a.M <= 8 || (a.x && w4_js(a, 8) <= 8)) w4_planes<1, 2>(st, a);
     else if (a.M <= 16 || w4_js(a, 16) <= (a.x ? 16 : (a.lo ? 8 : 2))) w4_planes<1, 4>(st, a);
     else w4_planes<2, 4>(st, a);
     return hipGetLastError();
