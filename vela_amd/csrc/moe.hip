@@ -60,6 +60,7 @@ __device__ __forceinline__ u64 route_recip(u64 s) {
 constexpr int LOGITS_X = 8;
 template <int T>
 __global__ void __launch_bounds__(256) moe_logits_kernel(RouteArgs a, int M) {
+    touch_args<int(sizeof(RouteArgs) + 4)>();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x0 = int(blockIdx.y) * LOGITS_X + 2 * wave, t0 = int(blockIdx.x) * T;
     if (x0 >= a.experts) return;
     int ch[T][2], cl[T][2];
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(RouteArgs a, int M) {
 // A block per token, which computes the logits, a wave U experts at once, or (U = 0) finds them in a.logits
 template <int U>
 __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
+    touch_args<int(sizeof(RouteArgs))>();
     __shared__ __align__(16) int s_z[MOE_EXPERTS + 16];
     __shared__ int s_h[MOE_EXPERTS], s_l[MOE_EXPERTS];
     __shared__ int s_top[MOE_TOPK];
@@ -306,6 +308,7 @@ constexpr int MOE_JS = 24;   // column tiles a segment has at most: 48 KiB of su
 template <bool DOWN, int P, int G>
 __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_lds) {
     constexpr int DEPTH = DOWN ? 6 : 4;   // 2 experts, 8 tokens, 4096 x 4480: up 13.3 us with 6, 12.6 with 4; down 27.6 against 28.5 for 43 tokens with 6
+    touch_args<int(sizeof(MoeArgs) + 8)>();
     extern __shared__ uint4 s_dyn[];
     __shared__ uint32_t s_max[16];
     __shared__ int s_se[16], s_pair[16];
@@ -410,6 +413,7 @@ constexpr int MOE_FEW = 24;
 template <int G>
 __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, int rows_lds) {
     constexpr int DEPTH = 6;   // one token, 4096 x 1536: 5.8 us, 8.5 with 4
+    touch_args<int(sizeof(MoeArgs) + 8)>();
     extern __shared__ uint4 s_dyn[];
     __shared__ int s_se[MOE_FEW], s_x[MOE_FEW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = __builtin_amdgcn_readfirstlane(blockDim.x >> 6);
@@ -458,6 +462,7 @@ __global__ void __launch_bounds__(1024) moe_down_few_kernel(MoeArgs a, int js, i
 
 // Y[t] = sat32(sat32(rshr(sum_j p y, 15)) + R[t]) over the columns of a pass, eight choices' loads in flight
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a) {
+    touch_args<int(sizeof(MoeArgs))>();
     const int c = int(blockIdx.x) * 256 + int(threadIdx.x), tok = blockIdx.y;
     if (c >= a.cols) return;
     const size_t o = size_t(tok) * a.ldy + a.col0 + c;

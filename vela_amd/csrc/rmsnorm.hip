@@ -6,7 +6,7 @@
 //   e = #{k in [7, 32): m >= 2^k}, q = clamp(rshr(y, e), -127, 127)     (the int16 view: 15 and 32767)
 //
 // A value moves 13 bytes (x, r and h in 32 bits, q in 8) and takes about twenty double operations, so long inputs are
-// bound by memory and few rows by the latency of the three reductions that follow one another (max |h|, ss, max |y|). A
+// bound by memory (4096 x 4096: 42.0 us, 5.2 TB/s) and few rows by the latency of the three reductions that follow one another (max |h|, ss, max |y|). A
 // row stays in registers from its one read on. The arithmetic is exact in double as for LayerNorm (see NormK): a shifted
 // value is at most 2^20 in magnitude, ss at most C 2^40 <= 2^53 for C <= 8192, and floor(ss / C) follows from the
 // correctly rounded quotient, whose error (below 2^-13) is smaller than the 1 / C gap of a non-integer quotient to the next integer.
@@ -38,10 +38,11 @@ struct RmsArgs {
 // VIEW: the int16 view instead of 8-bit rows
 template <int TR, int NV, bool VIEW>
 __global__ void __launch_bounds__(TR < 256 ? 256 : TR) rmsnorm_kernel(RmsArgs a) {
+    touch_args<int(sizeof(RmsArgs))>();
     constexpr int NW = TR / 64;
-    __shared__ uint32_t s_max[16];
-    __shared__ double s_sum[16];
-    __shared__ uint32_t s_ymax[16];
+    __shared__ uint32_t s_max[NW];
+    __shared__ double s_sum[NW];
+    __shared__ uint32_t s_ymax[NW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int tr = TR == 64 ? lane : int(threadIdx.x);
     const int row = TR == 64 ? int(blockIdx.x) * 4 + wave : int(blockIdx.x);
@@ -56,6 +57,9 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) rmsnorm_kernel(RmsArgs a)
         const int4 v = x[q4 < Q ? q4 : 0];
         h[j][0] = v.x; h[j][1] = v.y; h[j][2] = v.z; h[j][3] = v.w;
     }
+    int4 g[NV];   // the gains, on their way during the reductions: 4096 x 4096 46.0 -> 42.0 us
+#pragma unroll
+    for (int j = 0; j < NV; ++j) g[j] = reinterpret_cast<const int4*>(a.g)[tr + TR * j < Q ? tr + TR * j : 0];
     if (a.R) {
         const int4* r = reinterpret_cast<const int4*>(a.R + size_t(row) * a.C);
 #pragma unroll
@@ -107,8 +111,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) rmsnorm_kernel(RmsArgs a)
     for (int j = 0; j < NV; ++j) {
         const int q4 = tr + TR * j;
         const bool sl = q4 < Q;
-        const int4 gg = reinterpret_cast<const int4*>(a.g)[sl ? q4 : 0];
-        const int g4[4] = {gg.x, gg.y, gg.z, gg.w};
+        const int g4[4] = {g[j].x, g[j].y, g[j].z, g[j].w};
         unsigned slow = 0;   // bit k: element k needs the exact form
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -182,16 +185,15 @@ hipError_t launch_rmsnorm_q(hipStream_t st, const int32_t* X, const int32_t* R, 
                             int32_t* e, int Kp) {
     RmsArgs a{X, R, M, C, g, H, hi, lo, e, Kp, {}};
     for (int ex = 0; ex < 13; ++ex) a.eps.v[ex] = ((1LL << (32 - 2 * ex)) + den / 2) / den;
-    // Up to 1024 values a row is a wave's; from there on a block's of 256 threads, of 1024 where wide rows are fewer than CUs (37 x 5120: 7.1 us with
-    // 256, 6.4 with 1024; narrower rows measure the same either way, and from 500 rows on 1024 threads are slower, 9.3 -> 10.6 at 500 x 4096)
+    // Up to 1024 values a row is a wave's, up to 4096 a block's of 256 threads, wider ones of 512 (4096 x 8192: 83.8 us, 5.2 TB/s, 93.0 with 256
+    // threads of eight quads; 37 x 5120: 6.3, 7.1 with 256, 6.4 with 1024)
     const int Q = C / 4;
     if (Q <= 64) rmsnorm_launch<64, 1>(st, a);
     else if (Q <= 128) rmsnorm_launch<64, 2>(st, a);
     else if (Q <= 256) rmsnorm_launch<64, 4>(st, a);
     else if (Q <= 512) rmsnorm_launch<256, 2>(st, a);
     else if (Q <= 1024) rmsnorm_launch<256, 4>(st, a);
-    else if (M <= NCU) rmsnorm_launch<1024, 2>(st, a);
-    else rmsnorm_launch<256, 8>(st, a);
+    else rmsnorm_launch<512, 4>(st, a);
     return hipGetLastError();
 }
 

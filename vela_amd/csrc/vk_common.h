@@ -187,6 +187,16 @@ __device__ __forceinline__ void vm_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+// The first BYTES of the kernel's arguments, a 64-byte line at a time, in one round of scalar loads at its start: they are read cold
+// from memory, and loads that stand behind branches would each wait for memory again
+template <int BYTES>
+__device__ __forceinline__ void touch_args() {
+    static_assert(BYTES <= 6 * 64, "six lines of kernel arguments");
+    constexpr int last = (BYTES - 1) / 4;
+    const auto k = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" ::"s"(k[0]), "s"(k[last < 16 ? last : 16]), "s"(k[last < 32 ? last : 32]), "s"(k[last < 48 ? last : 48]), "s"(k[last < 64 ? last : 64]), "s"(k[last < 80 ? last : 80]));
+}
+
 // workgroup barrier that orders memory accesses in the compiler (no implicit waits)
 __device__ __forceinline__ void block_barrier() { asm volatile("s_barrier" : : : "memory"); }
 

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     // tiles in flight: 48 of a CU's sixteen waves; with 4 and 6 a wave, 5 x 11008 x 4096 took 11.6 and 12.3 against 11.4 us, 1 x 4096 x 22016 10.1
     // and 10.8 against 10.0, 1 x 8192 x 28672 23.7 and 24.1 against 24.1
     constexpr int TR = 4 * RR * MT, DEPTH = 3;
+    touch_args<int(sizeof(W4Args) + sizeof(W4Chunks) + 8)>();
     extern __shared__ uint4 s_dyn[];
     __shared__ uint32_t s_rm[TR];
     __shared__ int s_e[TR];
