@@ -12,7 +12,6 @@
 // correctly rounded quotient, whose error (below 2^-13) is smaller than the 1 / C gap of a non-integer quotient to the next integer.
 #include <climits>
 
-#include "dispatch_rules.h"
 #include "norm_math.h"
 #include "vk_common.h"
 

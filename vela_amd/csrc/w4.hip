@@ -83,7 +83,7 @@ hipError_t launch_w4_pack(hipStream_t st, int N, int K, int group, uint8_t* q, i
 
 // ---------------------------------------------------------------- products
 
-// What two columns' epilogue reads besides the sums: fetched before the products where a thread has one pair of columns
+// What two columns' epilogue reads besides the sums
 struct W4Epi {
     int4 c0, c1;
     int e, r0, r1;
@@ -112,6 +112,21 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     if (int(threadIdx.x) < rows) e = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     for (int i = threadIdx.x; i < tiles * TR * 16; i += blockDim.x) sums[i] = 0;
     ring.start(from, KT, tiles, 0, ch, lane, wave, waves);
+    // two columns a thread; a thread's first two's constants and residual come from here on, where there are registers for them
+    const int items = tiles * rows * 8;
+    W4Epi ep;
+    const auto fetch = [&](int i) {
+        const int ctt = w4_div(i >> 3, rows), t = (i >> 3) - ctt * rows, n = (ct0 + ctt) * 16 + 2 * (i & 7);
+        ep.c0 = a.w.cst[n];
+        ep.c1 = a.w.cst[n + 1];
+        ep.r0 = ep.r1 = 0;
+        if (a.R) {
+            const int32_t* R = a.R + size_t(row0 + t) * a.ldy + n;
+            if (n < a.w.N) ep.r0 = R[0];
+            if (n + 1 < a.w.N) ep.r1 = R[1];
+        }
+    };
+    if (MT == 1 && int(threadIdx.x) < items) fetch(threadIdx.x);
     if (a.geglu) w4_load_lut(lut, a.Lphi, lane, wave, waves);
     if (int(threadIdx.x) < rows) {
         s_rm[threadIdx.x] = 0;
@@ -130,21 +145,7 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
         ring.start(from, KT, tiles, c, ch, lane, wave, waves);   // on its way while the rows are staged
         __syncthreads();
     }
-    // two columns a thread
-    const int items = tiles * rows * 8;
-    W4Epi ep;
-    const auto fetch = [&](int i) {
-        const int ctt = w4_div(i >> 3, rows), t = (i >> 3) - ctt * rows, n = (ct0 + ctt) * 16 + 2 * (i & 7);
-        ep.c0 = a.w.cst[n];
-        ep.c1 = a.w.cst[n + 1];
-        ep.r0 = ep.r1 = 0;
-        if (a.R) {
-            const int32_t* R = a.R + size_t(row0 + t) * a.ldy + n;
-            if (n < a.w.N) ep.r0 = R[0];
-            if (n + 1 < a.w.N) ep.r1 = R[1];
-        }
-    };
-    if (int(threadIdx.x) < items) fetch(threadIdx.x);
+    if (MT == 2 && int(threadIdx.x) < items) fetch(threadIdx.x);
     __syncthreads();
     for (int i = threadIdx.x; i < items; i += blockDim.x) {
         const int c = w4_div(i >> 3, rows), t = (i >> 3) - c * rows, n = (ct0 + c) * 16 + 2 * (i & 7), r = row0 + t;
