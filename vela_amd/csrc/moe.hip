@@ -1,4 +1,4 @@
-// A mixture-of-experts layer for few tokens: the router (vgemm_moe_route, one kernel) and the chosen experts' feed-forward on
+// A mixture-of-experts layer for few tokens: the router (vgemm_moe_route, one or two kernels) and the chosen experts' feed-forward on
 // 4-bit weights with its combination (vgemm_moe: up with GEGLU, down, and the sum over a token's choices).
 #include <algorithm>
 #include <cmath>
@@ -56,6 +56,9 @@ __device__ __forceinline__ u64 route_recip(u64 s) {
     return r >= i64(s) ? q + 1 : q;
 }
 
+// The router moves the layer's int8 weights once a token or four, which is little beside its latency: 3.5 us for 8 experts x 1024, 6.1 for 64 x
+// 2048, 9.2 for 16 tokens of 128 x 2048 in one kernel.
+//
 // Logits of T tokens and eight experts a block, two a wave. Plane sums stay below 16384 * 2^14 = 2^28.
 constexpr int LOGITS_X = 8;
 template <int T>
@@ -238,7 +241,9 @@ hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
 // ---------------------------------------------------------------- experts
 //
 // Both products are cut into items (row tile of at most 16 of an expert's pairs, segment of `js` column tiles), a block each,
-// which computes as w4_kernel.h says.
+// which computes as w4_kernel.h says. Bound by the chosen experts' weights where there are many (16 tokens x 8 of 128, 2048 x 768, groups of
+// 64: up 29.4 us for 135 MB, down 19.0 for 67) or they are large (2 tokens x 8 of 256, 7168 x 2048: up 47.7 us for 240 MB, down 26.8 for
+// 120), else by a block's chain of latencies (one token x 2 of 8, 1024 x 2048: 5.7 and 5.2 us).
 
 // Row tile `tile` of the pairs sorted by expert: its expert and rows; n = 0 past the last tile. pair[]: the tile's pairs, the same in every
 // block (in the order of the pairs), written by the first wave. Every block finds its own: a kernel that did it once took 2 to 5 us.
