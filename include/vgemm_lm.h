@@ -31,7 +31,7 @@ extern "C" {
  * y = sat32(rshr(floor((h 2^(25 - ex) + sd) / 2 sd) g, 16)). With lo == NULL: 8-bit rows hi [M x Kp], e = the
  * least shift >= 0 with max |y| < 2^(7 + e), q = clamp(rshr(y, e), -127, 127); else the int16 view of vgemm_lnorm_q. Columns
  * [C, Kp) hold the value 0. H (may be NULL, X or R) receives h. X, R, H [M x C] and g [C] 16-byte aligned,
- * C % 4 == 0, C <= 8192, Kp >= C, Kp % 4 == 0, hi / lo 4-byte aligned, M <= 2^23. M == 0 is a no-op. */
+ * C % 4 == 0, C <= 8192, Kp >= C, Kp % 4 == 0, hi / lo 4-byte aligned, M <= 2^22. M == 0 is a no-op. */
 int vgemm_rmsnorm_q(void* stream, const int32_t* X, const int32_t* R, int M, int C, const int32_t* g, int64_t den, int32_t* H, int8_t* hi, int8_t* lo,
                     int32_t* e, int Kp);
 
@@ -60,14 +60,14 @@ int vgemm_w4_pack(void* stream, const VgemmW4* W, int first, int n, const uint8_
  * and rowmax[r] = max(rowmax[r], |y|) when E->rowmax != NULL. A: VGEMM_SRC_I8 (lo may be NULL; ld8 >= K rounded up to 16, ld8 % 16
  * == 0, 16-byte aligned planes; columns past K are not used) or VGEMM_SRC_X32 (K == W->K, K % 4 == 0; row maxima in
  * rowmax). Made for rows up to a few tens: the weights are read once for every 16 or 32 of them.
- * M <= 2^20, ld8 <= 2^21, ldx <= 2^23 (else VGEMM_ERR_UNSUPPORTED). M == 0 is a no-op. */
+ * M <= 2^18, ld8 <= 2^21, ldx <= 2^23 (else VGEMM_ERR_UNSUPPORTED). M == 0 is a no-op. */
 int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const VgemmAEpi* E);
 
 /* Router of M tokens (rows of A, VGEMM_SRC_I8): logits z[x] = sat32(rshr(acc m, s - e) + b) of the int8 weights W [experts x ldw]
  * (K = A->K columns, ldw >= K, ldw % 16 == 0) and cst {m, s, b, wsum}; idx [M x topk] = the topk largest, in falling order, equal
  * ones by their index; p [M x topk] their shares in Q15: E_x = lutexp(max z - z[x]) by the attention's exp table Lexp (1025 entries in [0, 2^31)),
  * r = floor(2^62 / sum E) over the chosen (renorm != 0) or all experts, p = min(32767, (E r + 2^46) >> 47). logits [M x experts]
- * may be NULL; given, it lets the logits of a layer above 256 KiB of weights be computed by many CUs (p = 0 where sum E = 0). experts <= 512, topk <= 16, topk <= experts, K % 16 == 0, K <= 16384, M <= 2^20. */
+ * may be NULL; given, it lets the logits of a layer above 256 KiB of weights be computed by many CUs (p = 0 where sum E = 0). experts <= 512, topk <= 16, topk <= experts, K % 16 == 0, K <= 16384, M <= 2^18. */
 typedef struct VgemmMoeRoute {
     const int8_t* W; int ldw; const int32_t* cst;
     int experts, topk, renorm;

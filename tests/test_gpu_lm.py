@@ -234,6 +234,24 @@ def test_w4_many_columns_or_rows(gpu, kind, M, K, N):
     check_w4(np.random.default_rng(M + N), kind, M, N, K, 64, residual=True)
 
 
+def test_w4_most_rows(gpu):
+    """As many rows as a call takes, eight and sixteen a block: every row as the first ones repeat."""
+    M, n = 1 << 18, 64
+    for kind in ("x32", "q8"):
+        rng = np.random.default_rng(18)
+        few, w = Rows(rng, kind, n, 16), lm.Weights(rng, 5, 16, 32)
+        W, times = packed(w), lambda t: t.repeat(M // n, *([1] * (t.dim() - 1)))  # noqa: E731
+        keep = [times(t) for t in few.keep]
+        if kind == "x32":
+            A = vg.ASrc(src=vg.SRC_X32, x=vg.ptr(keep[0]), ldx=keep[0].shape[1], rowmax=vg.ptr(keep[1]), K=16)
+        else:
+            A = vg.ASrc(src=vg.SRC_I8, hi=vg.ptr(keep[0]), ld8=keep[0].shape[1], e=vg.ptr(keep[-1]), K=16)
+        y = torch.empty((M, 5), dtype=torch.int32, device="cuda")
+        vw.k_gemm_w4(A, M, W, vg.AEpi(Y=vg.ptr(y), ldy=5))
+        want = dev(lm.product(few.q, few.e, w.dense(), w.msb).astype(np.int32))
+        assert torch.equal(y.view(M // n, n, 5), want.expand(M // n, n, 5))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_w4_extremes(gpu, kind, group):

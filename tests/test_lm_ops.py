@@ -140,13 +140,13 @@ def test_limits():
     wide = _lib.ASrc(src=0, hi=FAKE, ld8=(1 << 21) + 16, K=64)
     R = _lib.MoeRoute(W=FAKE, ldw=64, cst=FAKE, experts=8, topk=2, Lexp=FAKE, idx=FAKE, p=FAKE)
     P = _lib.Moe(up=W, down=_lib.W4(N=64, K=32, group=64, count=1, q=FAKE, cst=FAKE), topk=1, idx=FAKE, p=FAKE, Lphi=FAKE, Y=FAKE, ldy=64, ws=FAKE, ws_bytes=1 << 20)
-    for call, msg in ((lambda: lib.vgemm_w4(None, ctypes.byref(rows), (1 << 20) + 1, ctypes.byref(W), ctypes.byref(E)), "w4: at most"),
+    for call, msg in ((lambda: lib.vgemm_w4(None, ctypes.byref(rows), (1 << 18) + 1, ctypes.byref(W), ctypes.byref(E)), "w4: at most"),
                       (lambda: lib.vgemm_w4(None, ctypes.byref(wide), 1, ctypes.byref(W), ctypes.byref(E)), "ld8 above"),
                       (lambda: lib.vgemm_w4(None, ctypes.byref(x32), 1, ctypes.byref(W), ctypes.byref(E)), "ldx above"),
-                      (lambda: lib.vgemm_moe_route(None, ctypes.byref(rows), (1 << 20) + 1, ctypes.byref(R)), "moe_route: at most"),
+                      (lambda: lib.vgemm_moe_route(None, ctypes.byref(rows), (1 << 18) + 1, ctypes.byref(R)), "moe_route: at most"),
                       (lambda: lib.vgemm_moe_route(None, ctypes.byref(wide), 1, ctypes.byref(R)), "ld8 above"),
                       (lambda: lib.vgemm_moe(None, ctypes.byref(wide), 1, ctypes.byref(P)), "ld8 above"),
-                      (lambda: lib.vgemm_rmsnorm_q(None, FAKE, None, (1 << 23) + 1, 64, FAKE, 100000, None, FAKE, None, FAKE, 64), "rmsnorm_q: at most")):
+                      (lambda: lib.vgemm_rmsnorm_q(None, FAKE, None, (1 << 22) + 1, 64, FAKE, 100000, None, FAKE, None, FAKE, 64), "rmsnorm_q: at most")):
         assert call() == -3 and msg in last()
 
 

@@ -55,8 +55,8 @@ vk::W4View w4_view(const VgemmW4& W) {
 
 // strides that keep the rows a kernel addresses with 32-bit offsets within 2^30 bytes: 512 int8 rows, 32 int32 rows
 constexpr int MAX_LD8 = 1 << 21, MAX_LDX = 1 << 23;
-// rows of a call: what a grid holds
-constexpr int MAX_ROWS = 1 << 20, MAX_NORM_ROWS = 1 << 23;
+// rows of a call: what a grid holds (65535 tiles of eight rows along its second axis, 2^32 threads)
+constexpr int MAX_ROWS = 1 << 18, MAX_NORM_ROWS = 1 << 22;
 
 int rows_limit(const char* what, int M, int most) { return M > most ? fail(VGEMM_ERR_UNSUPPORTED, "%s: at most %d rows a call, not %d", what, most, M) : VGEMM_OK; }
 
