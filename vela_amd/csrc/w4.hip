@@ -8,76 +8,73 @@ namespace vk {
 
 // ---------------------------------------------------------------- layout
 
-// One thread per 16 bytes of a tile (a lane's share): grid.x over tiles of a matrix, grid.y over matrices.
-__global__ void __launch_bounds__(256) w4_pack_kernel(int N, int K, int group, uint8_t* __restrict__ q, size_t stride, const uint8_t* __restrict__ nib, int ldn,
-                                                      const uint16_t* __restrict__ scale, const uint8_t* __restrict__ zero, int lds) {
-    const int KT = w4_kt(K), CT = w4_ct(N), NG = 128 / group;
-    const int tile = int(blockIdx.x) * 4 + int(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (tile >= CT * KT) return;
-    const int ct = tile / KT, kt = tile - ct * KT, n = ct * 16 + (lane & 15), j = lane >> 4;
+// A block per column tile, a wave every fourth of its tiles of K, a lane its 16 bytes of the tile: four pieces of eight nibbles, piece
+// (h, i) half h of bytes 8 i and on. The column constants' wsum = sum of (u - z) sc goes along: |wsum| <= 32768 * 15 * 4095 < 2^31.
+// 4096 x 22016 with groups of 128: 87 us (a thread a byte, the sums by a second kernel: 173 + 111 us).
+template <int G>
+__global__ void __launch_bounds__(256) w4_pack_kernel(int N, int K, uint8_t* __restrict__ q, size_t stride, int4* __restrict__ cst, const uint8_t* __restrict__ nib, int ldn,
+                                                      const uint16_t* __restrict__ scale, const uint8_t* __restrict__ zero, int lds, const int32_t* __restrict__ msb) {
+    constexpr int NG = 128 / G;
+    __shared__ int s_sum[4][16];
+    const int KT = w4_kt(K), CT = w4_ct(N), ct = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = ct * 16 + (lane & 15), j = lane >> 4;
     q += stride * blockIdx.y;
     const size_t row = size_t(blockIdx.y) * N + n;
-    uint8_t b[16];
+    const auto zero_of = [&](int g) { return zero ? unsigned(zero[row * lds + g] & 15) : 8u; };
+    const auto scale_of = [&](int g) { return min(unsigned(scale[row * lds + g]), 4095u); };
+    int sum = 0;
+    for (int kt = wave; kt < KT; kt += 4) {
+        unsigned x[2][2] = {{0, 0}, {0, 0}};   // a piece's nibbles in order
+        if (n < N) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = 0;
-    if (n < N) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            unsigned v = 0;
             for (int h = 0; h < 2; ++h) {
-                const int k = kt * 128 + 64 * h + (group == 32 ? 32 * (i >> 3) + 8 * j + (i & 7) : 16 * j + i);
-                unsigned u = 8;
-                if (k < K) u = (nib[row * ldn + (k >> 1)] >> (4 * (k & 1))) & 15u;
-                else if (zero) u = zero[row * lds + min(k / group, (K - 1) / group)] & 15u;
-                v |= u << (4 * h);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = kt * 128 + 64 * h + (G == 32 ? 32 * i + 8 * j : 16 * j + 8 * i);
+                    const int g = min(k, K - 1) / G;
+                    const unsigned z = zero_of(g);
+                    if (k + 8 <= K) {
+                        __builtin_memcpy(&x[h][i], nib + row * ldn + (k >> 1), 4);   // at any address
+                    } else {
+                        for (int e = 0; e < 8; ++e) {   // past the row's end: the zero point
+                            const unsigned u = k + e < K ? (nib[row * ldn + ((k + e) >> 1)] >> (4 * (e & 1))) & 15u : z;
+                            x[h][i] |= u << (4 * e);
+                        }
+                    }
+                    const int s = __builtin_amdgcn_udot4(x[h][i] & 0x0f0f0f0fu, 0x01010101u, __builtin_amdgcn_udot4(x[h][i] >> 4 & 0x0f0f0f0fu, 0x01010101u, 0u, false), false);
+                    sum += (s - 8 * int(z)) * int(scale_of(g));
+                }
             }
-            b[i] = uint8_t(v);
+        }
+        uint4 w;
+        unsigned* wp = &w.x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {   // byte b of a piece: nibble b of both halves
+            const unsigned even = (x[0][i] & 0x0f0f0f0fu) | (x[1][i] << 4 & 0xf0f0f0f0u), odd = (x[0][i] >> 4 & 0x0f0f0f0fu) | (x[1][i] & 0xf0f0f0f0u);
+            wp[2 * i] = __builtin_amdgcn_perm(odd, even, 0x05010400u);
+            wp[2 * i + 1] = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+        }
+        const size_t tile = size_t(ct) * KT + kt;
+        reinterpret_cast<uint4*>(q + tile * 1024)[lane] = w;
+        uint16_t* words = reinterpret_cast<uint16_t*>(q + size_t(CT) * KT * 1024 + tile * 32 * NG);
+        if (j < NG) {   // column lane & 15, group j of the tile
+            const int g = kt * NG + j;
+            words[(lane & 15) * NG + j] = uint16_t(n < N && g * G < K ? zero_of(g) << 12 | scale_of(g) : 8u << 12);
         }
     }
-    uint4 w;
-    w.x = b[0] | b[1] << 8 | b[2] << 16 | unsigned(b[3]) << 24;
-    w.y = b[4] | b[5] << 8 | b[6] << 16 | unsigned(b[7]) << 24;
-    w.z = b[8] | b[9] << 8 | b[10] << 16 | unsigned(b[11]) << 24;
-    w.w = b[12] | b[13] << 8 | b[14] << 16 | unsigned(b[15]) << 24;
-    reinterpret_cast<uint4*>(q + size_t(tile) * 1024)[lane] = w;
-    uint16_t* s = reinterpret_cast<uint16_t*>(q + size_t(CT) * KT * 1024 + size_t(tile) * 32 * NG);
-    for (int i = lane; i < 16 * NG; i += 64) {
-        const int c = i / NG, g = kt * NG + i % NG, m = ct * 16 + c;
-        unsigned word = 8u << 12;
-        if (m < N && g * group < K) {
-            const size_t at = (size_t(blockIdx.y) * N + m) * lds + g;
-            word = (zero ? zero[at] & 15u : 8u) << 12 | min(unsigned(scale[at]), 4095u);
-        }
-        s[i] = uint16_t(word);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (lane < 16) s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        const int all = s_sum[0][lane] + s_sum[1][lane] + s_sum[2][lane] + s_sum[3][lane];
+        cst[size_t(blockIdx.y) * CT * 16 + n] = n < N ? make_int4(msb[4 * row], msb[4 * row + 1], msb[4 * row + 2], all) : make_int4(0, 0, 0, 0);
     }
-}
-
-// cst of column n: {m, s, b} as given and wsum = sum of (u - z) sc, |wsum| <= 32768 * 15 * 4095 < 2^31. One wave per column.
-__global__ void __launch_bounds__(256) w4_cst_kernel(int N, int K, int group, int4* __restrict__ cst, const uint8_t* __restrict__ nib, int ldn,
-                                                     const uint16_t* __restrict__ scale, const uint8_t* __restrict__ zero, int lds, const int32_t* __restrict__ msb) {
-    const int n = int(blockIdx.x) * 4 + int(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int N16 = w4_ct(N) * 16;
-    if (n >= N16) return;
-    int4 c = make_int4(0, 0, 0, 0);
-    if (n < N) {
-        const size_t row = size_t(blockIdx.y) * N + n;
-        int sum = 0;
-        for (int k = lane; k < K; k += 64) {
-            const int g = k / group, u = (nib[row * ldn + (k >> 1)] >> (4 * (k & 1))) & 15;
-            sum += (u - (zero ? int(zero[row * lds + g] & 15) : 8)) * min(int(scale[row * lds + g]), 4095);
-        }
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        c = make_int4(msb[4 * row], msb[4 * row + 1], msb[4 * row + 2], sum);
-    }
-    if (lane == 0) cst[size_t(blockIdx.y) * N16 + n] = c;
 }
 
 hipError_t launch_w4_pack(hipStream_t st, int N, int K, int group, uint8_t* q, int4* cst, int n, const uint8_t* nib, int ldn, const uint16_t* scale,
                           const uint8_t* zero, int lds, const int32_t* msb) {
-    const int tiles = w4_ct(N) * w4_kt(K);
-    const size_t stride = w4_bytes(N, K, group);
-    hipLaunchKernelGGL(w4_pack_kernel, dim3(cdiv(tiles, 4), n), dim3(256), 0, st, N, K, group, q, stride, nib, ldn, scale, zero, lds);
-    hipLaunchKernelGGL(w4_cst_kernel, dim3(cdiv(w4_ct(N) * 16, 4), n), dim3(256), 0, st, N, K, group, cst, nib, ldn, scale, zero, lds, msb);
+    const auto kernel = group == 32 ? w4_pack_kernel<32> : (group == 64 ? w4_pack_kernel<64> : w4_pack_kernel<128>);
+    hipLaunchKernelGGL(kernel, dim3(w4_ct(N), n), dim3(256), 0, st, N, K, q, w4_bytes(N, K, group), cst, nib, ldn, scale, zero, lds, msb);
     return hipGetLastError();
 }
 
