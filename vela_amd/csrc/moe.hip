@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     __shared__ __align__(16) int s_z[MOE_EXPERTS + 16];
     __shared__ int s_h[MOE_EXPERTS], s_l[MOE_EXPERTS];
     __shared__ int s_top[MOE_TOPK];
-    __shared__ i64 s_exp[EXP_N], s_sum[ROUTE_THREADS / 64];
+    __shared__ i64 s_exp[EXP_N];
+    __shared__ u64 s_sum[ROUTE_THREADS / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x;
     const int8_t* hi = a.hi + size_t(t) * a.ld8;
     const int8_t* lo = a.lo ? a.lo + size_t(t) * a.ld8 : nullptr;
@@ -208,14 +209,17 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
     const uint32_t top = uint32_t(s_top[0]);
     const i64 mine = i < a.topk ? moe_lutexp(top - uint32_t(s_top[i]), s_exp) : 0;   // the i-th choice's
     const int members = a.renorm ? a.topk : a.experts;
+    u64 sum = 0;   // of this wave's members; the chosen ones are all in the first wave, and each of its lanes has their sum
     if (64 * wave < members) {
-        const i64 part = a.renorm ? mine : (i < a.experts ? moe_lutexp(top - uint32_t(z), s_exp) : 0), sum = wave_sum64(part);
-        if (lane == 0) s_sum[wave] = sum;
+        sum = u64(wave_sum64(a.renorm ? mine : (i < a.experts ? moe_lutexp(top - uint32_t(z), s_exp) : 0)));
+        if (!a.renorm && lane == 0) s_sum[wave] = sum;
     }
-    if (!a.renorm) __syncthreads();   // the chosen are all in the first wave
+    if (!a.renorm) __syncthreads();
     if (i < a.topk) {
-        u64 sum = 0;
-        for (int w = 0; 64 * w < members; ++w) sum += u64(s_sum[w]);
+        if (!a.renorm) {
+            sum = 0;
+            for (int w = 0; 64 * w < members; ++w) sum += s_sum[w];
+        }
         const u64 p = (u64(mine) * route_recip(sum) + (u64(1) << 46)) >> 47;
         a.p[size_t(t) * a.topk + i] = int(min(p, u64(32767)));
     }

@@ -159,12 +159,6 @@ struct W4Chunks {
     }
 };
 
-// orders a wave's LDS accesses for its other lanes (LDS operations of a wave run in order)
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // i / per by a multiplication, for i * per < 2^32
 struct W4Per {
     unsigned per, m;
