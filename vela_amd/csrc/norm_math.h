@@ -64,20 +64,6 @@ __device__ __forceinline__ double wave_sumf64(double v) {
     v += dppf64<DPP_MIRROR>(v);
     return (readlanef64(v, 0) + readlanef64(v, 16)) + (readlanef64(v, 32) + readlanef64(v, 48));
 }
-__device__ __forceinline__ int wave_min32(int v) {
-    v = min(v, dpp32<DPP_XOR1>(v));
-    v = min(v, dpp32<DPP_XOR2>(v));
-    v = min(v, dpp32<DPP_HALF_MIRROR>(v));
-    v = min(v, dpp32<DPP_MIRROR>(v));
-    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-}
-__device__ __forceinline__ int wave_max32(int v) {
-    v = max(v, dpp32<DPP_XOR1>(v));
-    v = max(v, dpp32<DPP_XOR2>(v));
-    v = max(v, dpp32<DPP_HALF_MIRROR>(v));
-    v = max(v, dpp32<DPP_MIRROR>(v));
-    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-}
 __device__ __forceinline__ uint32_t wave_umax32(uint32_t v) {
     v = max(v, uint32_t(dpp32<DPP_XOR1>(int(v))));
     v = max(v, uint32_t(dpp32<DPP_XOR2>(int(v))));
