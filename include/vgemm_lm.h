@@ -54,7 +54,7 @@ int vgemm_w4_pack(void* stream, const VgemmW4* W, int first, int n, const uint8_
 
 /* Y = A W^T for M rows (W->count == 1): acc = sum_k q[r, k] w[n, k], y = sat32(rshr(acc m, s - e) + b) (acc m wraps in 64 bits),
  * then as vgemm_hl2's epilogues
- *   VGEMM_EPI_PLAIN  + residual (stride ldy, may be Y), saturated
+ *   VGEMM_EPI_PLAIN  + residual (stride ldy, may be Y), saturated; gnstat must be NULL
  *   VGEMM_EPI_GEGLU  columns (a, g) interleaved, N even: sat32(rshr(a sat32(rshr(g lut16i(g, Lphi), 16)), 16)); with a sigmoid
  *                    table it is a * SiLU(g)
  * and rowmax[r] = max(rowmax[r], |y|) when E->rowmax != NULL. A: VGEMM_SRC_I8 (lo may be NULL; ld8 >= K rounded up to 16, ld8 % 16

@@ -105,6 +105,7 @@ int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const Vg
     if (!A || !E || M < 0) return fail(VGEMM_ERR_ARG, "w4: bad arguments");
     if (int rc = w4_weights("w4", W)) return rc;
     if (W->count != 1) return fail(VGEMM_ERR_ARG, "w4: one matrix expected, not %d", W->count);
+    if (E->epi == VGEMM_EPI_PLAIN && E->gnstat) return fail(VGEMM_ERR_ARG, "w4: no GroupNorm statistics (gnstat must be NULL)");
     if (M == 0) return ok();
     if (int rc = rows_limit("w4", M, MAX_ROWS)) return rc;
     vk::W4Args a{};
