@@ -6,9 +6,10 @@ import torch
 
 from tests import lm_math as lm
 from tests.conftest import assert_equal, to_np
-from tests.test_gpu_lm import Rows, dev
+from tests.test_gpu_lm import Rows, dev, packed
 from vela_amd import gemm as vg
 from vela_amd import moe as vm
+from vela_amd import w4 as vw
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,26 @@ def test_route_shares_of_many_tokens(gpu, E, topk):
         vm.k_moe_route(rows.A, M, vm.MoeRoute(W=vg.ptr(dw), ldw=K, cst=vg.ptr(dc), experts=E, topk=topk, renorm=renorm, Lexp=vg.ptr(dl), idx=vg.ptr(di), p=vg.ptr(dp)))
         assert_equal(to_np(di), idx, f"renorm {renorm} idx")
         assert_equal(to_np(dp), p, f"renorm {renorm} p")
+
+
+def test_pack_of_sources_freed_at_once_on_a_busy_stream(gpu):
+    """Sources that nobody holds after the call, whose memory the next tensors of their own stream ask for while the packing
+    waits behind other work: as from sources that are kept."""
+    rng = np.random.default_rng(50)
+    w = lm.Weights(rng, 256, 2048, 64)
+    dense = packed(w)
+    a, b = torch.randn((4096, 4096), device="cuda"), torch.empty((4096, 4096), device="cuda")
+    W, st = vw.W4Weights(256, 2048, 64), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        for _ in range(20):
+            torch.mm(a, a, out=b)
+    parts = [dev(t) for t in (w.nib, w.sc, w.z, w.msb)]
+    shapes = [(t.shape, t.dtype) for t in parts]
+    st.wait_stream(torch.cuda.current_stream())
+    W.pack(*parts, stream=st)
+    del parts
+    junk = [torch.full(s, 85, dtype=dt, device="cuda") for s, dt in shapes for _ in range(3)]
+    torch.cuda.synchronize()
+    assert torch.equal(W.q, dense.q) and torch.equal(W.cst, dense.cst)
+    assert all(bool((t == 85).all()) for t in junk)

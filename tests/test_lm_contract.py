@@ -1,11 +1,13 @@
 """The language-model operators without a GPU, beyond their argument checks: what the sources and the Python objects promise."""
+import contextlib
 import ctypes
 import re
 from pathlib import Path
 
 import pytest
+import torch
 
-from vela_amd import _lib
+from vela_amd import _lib, w4
 
 ROOT = Path(__file__).resolve().parent.parent
 CSRC = ROOT / "vela_amd" / "csrc"
@@ -32,3 +34,46 @@ def test_w4_statistics(epi, rc):
     A, E = _lib.ASrc(src=0, hi=FAKE, ld8=64), _lib.AEpi(epi=epi, Y=FAKE, ldy=64, Lphi=FAKE, gnstat=FAKE, gnT=64)
     assert lib.vgemm_w4(None, ctypes.byref(A), 0, ctypes.byref(W), ctypes.byref(E)) == rc
     assert ("statistics" in lib.vgemm_last_error().decode()) == (rc != 0)
+
+
+class PackCall:
+    """W4Weights.pack on CPU tensors with the library, the CUDA contexts and record_stream replaced by recorders."""
+
+    def __init__(self, monkeypatch, device="cuda:1"):
+        self.where, self.calls, self.recorded, self.device = [], [], [], torch.device(device)
+        me = self
+
+        class Lib:
+            def vgemm_w4_pack(self, stream, *args):
+                me.calls.append((stream, tuple(me.where)))
+                return 0
+
+        @contextlib.contextmanager
+        def enter(kind, what):
+            me.where.append((kind, what))
+            yield
+            me.where.pop()
+
+        monkeypatch.setattr(w4, "load", Lib)
+        monkeypatch.setattr(w4, "ptr", lambda t: None if t is None else t.data_ptr())
+        monkeypatch.setattr(w4, "stream_ptr", lambda s=None: ("raw", s))
+        monkeypatch.setattr(torch.cuda, "device", lambda d: enter("device", d))
+        monkeypatch.setattr(torch.cuda, "stream", lambda s: enter("stream", s))
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: "current")
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda raw, device=None: ("external", raw))
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: me.recorded.append((t.data_ptr(), s)))
+        self.W = w4.W4Weights.__new__(w4.W4Weights)
+        self.W.N, self.W.K, self.W.group, self.W.count, self.W.desc = 8, 64, 32, 1, _lib.W4()
+        self.W.q, self.W.cst = torch.zeros(2048, dtype=torch.uint8), torch.zeros((1, 16, 4), dtype=torch.int32)
+        self.parts = [torch.zeros((8, 32), dtype=torch.uint8), torch.zeros((8, 2), dtype=torch.int16), torch.zeros((8, 2), dtype=torch.uint8),
+                      torch.zeros((8, 4), dtype=torch.int32)]
+
+
+@pytest.mark.parametrize("stream", [None, "side", 1234])
+def test_pack_keeps_memory_until_its_stream_is_done(monkeypatch, stream):
+    """The sources may be freed right after the call, and so may the weights: the allocator has to know the stream that uses them."""
+    c = PackCall(monkeypatch)
+    c.W.pack(*c.parts, stream=stream)
+    assert len(c.calls) == 1
+    used = {t.data_ptr() for t in (*c.parts, c.W.q, c.W.cst)}
+    assert {p for p, _ in c.recorded} == used and {s for _, s in c.recorded} == {"current"}   # the one made current for the call

@@ -35,7 +35,7 @@ class W4Weights:
     def pack(self, nib: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, msb: torch.Tensor, first: int = 0, stream=None) -> None:
         """Lay out matrices first, first + 1, ...: nib uint8 [(n,) N, >= K/2] (column 2i in the low half of byte i), scale
         int16 or uint16 [(n,) N, groups], zero uint8 alike or None (8 throughout), msb int32 [(n,) N, 4] {m, s, b, unused}. Row
-        strides may be larger than the rows."""
+        strides may be larger than the rows. The sources need not be kept after the call."""
         N, groups = self.N, (self.K + self.group - 1) // self.group
         n = nib.shape[0] if nib.dim() == 3 else 1
         # from one row to the next, over all matrices
@@ -60,6 +60,9 @@ class W4Weights:
             msb = rows(msb, (torch.int32,), 4, "msb")[..., :4].contiguous()
             check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
                                        ptr(msb)))
+            for t in (nib, scale, zero, msb, self.q, self.cst):   # none of them is reused, once freed, before the kernel is done
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream())
 
 
 def k_gemm_w4(A: ASrc, M: int, W: W4Weights | W4, E: AEpi, stream=None) -> None:
