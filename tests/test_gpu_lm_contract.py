@@ -34,21 +34,23 @@ def test_route_shares_of_many_tokens(gpu, E, topk):
         assert_equal(to_np(dp), p, f"renorm {renorm} p")
 
 
-def test_pack_of_sources_freed_at_once_on_a_busy_stream(gpu):
+@pytest.mark.parametrize("strided", [False, True])
+def test_pack_of_sources_freed_at_once_on_a_busy_stream(gpu, strided):
     """Sources that nobody holds after the call, whose memory the next tensors of their own stream ask for while the packing
-    waits behind other work: as from sources that are kept."""
+    waits behind other work, or first the copies of rows that are laid out otherwise: as from sources that are kept."""
     rng = np.random.default_rng(50)
     w = lm.Weights(rng, 256, 2048, 64)
     dense = packed(w)
     a, b = torch.randn((4096, 4096), device="cuda"), torch.empty((4096, 4096), device="cuda")
     W, st = vw.W4Weights(256, 2048, 64), torch.cuda.Stream()
+    parts = [dev(t) for t in (w.nib, w.sc, w.z, w.msb)]
+    if strided:
+        parts = [t.t().contiguous().t() for t in parts]
+    shapes = [(t.shape, t.dtype) for t in parts]
     torch.cuda.synchronize()
     with torch.cuda.stream(st):
         for _ in range(20):
             torch.mm(a, a, out=b)
-    parts = [dev(t) for t in (w.nib, w.sc, w.z, w.msb)]
-    shapes = [(t.shape, t.dtype) for t in parts]
-    st.wait_stream(torch.cuda.current_stream())
     W.pack(*parts, stream=st)
     del parts
     junk = [torch.full(s, 85, dtype=dt, device="cuda") for s, dt in shapes for _ in range(3)]

@@ -77,3 +77,11 @@ def test_pack_keeps_memory_until_its_stream_is_done(monkeypatch, stream):
     assert len(c.calls) == 1
     used = {t.data_ptr() for t in (*c.parts, c.W.q, c.W.cst)}
     assert {p for p, _ in c.recorded} == used and {s for _, s in c.recorded} == {"current"}   # the one made current for the call
+
+
+def test_pack_keeps_sources_that_it_copies(monkeypatch):
+    """Rows that are laid out otherwise are copied on the call's stream, which reads the given ones."""
+    c = PackCall(monkeypatch)
+    strided = [torch.zeros((t.shape[1], t.shape[0]), dtype=t.dtype).t() for t in c.parts]
+    c.W.pack(*strided, stream="side")
+    assert {t.data_ptr() for t in strided} <= {p for p, _ in c.recorded}

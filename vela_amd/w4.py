@@ -41,28 +41,30 @@ class W4Weights:
         # from one row to the next, over all matrices
         pitch = lambda t: t.stride(-2) if N > 1 else (t.stride(0) if n > 1 else t.shape[-1])  # noqa: E731
 
-        def rows(t, dtypes, width, name):
+        sources = [("nib", nib, (torch.uint8,), (self.K + 1) // 2), ("scale", scale, (torch.int16, torch.uint16), groups), ("zero", zero, (torch.uint8,), groups),
+                   ("msb", msb, (torch.int32,), 4)]
+        for name, t, dtypes, width in sources:
+            if t is None and name == "zero":
+                continue
             shape = (n, N) if nib.dim() == 3 else (N,)
             if t.dtype not in dtypes or t.dim() != nib.dim() or tuple(t.shape[:-1]) != shape or t.shape[-1] < width or t.device != self.q.device:
                 raise ValueError(f"W4Weights.pack: {name} of shape {tuple(t.shape)}, {t.dtype} on {t.device}")
-            if t.stride(-1) != 1 or pitch(t) < t.shape[-1] or (n > 1 and t.stride(0) != N * pitch(t)):
-                t = t.contiguous()
-            return t
+
+        def rows(t):
+            return t.contiguous() if t.stride(-1) != 1 or pitch(t) < t.shape[-1] or (n > 1 and t.stride(0) != N * pitch(t)) else t
 
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream)
         with torch.cuda.stream(stream):   # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
-            nib = rows(nib, (torch.uint8,), (self.K + 1) // 2, "nib")
-            scale = rows(scale, (torch.int16, torch.uint16), groups, "scale")
-            zero = rows(zero, (torch.uint8,), groups, "zero") if zero is not None else None
-            if zero is not None and pitch(zero) != pitch(scale):
-                scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
-            msb = rows(msb, (torch.int32,), 4, "msb")[..., :4].contiguous()
-            check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
-                                       ptr(msb)))
-            for t in (nib, scale, zero, msb, self.q, self.cst):   # none of them is reused, once freed, before the kernel is done
+            for t in (nib, scale, zero, msb, self.q, self.cst):   # none of them is reused, once freed, before the call's work is done
                 if t is not None:
                     t.record_stream(torch.cuda.current_stream())
+            nib, scale, zero = rows(nib), rows(scale), rows(zero) if zero is not None else None
+            if zero is not None and pitch(zero) != pitch(scale):
+                scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
+            msb = msb[..., :4].contiguous()
+            check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
+                                       ptr(msb)))
 
 
 def k_gemm_w4(A: ASrc, M: int, W: W4Weights | W4, E: AEpi, stream=None) -> None:
