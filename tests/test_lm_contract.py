@@ -2,6 +2,7 @@
 import contextlib
 import ctypes
 import re
+import types
 from pathlib import Path
 
 import pytest
@@ -85,3 +86,21 @@ def test_pack_keeps_sources_that_it_copies(monkeypatch):
     strided = [torch.zeros((t.shape[1], t.shape[0]), dtype=t.dtype).t() for t in c.parts]
     c.W.pack(*strided, stream="side")
     assert {t.data_ptr() for t in strided} <= {p for p, _ in c.recorded}
+
+
+@pytest.mark.parametrize("stream", [None, "side", 1234])
+def test_pack_runs_on_the_device_of_the_weights(monkeypatch, stream):
+    """Whatever device is current; a raw handle is one of that device."""
+    c = PackCall(monkeypatch)
+    c.W.pack(*c.parts, stream=stream)
+    (given, where), = c.calls
+    kinds = [k for k, _ in where]
+    assert where[0] == ("device", c.W.q.device) and kinds == ["device", "stream"]
+    assert where[1] == ("stream", ("external", 1234) if stream == 1234 else stream)
+
+
+def test_pack_refuses_a_stream_of_another_device(monkeypatch):
+    c = PackCall(monkeypatch)
+    with pytest.raises(ValueError, match="stream of cuda:3"):
+        c.W.pack(*c.parts, stream=types.SimpleNamespace(device=torch.device("cuda:3"), cuda_stream=5))
+    assert not c.calls

@@ -35,7 +35,8 @@ class W4Weights:
     def pack(self, nib: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, msb: torch.Tensor, first: int = 0, stream=None) -> None:
         """Lay out matrices first, first + 1, ...: nib uint8 [(n,) N, >= K/2] (column 2i in the low half of byte i), scale
         int16 or uint16 [(n,) N, groups], zero uint8 alike or None (8 throughout), msb int32 [(n,) N, 4] {m, s, b, unused}. Row
-        strides may be larger than the rows. The sources need not be kept after the call."""
+        strides may be larger than the rows. The sources need not be kept after the call, which runs on the
+        weights' device whichever is current; stream, where given, is one of that device."""
         N, groups = self.N, (self.K + self.group - 1) // self.group
         n = nib.shape[0] if nib.dim() == 3 else 1
         # from one row to the next, over all matrices
@@ -53,9 +54,11 @@ class W4Weights:
         def rows(t):
             return t.contiguous() if t.stride(-1) != 1 or pitch(t) < t.shape[-1] or (n > 1 and t.stride(0) != N * pitch(t)) else t
 
-        if isinstance(stream, int):
-            stream = torch.cuda.ExternalStream(stream)
-        with torch.cuda.stream(stream):   # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
+        dev = self.q.device
+        if getattr(stream, "device", dev) != dev:
+            raise ValueError(f"W4Weights.pack: a stream of {stream.device} for weights on {dev}")
+        # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
+        with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
             for t in (nib, scale, zero, msb, self.q, self.cst):   # none of them is reused, once freed, before the call's work is done
                 if t is not None:
                     t.record_stream(torch.cuda.current_stream())
