@@ -36,7 +36,7 @@ int vgemm_rmsnorm_q(void* stream, const int32_t* X, const int32_t* R, int M, int
                     int32_t* e, int Kp);
 
 /* `count` matrices of N x K 4-bit weights, w[n, k] = (u[n, k] - z[n, k / group]) sc[n, k / group] with u, z in 0..15 and
- * sc in 0..4095; group 32, 64 or 128 (the last group of a row may be short), N >= 1, 1 <= K <= 32768. q holds count *
+ * sc in 0..4095; group 32, 64 or 128 (the last group of a row may be short), 1 <= N <= 2^24, 1 <= K <= 32768. q holds count *
  * vgemm_w4_bytes(N, K, group) bytes, cst [count x N16 x 4] int32 {m, s, b, wsum} with N16 = N rounded up to 16; both
  * 16-byte aligned, written by vgemm_w4_pack. */
 typedef struct VgemmW4 {

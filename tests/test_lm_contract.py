@@ -104,3 +104,13 @@ def test_pack_refuses_a_stream_of_another_device(monkeypatch):
     with pytest.raises(ValueError, match="stream of cuda:3"):
         c.W.pack(*c.parts, stream=types.SimpleNamespace(device=torch.device("cuda:3"), cuda_stream=5))
     assert not c.calls
+
+
+def test_most_columns():
+    """2^24 columns a matrix, with the limit in the message."""
+    lib = _lib.load()
+    assert w4.w4_bytes(1 << 24, 64, 64) > 0 and w4.w4_bytes((1 << 24) + 1, 64, 64) == 0
+    W = _lib.W4(N=(1 << 24) + 1, K=64, group=64, count=1, q=FAKE, cst=FAKE)
+    A, E = _lib.ASrc(src=0, hi=FAKE, ld8=64), _lib.AEpi(Y=FAKE, ldy=1 << 25)
+    assert lib.vgemm_w4(None, ctypes.byref(A), 1, ctypes.byref(W), ctypes.byref(E)) == -1
+    assert "N <= 2^24" in lib.vgemm_last_error().decode()

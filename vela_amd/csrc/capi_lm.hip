@@ -43,7 +43,7 @@ bool w4_shape(int N, int K, int group) { return N >= 1 && N <= (1 << 24) && K >=
 int w4_weights(const char* what, const VgemmW4* W) {
     if (!W || !W->q || !W->cst || !aligned(W->q, 16) || !aligned(W->cst, 16) || W->count < 1)
         return fail(VGEMM_ERR_ARG, "%s: weights need q and cst, 16-byte aligned, and count >= 1", what);
-    if (!w4_shape(W->N, W->K, W->group)) return fail(VGEMM_ERR_ARG, "%s: weights need N >= 1, 1 <= K <= 32768 and a group of 32, 64 or 128", what);
+    if (!w4_shape(W->N, W->K, W->group)) return fail(VGEMM_ERR_ARG, "%s: weights need N >= 1, N <= 2^24, 1 <= K <= 32768 and a group of 32, 64 or 128", what);
     return VGEMM_OK;
 }
 

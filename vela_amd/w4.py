@@ -26,7 +26,7 @@ class W4Weights:
     def __init__(self, N: int, K: int, group: int, count: int = 1, device="cuda"):
         nb = w4_bytes(N, K, group)
         if not nb or count < 1:
-            raise ValueError(f"W4Weights: N >= 1, 1 <= K <= 32768, group 32, 64 or 128 and count >= 1 expected, got {N}, {K}, {group}, {count}")
+            raise ValueError(f"W4Weights: 1 <= N <= 2^24, 1 <= K <= 32768, group 32, 64 or 128 and count >= 1 expected, got {N}, {K}, {group}, {count}")
         self.N, self.K, self.group, self.count = N, K, group, count
         self.q = torch.empty(count * nb, dtype=torch.uint8, device=device)
         self.cst = torch.empty((count, (N + 15) // 16 * 16, 4), dtype=torch.int32, device=device)
