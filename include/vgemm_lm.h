@@ -90,6 +90,7 @@ typedef struct VgemmMoe {
     int32_t* Y; int ldy; const int32_t* residual;
     void* ws; size_t ws_bytes;
 } VgemmMoe;
+/* 0: no tokens, or a topk or F that a layer does not take */
 size_t vgemm_moe_workspace_bytes(int M, int topk, int F);
 int vgemm_moe(void* stream, const VgemmASrc* A, int M, const VgemmMoe* P);
 

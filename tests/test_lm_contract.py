@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from vela_amd import _lib, w4
+from vela_amd import _lib, moe, w4
 
 ROOT = Path(__file__).resolve().parent.parent
 CSRC = ROOT / "vela_amd" / "csrc"
@@ -114,3 +114,13 @@ def test_most_columns():
     A, E = _lib.ASrc(src=0, hi=FAKE, ld8=64), _lib.AEpi(Y=FAKE, ldy=1 << 25)
     assert lib.vgemm_w4(None, ctypes.byref(A), 1, ctypes.byref(W), ctypes.byref(E)) == -1
     assert "N <= 2^24" in lib.vgemm_last_error().decode()
+
+
+@pytest.mark.parametrize("F", [-4, 0, 63, 32772, 1 << 30, (1 << 31) - 4])
+def test_no_workspace_for_sizes_a_layer_does_not_take(F):
+    assert moe.moe_workspace_bytes(3, 2, F) == 0
+
+
+def test_workspace_of_the_widest_experts():
+    pairs, F = 512, 32768   # the rows of v and of a pass of the down product, the maxima of v's column tiles
+    assert moe.moe_workspace_bytes(1 << 30, 16, F) == pairs * (F + 8192 + 2 * F // 16) * 4

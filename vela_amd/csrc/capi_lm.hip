@@ -154,7 +154,7 @@ int vgemm_moe_route(void* stream, const VgemmASrc* A, int M, const VgemmMoeRoute
 static int moe_pass(int M, int topk) { return std::min(M, vk::MOE_PAIRS / topk); }
 
 size_t vgemm_moe_workspace_bytes(int M, int topk, int F) {
-    if (M <= 0 || topk < 1 || topk > vk::MOE_TOPK || F < 1) return 0;
+    if (M <= 0 || topk < 1 || topk > vk::MOE_TOPK || F < 1 || F > 32768 || F % 4) return 0;
     return size_t(moe_pass(M, topk)) * topk * (size_t(F) + vk::MOE_COLS + vk::w4_ct(2 * F)) * 4;
 }
 
