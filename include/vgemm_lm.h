@@ -1,6 +1,8 @@
 /*
  * vgemm_lm -- operators of a language model's decode step in the library's exact integer arithmetic: part of
- * libvgemm.so, beside the W8A16 products, norms and GEGLU blocks of vgemm.h. No counterparts in the reference.
+ * libvgemm.so, beside the W8A16 products, norms and GEGLU blocks of vgemm.h. No counterparts in the reference. Of such a
+ * step these are the norms, the projections and the feed-forward layers, dense or of experts; rotary positions, attention over a
+ * cache and sampling are not there, and no engine block or container of vgemm_engine.h / vgemm_model.h uses them.
  *
  *   vgemm_rmsnorm_q     residual addition, root-mean-square norm, 8-bit rows (or the int16 view)
  *   vgemm_w4_pack       4-bit weights with group scales and zero points, laid out for the products
@@ -59,7 +61,7 @@ int vgemm_w4_pack(void* stream, const VgemmW4* W, int first, int n, const uint8_
  *                    table it is a * SiLU(g)
  * and rowmax[r] = max(rowmax[r], |y|) when E->rowmax != NULL. A: VGEMM_SRC_I8 (lo may be NULL; ld8 >= K rounded up to 16, ld8 % 16
  * == 0, 16-byte aligned planes; columns past K are not used) or VGEMM_SRC_X32 (K == W->K, K % 4 == 0; row maxima in
- * rowmax). Made for rows up to a few tens: the weights are read once for every 16 or 32 of them.
+ * rowmax). Made for rows up to a few tens: the weights are read once for every 8, 16 or 32 of them.
  * M <= 2^18, ld8 <= 2^21, ldx <= 2^23 (else VGEMM_ERR_UNSUPPORTED). M == 0 is a no-op. */
 int vgemm_w4(void* stream, const VgemmASrc* A, int M, const VgemmW4* W, const VgemmAEpi* E);
 

@@ -227,8 +227,9 @@ __global__ void __launch_bounds__(ROUTE_THREADS) moe_route_kernel(RouteArgs a) {
 
 hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
     const int waves = ROUTE_THREADS / 64;
-    // One block reads 256 x 7168 in 25.8 us, 512 x 16384 in 92: with room for the logits a kernel before computes them on many CUs, 3.8 + 4.9
-    // and 4.9 + 4.7 us (128 x 2048 takes 6.6 us in one)
+    // One block reads 256 x 7168 in 26.0 us, 512 x 4096 in 29.2: with room for the logits a kernel before computes them on many CUs, 3.7 + 4.8
+    // and 3.2 + 4.7 us. 128 x 2048 takes 6.8 us in one kernel and 3.1 + 3.1 in two for one token, 7.4 and 4.1 + 4.0 for sixteen, 129 x 2048 8.9
+    // and 3.1 + 4.8: the tokens, each with a block of its own either way, change little of it.
     if (a.logits && (long long)a.experts * a.K > ROUTE_ONE) {
         if (M < 4) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(M, cdiv(a.experts, LOGITS_X)), dim3(256), 0, st, a, M);
         else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(cdiv(M, 4), cdiv(a.experts, LOGITS_X)), dim3(256), 0, st, a, M);
@@ -247,7 +248,7 @@ hipError_t launch_moe_route(hipStream_t st, const RouteArgs& a, int M) {
 // Both products are cut into items (row tile of at most 16 of an expert's pairs, segment of `js` column tiles), a block each,
 // which computes as w4_kernel.h says. Bound by the chosen experts' weights where there are many (16 tokens x 8 of 128, 2048 x 768, groups of
 // 64: up 29.4 us for 135 MB, down 19.0 for 67) or they are large (2 tokens x 8 of 256, 7168 x 2048: up 47.7 us for 240 MB, down 26.8 for
-// 120), else by a block's chain of latencies (one token x 2 of 8, 1024 x 2048: 5.7 and 5.2 us).
+// 120), else by a block's chain of latencies (one token x 2 of 8, 1024 x 2048: 5.7 and 5.6 us).
 
 // Row tile `tile` of the pairs sorted by expert: its expert and rows; n = 0 past the last tile. pair[]: the tile's pairs, the same in every
 // block (in the order of the pairs), written by the first wave. Every block finds its own: a kernel that did it once took 2 to 5 us.
@@ -347,7 +348,9 @@ __global__ void __launch_bounds__(1024) moe_kernel(MoeArgs a, int js, int rows_l
     ring.start(from, KT, tiles, 0, ch, lane, wave, waves);
     for (int k = threadIdx.x; k < tiles * 256; k += blockDim.x) sums[k] = 0;
     if (int(threadIdx.x) < n) s_max[threadIdx.x] = 0;
-    // two columns a thread; its first two's constants come from here on, in the down product, which has no registers for them, from its end
+    // two columns a thread; its first two's constants are asked for here, in the down product, which has no registers for them, at its
+    // end. The barrier that publishes the pairs waits for them, the first tiles and the gate's table, before the rows are asked for; so
+    // does the one between chunks for the next chunk's first tiles.
     const int outs = tiles * n * 8, TR = n <= 4 ? 4 : 16;
     const int4* cst = W.cst + size_t(x) * W.CT * 16;
     int4 c0, c1;
@@ -544,10 +547,19 @@ hipError_t launch_moe(hipStream_t st, const MoeArgs& args) {
     if (a.lo) moe_product<false, 2>(st, a, a.group_up, up);
     else moe_product<false, 1>(st, a, a.group_up, up);
     if (hipError_t e = hipGetLastError()) return e;
-    // Few pairs, rows that fit in LDS: their products and the sums at once, 4 tokens of 8 experts x 2, 4096 x 1536: 8.8 against 13.3 + 4.7 us; 24
-    // pairs of 64 experts, 2048 x 1408, 14.5 against 11.7 + 4.0, 32 pairs 17.2 against 12.5 + 4.0. A pair
-    // reads its expert's matrix by itself: not where that is more than 64 MB beyond a read each of the chosen experts (16 pairs of 2
-    // experts: 4096 x 1536, 44 MB, 11.5 against 9.2 + 4.5 us; 4096 x 4480, 129 MB, 28.2 against 13.0 + 4.7).
+    // Few pairs, rows that fit in LDS: their products and the sums at once. One kernel against two, us:
+    //   pairs  experts                 one     two
+    //     8       8    4096 x 1536     8.6    12.8 + 3.9
+    //    12      64    2048 x 1408     9.1     9.2 + 4.6
+    //    24      64    2048 x 1408    14.1    11.1 + 4.7
+    //    24      32    1024 x 512      8.6     7.0 + 3.9
+    //    24       8    2048 x 2048    16.3    10.3 + 4.7
+    //    24     256    4096 x 512      9.8    10.6 + 4.7
+    //    32      64    2048 x 1408    17.7    14.7 + 4.7
+    //    32      16    2048 x 768     11.4     7.8 + 4.0
+    //    32     256    4096 x 512     12.0    11.9 + 4.7
+    // A pair reads its expert's matrix by itself: not where that is more than 64 MB beyond a read each of the chosen experts (16 pairs of
+    // 2 experts: 4096 x 1536, 44 MB, 11.3 against 8.8 + 4.5; 4096 x 4480, 129 MB, 24.5 against 12.8 + 4.6).
     const int pairs = a.M * a.topk, js = std::min(8, cdiv(a.down.CT, NCU)), rows = pairs * 2 * (a.down.KT * 128 + 16);
     if (pairs <= MOE_FEW && rows + pairs * js * 512 + a.M * js * 128 + 2 * MOE_FEW * 4 <= 160 << 10 && (pairs - moe_chosen(a)) * double(a.down_stride) <= 64e6) {
         if (a.group_down == 32) moe_down_few<32>(st, a, js, rows);

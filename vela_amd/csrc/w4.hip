@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(1024) w4_kernel(W4Args a, int js, W4Chunks ch,
     const W4Columns from{a.w.q + size_t(ct0) * KT * 1024, a.w.s + size_t(ct0) * KT * (4096 / G), KT};
     const bool x32 = P == 2 && a.x;
     W4Ring<G, DEPTH> ring;
-    int e = 0;   // of row threadIdx.x, asked for before the tiles so that nobody waits for those
+    int e = 0;   // of row threadIdx.x. Storing it to s_e waits for every load asked for until then (how many is not known at compile
+                 // time), the first tiles and the gate's table among them, and the rows are asked for only after that
     if (int(threadIdx.x) < rows) e = x32 ? rowexp_u32(a.xmax[row0 + threadIdx.x]) : (a.e ? a.e[row0 + threadIdx.x] : 0);
     for (int i = threadIdx.x; i < tiles * TR * 16; i += blockDim.x) sums[i] = 0;
     ring.start(from, KT, tiles, 0, ch, lane, wave, waves);
@@ -208,21 +209,22 @@ static void w4_planes(hipStream_t st, const W4Args& a) {
 // More than sixteen rows go in blocks of 16 where a block then has few column tiles, so that staging (and quantising) the rows counts
 // more than reading the weights again, else in blocks of 32; int32 rows by the same reason in blocks of 8:
 //                                   16        32 rows a block
-//   int32, 32 x 11008 x 4096        23.0      44.1 us    2 column tiles a block of 16 rows
-//          64 x 4096 x 12288        23.1      24.8      12
-//          64 x 4096 x 22016        38.4      36.2      22
-//   16-bit, 32 x 11008 x 4096       14.7      21.2       2
-//          128 x 4096 x 4096        14.4      14.0       8
-//          64 x 4096 x 12288        20.2      19.2      12
-//   8-bit, 32 x 11008 x 4096        11.5      13.0       2
-//          20 x 4096 x 4096          6.2       6.0       2
-//          128 x 4096 x 4096        11.8      10.0       8
-//          32 x 4096 x 22016        18.2      12.8      11
+//   int32, 32 x 11008 x 4096        22.7      46.9 us    2 column tiles a block of 16 rows
+//          64 x 4096 x 12288        20.6      23.0      12
+//          64 x 4096 x 22016        37.4      40.3      22
+//   16-bit, 32 x 11008 x 4096       15.1      21.9       2
+//          128 x 4096 x 4096        14.5      14.3       8
+//          64 x 4096 x 12288        17.8      17.4      12
+//   8-bit, 32 x 11008 x 4096        11.3      12.8       2
+//          20 x 4096 x 4096          6.0       5.9       2
+//          128 x 4096 x 4096        11.9       9.3       8
+//          32 x 4096 x 22016        18.0      12.8      11
 //                                    8        16 rows a block
-//   int32, 16 x 11008 x 4096        15.0      20.5 us    2 column tiles a block of 8 rows
-//          32 x 11008 x 4096        20.1      22.9       4
-//          64 x 11008 x 4096        29.3      28.8       8
-//          16 x 4096 x 22016        20.3      15.8      11
+//   int32, 16 x 11008 x 4096        14.2      19.9 us    2 column tiles a block of 8 rows
+//          32 x 11008 x 4096        19.4      22.7       4
+//          64 x 11008 x 4096        28.2      28.1       8
+//          16 x 4096 x 22016        19.3      14.8      11
+// (Two medians differ by up to 5 %, so the line for int32 rows, between 12 and 22 tiles, could stand higher.)
 hipError_t launch_w4(hipStream_t st, const W4Args& a) {
     if (a.M <= 4) w4_planes<1, 1>(st, a);
     else if (a.M <= 8 || (a.x && w4_js(a, 8) <= 8)) w4_planes<1, 2>(st, a);

@@ -20,7 +20,7 @@
 // waves, which stream them with DEPTH tiles in flight and add each column tile's sums to 64-bit integers in LDS; the epilogue
 // reads those. Integer sums: their order does not matter.
 //
-// Bound by the weights' stream for a few rows (1 x 8192 x 28672, groups of 128: 24.0 us, 5.05 TB/s; 1 x 4096 x 22016 9.4-10 us), for tens
+// Bound by the weights' stream for a few rows (1 x 8192 x 28672, groups of 128: 24.0 us, 5.05 TB/s; 1 x 4096 x 22016 9.4-10.2 us), for tens
 // of rows by their staging and the groups' scaling (64 x 4096 x 22016 21.3 us; 51 x 2600 x 9999 in 16 bits, groups of 32, 18 us).
 #pragma once
 #include "vk_common.h"
