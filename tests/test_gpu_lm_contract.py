@@ -198,3 +198,23 @@ def test_moe_graph_of_other_rows(gpu, M, E, topk, D, F):
         torch.cuda.synchronize()
         assert_equal(to_np(L.y), y, f"eager {i}")
     graph.destroy()
+
+
+def test_pack_on_a_busy_raw_stream(gpu):
+    """As above, on a raw handle: what the caller's stream does next, and what reuses the sources' memory, comes after the packing."""
+    rng = np.random.default_rng(51)
+    w = lm.Weights(rng, 256, 2048, 64)
+    dense = packed(w)
+    a, b = torch.randn((4096, 4096), device="cuda"), torch.empty((4096, 4096), device="cuda")
+    W, st = vw.W4Weights(256, 2048, 64), torch.cuda.Stream()
+    parts = [dev(t) for t in (w.nib, w.sc, w.z, w.msb)]
+    shapes = [(t.shape, t.dtype) for t in parts]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        for _ in range(20):
+            torch.mm(a, a, out=b)
+    W.pack(*parts, stream=st.cuda_stream)
+    del parts
+    junk = [torch.full(s, 85, dtype=dt, device="cuda") for s, dt in shapes for _ in range(3)]
+    assert torch.equal(W.q, dense.q) and torch.equal(W.cst, dense.cst)   # no synchronization before
+    assert all(bool((t == 85).all()) for t in junk)

@@ -37,6 +37,11 @@ def test_w4_statistics(epi, rc):
     assert ("statistics" in lib.vgemm_last_error().decode()) == (rc != 0)
 
 
+class External:
+    def __init__(self, raw, device=None):
+        self.raw = raw
+
+
 class PackCall:
     """W4Weights.pack on CPU tensors with the library, the CUDA contexts and record_stream replaced by recorders."""
 
@@ -60,8 +65,14 @@ class PackCall:
         monkeypatch.setattr(w4, "stream_ptr", lambda s=None: ("raw", s))
         monkeypatch.setattr(torch.cuda, "device", lambda d: enter("device", d))
         monkeypatch.setattr(torch.cuda, "stream", lambda s: enter("stream", s))
-        monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: "current")
-        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda raw, device=None: ("external", raw))
+        self.waits = []
+
+        class Current(str):   # the current stream: the caller's, or the one made current for the call
+            def wait_stream(self, other):
+                me.waits.append((str(self), str(other), len(me.calls)))
+
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: Current("current" if any(k == "stream" for k, _ in me.where) else "caller's"))
+        monkeypatch.setattr(torch.cuda, "ExternalStream", External)
         monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: me.recorded.append((t.data_ptr(), s)))
         self.W = w4.W4Weights.__new__(w4.W4Weights)
         self.W.N, self.W.K, self.W.group, self.W.count, self.W.desc = 8, 64, 32, 1, _lib.W4()
@@ -70,7 +81,7 @@ class PackCall:
                       torch.zeros((8, 4), dtype=torch.int32)]
 
 
-@pytest.mark.parametrize("stream", [None, "side", 1234])
+@pytest.mark.parametrize("stream", [None, "side"])
 def test_pack_keeps_memory_until_its_stream_is_done(monkeypatch, stream):
     """The sources may be freed right after the call, and so may the weights: the allocator has to know the stream that uses them."""
     c = PackCall(monkeypatch)
@@ -78,6 +89,16 @@ def test_pack_keeps_memory_until_its_stream_is_done(monkeypatch, stream):
     assert len(c.calls) == 1
     used = {t.data_ptr() for t in (*c.parts, c.W.q, c.W.cst)}
     assert {p for p, _ in c.recorded} == used and {s for _, s in c.recorded} == {"current"}   # the one made current for the call
+
+
+@pytest.mark.parametrize("stream", [1234, External(1234)])
+def test_pack_on_a_raw_stream(monkeypatch, stream):
+    """The owner of a raw stream may end it before the weights go, so the allocator must not hold on to it: the caller's stream waits
+    for the packing instead, once it is launched."""
+    c = PackCall(monkeypatch)
+    c.W.pack(*c.parts, stream=stream)
+    assert len(c.calls) == 1 and not c.recorded
+    assert c.waits == [("caller's", "current", 1)]
 
 
 def test_pack_keeps_sources_that_it_copies(monkeypatch):
@@ -96,7 +117,7 @@ def test_pack_runs_on_the_device_of_the_weights(monkeypatch, stream):
     (given, where), = c.calls
     kinds = [k for k, _ in where]
     assert where[0] == ("device", c.W.q.device) and kinds == ["device", "stream"]
-    assert where[1] == ("stream", ("external", 1234) if stream == 1234 else stream)
+    assert where[1][1] == stream if stream != 1234 else where[1][1].raw == 1234
 
 
 def test_pack_refuses_a_stream_of_another_device(monkeypatch):

@@ -36,7 +36,8 @@ class W4Weights:
         """Lay out matrices first, first + 1, ...: nib uint8 [(n,) N, >= K/2] (column 2i in the low half of byte i), scale
         int16 or uint16 [(n,) N, groups], zero uint8 alike or None (8 throughout), msb int32 [(n,) N, 4] {m, s, b, unused}. Row
         strides may be larger than the rows. The sources need not be kept after the call, which runs on the
-        weights' device whichever is current; stream, where given, is one of that device."""
+        weights' device whichever is current; stream, where given, is one of that device. The current stream waits for the work on a
+        stream that is given as a raw handle."""
         N, groups = self.N, (self.K + self.group - 1) // self.group
         n = nib.shape[0] if nib.dim() == 3 else 1
         # from one row to the next, over all matrices
@@ -57,17 +58,26 @@ class W4Weights:
         dev = self.q.device
         if getattr(stream, "device", dev) != dev:
             raise ValueError(f"W4Weights.pack: a stream of {stream.device} for weights on {dev}")
-        # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
-        with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
-            for t in (nib, scale, zero, msb, self.q, self.cst):   # none of them is reused, once freed, before the call's work is done
-                if t is not None:
-                    t.record_stream(torch.cuda.current_stream())
-            nib, scale, zero = rows(nib), rows(scale), rows(zero) if zero is not None else None
-            if zero is not None and pitch(zero) != pitch(scale):
-                scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
-            msb = msb[..., :4].contiguous()
-            check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
-                                       ptr(msb)))
+        raw = isinstance(stream, (int, torch.cuda.ExternalStream))
+        with torch.cuda.device(dev):
+            callers = torch.cuda.current_stream()
+            # copies of rows that are laid out otherwise are made, and freed, on the kernels' stream
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+                own = torch.cuda.current_stream()
+                if not raw:   # nothing that the call uses is handed out again, once freed, before its work is done
+                    for t in (nib, scale, zero, msb, self.q, self.cst):
+                        if t is not None:
+                            t.record_stream(own)
+                try:
+                    nib, scale, zero = rows(nib), rows(scale), rows(zero) if zero is not None else None
+                    if zero is not None and pitch(zero) != pitch(scale):
+                        scale, zero = scale[..., :groups].contiguous(), zero[..., :groups].contiguous()
+                    msb = msb[..., :4].contiguous()
+                    check(load().vgemm_w4_pack(stream_ptr(stream), ctypes.byref(self.desc), first, n, ptr(nib), pitch(nib), ptr(scale), ptr(zero), pitch(scale),
+                                               ptr(msb)))
+                finally:
+                    if raw:   # its owner may end it while the weights live, so the allocator may not hold on to it: the caller's stream waits
+                        callers.wait_stream(own)
 
 
 def k_gemm_w4(A: ASrc, M: int, W: W4Weights | W4, E: AEpi, stream=None) -> None:
