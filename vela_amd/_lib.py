@@ -134,6 +134,40 @@ class Moe(_Fields):
                 ("ws", P), ("ws_bytes", SZ)]
 
 
+class Kv(_Fields):
+    """VgemmKv (include/vgemm_kv.h): the pages of a key-value cache."""
+
+    _fields_ = [("pages", I), ("page", I), ("heads", I), ("D", I), ("bits", I), ("data", P), ("shift", P)]
+
+
+class KvPlan(_Fields):
+    """VgemmKvPlan (include/vgemm_kv.h)."""
+
+    _fields_ = [("R", I), ("tokens", I), ("pages", I), ("page", I), ("width", I), ("ldt", I), ("len", P), ("add", P), ("table", P), ("free", P),
+                ("nfree", P), ("new_len", P), ("start", P), ("slot", P), ("pos", P), ("used", P)]
+
+
+class KvAttn(_Fields):
+    """VgemmKvAttn (include/vgemm_kv.h)."""
+
+    _fields_ = [("Q", P), ("ldq", I), ("rows", I), ("Hq", I), ("table", P), ("ldt", I), ("width", I), ("len", P), ("max_len", I), ("window", I), ("m", I),
+                ("s", I), ("Lexp", P), ("out", P), ("ldo", I), ("rowmax", P), ("ws", P), ("ws_bytes", SZ)]
+
+
+class BeamSelect(_Fields):
+    """VgemmBeam (include/vgemm_kv.h)."""
+
+    _fields_ = [("groups", I), ("beams", I), ("V", I), ("n", I), ("logits", P), ("ldz", I), ("score", P), ("Lexp", P), ("Lln", P), ("out_score", P),
+                ("parent", P), ("token", P), ("ws", P), ("ws_bytes", SZ)]
+
+
+class BeamTables(_Fields):
+    """VgemmBeamTables (include/vgemm_kv.h)."""
+
+    _fields_ = [("rows", I), ("page", I), ("width", I), ("ldt", I), ("parent", P), ("len", P), ("table", P), ("fresh", P), ("out_len", P),
+                ("out_table", P), ("src", P), ("dst", P)]
+
+
 # (name, restype, argtypes) of every entry point declared in include/vgemm.h, include/vgemm_model.h and
 # include/vgemm_engine.h
 SIGNATURES = [
@@ -218,6 +252,20 @@ LM_SIGNATURES = [
     ("vgemm_moe", I, [P, ctypes.POINTER(ASrc), I, ctypes.POINTER(Moe)]),
 ]
 
+# the entry points declared in include/vgemm_kv.h
+KV_SIGNATURES = [
+    ("vgemm_kv_page_bytes", SZ, [I, I, I, I]),
+    ("vgemm_kv_plan", I, [P, ctypes.POINTER(KvPlan)]),
+    ("vgemm_kv_write", I, [P, ctypes.POINTER(Kv), P, P, I, P, I]),
+    ("vgemm_kv_read", I, [P, ctypes.POINTER(Kv), P, I, P, P, I]),
+    ("vgemm_kv_copy", I, [P, ctypes.POINTER(Kv), P, P, I]),
+    ("vgemm_kv_attention_workspace_bytes", SZ, [I, I, I, I]),
+    ("vgemm_kv_attention", I, [P, ctypes.POINTER(Kv), ctypes.POINTER(KvAttn)]),
+    ("vgemm_beam_workspace_bytes", SZ, [I, I, I, I]),
+    ("vgemm_beam_select", I, [P, ctypes.POINTER(BeamSelect)]),
+    ("vgemm_beam_tables", I, [P, ctypes.POINTER(BeamTables)]),
+]
+
 _lib = None
 
 
@@ -228,7 +276,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH} is not built: run `python -m vela_amd.build` (there is no fallback path)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, res, args in SIGNATURES + LM_SIGNATURES:
+        for name, res, args in SIGNATURES + LM_SIGNATURES + KV_SIGNATURES:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
