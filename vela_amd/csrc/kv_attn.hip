@@ -10,8 +10,8 @@
 //   * Scores: wave w has the positions [64 w, 64 w + 64). The keys are the A operand; row i of subtile ks is position 16 (i / 4) + 4 ks + i % 4, so that
 //     lane (fg, query) ends with the scores of the 16 positions from 16 fg on, in order. Quarters of four tokens
 //     lie together in a page (vgemm_kv.h), so a load touches four runs of 256 bytes.
-//   * Queries are quantised by every wave for itself while its keys are on their way, in signed digits q = 256 h + l (15 bits leave h in [-64, 64]),
-//     so that keys of 8 bits need two products a piece and no correction.
+//   * Queries are quantised while the first keys are on their way, in signed digits q = 256 h + l (15 bits leave h in [-64, 64]), so that
+//     keys of 8 bits need two products a piece and no correction. They stand in LDS: registers are for the keys and values in flight.
 //   * A score is floor(S m 2^(eq + ek - s) + 1/2) in double: |S m| <= 2^52, so the product is exact and so is the sum with 1/2.
 //   * Weights with the values' shifts, x = -P 2^(ev - least ev of the span), go as signed digits of 8 bits through LDS: two digits where all shifts
 //     are equal, three up to 8 apart, up to six in general. Negated, the top digit lies in [-128, 0].
@@ -29,6 +29,8 @@ namespace vk {
 namespace {
 
 constexpr int EXP_N = 1025;
+
+
 constexpr int MAX_DIGITS = 6;         // 15 bits and shifts up to 25 apart
 constexpr int P_LD = KV_SPAN + 16;    // bytes of a query's weights in LDS, one digit: rows 4 banks apart
 constexpr int TOP_SHIFT = 25;         // of an int32 in 8 bits
@@ -38,6 +40,36 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 __device__ __forceinline__ i64 shfl_xor64(i64 v, int d) { return i64(__shfl_xor((long long)v, d)); }
 
+// over the four lanes (fg, fr) of a query, fg = 0..3
+__device__ __forceinline__ int across_max(int v) {
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(int(a[0]), int(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(int(b[0]), int(b[1]));
+}
+__device__ __forceinline__ int across_sum(int v) {
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = int(a[0] + a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return int(b[0] + b[1]);
+}
+
+// inclusive running sum over the wave: within rows of sixteen, then the rows' totals handed on
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3, then 31 into 2 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ int max_u16x2(int a, int b) {
+    return __builtin_bit_cast(int, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+
 // floor(n / l) saturated to 32 bits, l > 0, inv = 1 / l: the quotient in double is off by less than one
 __device__ __forceinline__ int div_sat(i64 n, i64 l, double inv) {
     double q = floor(double(n) * inv);
@@ -46,269 +78,374 @@ __device__ __forceinline__ int div_sat(i64 n, i64 l, double inv) {
     if (r >= l) q += 1.0;
     return cvt_sat(q);
 }
+// the same for |n| + l below 2^53, where the remainder is exact in double
+__device__ __forceinline__ int div_sat53(double n, double l, double inv) {
+    double q = floor(n * inv);
+    const double r = fma(-q, l, n);
+    q += r >= l ? 1.0 : r < 0.0 ? -1.0 : 0.0;
+    return cvt_sat(q);
+}
 
 struct Lds {
     uint2 table[EXP_N];                        // entry i: Lexp[i] + 2^14, Lexp[i + 1] - Lexp[i]; the last one stands for 0
     int8_t p[MAX_DIGITS][16][P_LD];
-    int mx[4][16], sum[4][16], lo[4], hi[4];
+    int mx[4][16], sum[4][16], ev[4];
     i64 x[4][16];
+    double scale[16];
+    int qsum[16];
 };
 
 // rshr(lutexp(d), 15), at most 32767
 __device__ __forceinline__ int weight(const Lds& s, unsigned d) {
     const uint2 t = s.table[min(d >> 10, unsigned(EXP_N - 1))];
     const i64 prod = i64(int(t.y)) * int(d & 1023);
-    return min(int((t.x + unsigned(int(prod >> 10))) >> 15), 32767);
+    return int(min((t.x + unsigned(int(prod >> 10))) >> 15, 32767u));
 }
 
-template <int NS, int PL>
-__global__ void __launch_bounds__(256) kv_attn_kernel(KvAttnArgs a) {
-    constexpr bool EARLY = NS * PL <= 4;       // values asked for with the keys: 32 NS PL registers for both
+// blocks of four waves that a CU holds at a time, by their registers
+constexpr int kv_held(int D, int planes) { return D <= 128 && planes == 1 ? 3 : (D + 63) / 64 * planes > 4 ? 1 : 2; }
+
+constexpr int DEAL_ROWS = 2048;   // sequences whose spans are dealt evenly: their running sums stand where the weights will
+
+__device__ __forceinline__ int kv_len(const KvAttnArgs& a, int row) { return int(min(i64(max(min(a.len[row], a.max_len), 0)), i64(a.width) << a.c.lp)); }
+__device__ __forceinline__ int kv_first(const KvAttnArgs& a, int n) { return a.window > 0 ? max(0, n - a.window) : 0; }
+
+// EXACT: D == 64 NS, so that the loads' offsets are constants. DEAL: blocks take runs of spans of one sequence and key head, as even as
+// the lengths allow, so that there are about `chunks` runs a head over all sequences; every block counts them from the lengths. Else a block has
+// one span, or each gridDim.z-th.
+template <int NS, int PL, bool EXACT, bool DEAL>
+__global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAttnArgs a, int chunks) {
+    constexpr bool EARLY = NS * PL <= 4;       // values asked for beside the keys, and the next span's keys during the softmax: 32 NS PL registers for both
     __shared__ __attribute__((aligned(16))) Lds s;
+    __shared__ __attribute__((aligned(16))) int8_t qs[2][16][64 * NS + 16];
+    touch_args<int(sizeof(KvAttnArgs) + 4)>();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
-    const int head = blockIdx.x / a.qtiles, q0 = (blockIdx.x % a.qtiles) * 16, row = blockIdx.y;
-    const KvView& c = a.c;
-    const int D = c.D, P = 1 << c.lp;
-    const int n = int(min(i64(max(min(a.len[row], a.max_len), 0)), i64(a.width) << c.lp)), first = a.window > 0 ? max(0, n - a.window) : 0;
-    const int u0 = first / KV_SPAN, u1 = (n + KV_SPAN - 1) / KV_SPAN;
-    const int nq = min(16, a.group - q0);      // query heads of this block
-    const bool mine = fr < nq;
-    const int qh = head * a.group + q0 + fr;
-    if (n == 0) {
-        if (blockIdx.z == 0)
-            for (int i = tid; i < nq * D; i += 256) a.out[size_t(row) * a.ldo + (head * a.group + q0) * D + i] = 0;
-        return;
-    }
-    if (u0 + int(blockIdx.z) >= u1) return;
-
-    for (int i = tid; i < EXP_N; i += 256) {
-        const i64 t = a.Lexp[i], t1 = a.Lexp[min(i + 1, EXP_N - 1)];
-        s.table[i] = i < EXP_N - 1 ? make_uint2(unsigned(t) + (1u << 14), unsigned(t1 - t)) : make_uint2(0, 0);
-    }
-
-    // queries: lane (fg, fr) holds the values [64 c + 16 fg, + 16) of query fr
-    v4i qd[NS][2];
-    int qsum = 0;
-    double scale;
-    {
-        int x[NS][16];
-        unsigned m = 0;
-        const int32_t* q = a.Q + size_t(row) * a.ldq + size_t(mine ? qh : head * a.group) * D;
+    const int head = blockIdx.x / a.qtiles, q0 = (blockIdx.x % a.qtiles) * 16, nq = min(16, a.group - q0);   // key head, its first query head here and their number
+    int row = blockIdx.y, chunk = blockIdx.z, split = gridDim.z;
+    auto zero_row = [&](int r) {               // a sequence without tokens
+        for (int i = tid; i < nq * (EXACT ? 64 * NS : a.c.D); i += 256) a.out[size_t(r) * a.ldo + size_t(head * a.group + q0) * (EXACT ? 64 * NS : a.c.D) + i] = 0;
+    };
+    if constexpr (DEAL) {
+        static_assert(DEAL_ROWS * 4 <= int(sizeof s.p), "running sums");
+        constexpr int EACH = DEAL_ROWS / 256;
+        int* start = reinterpret_cast<int*>(&s.p[0][0][0]);
+        const int each = (a.rows + 255) >> 8;      // sequences of a thread: tid, tid + 256, ...
+        int count[EACH], sum = 0;
 #pragma unroll
-        for (int b = 0; b < NS; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 64 * b + 16 * fg + 4 * i;
-                const int4 v = mine && d < D ? *reinterpret_cast<const int4*>(q + d) : make_int4(0, 0, 0, 0);
-                x[b][4 * i] = v.x; x[b][4 * i + 1] = v.y; x[b][4 * i + 2] = v.z; x[b][4 * i + 3] = v.w;
-                m = max(max(m, max(uabs(v.x), uabs(v.y))), max(uabs(v.z), uabs(v.w)));
-            }
-        m = max(m, unsigned(__shfl_xor(int(m), 16)));
-        m = max(m, unsigned(__shfl_xor(int(m), 32)));
-        const int e = max(0, 32 - __clz(int(m)) - 14);
-#pragma unroll
-        for (int b = 0; b < NS; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                unsigned h = 0, l = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int v = x[b][4 * i + j], r = e ? (v >> e) + ((v >> (e - 1)) & 1) : v;
-                    qsum += r;
-                    h |= unsigned(((r + 128) >> 8) & 255) << (8 * j);
-                    l |= unsigned(r & 255) << (8 * j);
-                }
-                qd[b][0][i] = int(h);
-                qd[b][1][i] = int(l);
-            }
-        if (PL == 2) {
-            qsum += __shfl_xor(qsum, 16);
-            qsum += __shfl_xor(qsum, 32);
+        for (int i = 0; i < EACH; ++i) {
+            count[i] = 0;
+            if (i >= each) break;
+            const int r = tid + 256 * i, n = r < a.rows ? kv_len(a, r) : 0;
+            count[i] = (n + KV_SPAN - 1) / KV_SPAN - kv_first(a, n) / KV_SPAN;
+            sum += count[i];
         }
-        scale = ldexp(double(a.m), e - a.s);
-    }
-    __syncthreads();
-
-    const int pieces = D >> 4;
-    const int32_t* table = a.table + size_t(row) * a.ldt;
-    for (int u = u0 + int(blockIdx.z); u < u1; u += int(gridDim.z)) {
-        const int base = u * KV_SPAN;
-        // pages of the span's sixteen groups, in lanes 0..15
-        int page;
-        {
-            const int pos = base + 16 * fr;
-            page = pos < n ? table[pos >> c.lp] : -1;
-            if (unsigned(page) >= unsigned(c.pages)) page = -1;
-        }
-        // group g of the span: its bytes in a page of keys, and whether there is one
-        auto group = [&](int g, bool& there) {
-            const int p = __shfl(page, g);
-            there = p >= 0;
-            return c.keys(max(p, 0), head) + (((base + 16 * g) & (P - 1)) >> 4) * c.group_bytes();
+        // runs of at most m spans, inv = 1 / m: below 2^16 the product is off by less than 0.5 / m
+        auto runs_of = [](int n, int m, float inv) { return int((float(n + m - 1) + 0.5f) * inv); };
+        // the sum over the threads before this one, and over all
+        auto block_sum = [&](int slot, int v, int& total) {
+            const int run = wave_scan(v);
+            if (lane == 63) s.sum[slot][wave] = run;
+            __syncthreads();
+            const int w0 = s.sum[slot][0], w1 = s.sum[slot][1], w2 = s.sum[slot][2], w3 = s.sum[slot][3];
+            total = w0 + w1 + w2 + w3;
+            return run - v + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
         };
-        bool there;
-        const int8_t* kg = group(4 * wave + (fr >> 2), there) + (fr & 3) * 16 + fg * 64;
-        v4i kv[4][NS][PL], vv[NS][4][PL];
+        int total;
+        block_sum(0, sum, total);
+        const int most = max(1, (total + chunks - 1) / chunks);   // spans of a run
+        sum = 0;
+        const float inv = 1.f / float(most);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int i = 0; i < EACH; ++i) {
+            if (i >= each) break;
+            count[i] = runs_of(count[i], most, inv);
+            sum += count[i];
+        }
+        int run = block_sum(1, sum, total);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {           // in the order of threads
+            if (i >= each) break;
+            start[tid * each + i] = run;
+            run += count[i];
+        }
+        __syncthreads();
+        for (int r = blockIdx.y; r < a.rows; r += int(gridDim.y))
+            if (kv_len(a, r) == 0) zero_row(r);
+        if (int(blockIdx.y) >= total) return;
+        int lo = 0, hi = 256 * each;               // the last sequence whose runs begin at or before this one
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= int(blockIdx.y)) lo = mid;
+            else hi = mid;
+        }
+        const int t = each == 1 ? lo : lo / each;
+        row = __builtin_amdgcn_readfirstlane(t + (lo - t * each) * 256);
+        chunk = __builtin_amdgcn_readfirstlane(int(blockIdx.y) - start[lo]);
+        split = __builtin_amdgcn_readfirstlane((lo + 1 < 256 * each ? start[lo + 1] : total) - start[lo]);
+        __syncthreads();
+    }
+    const KvView& c = a.c;
+    const int D = EXACT ? 64 * NS : c.D, P = 1 << c.lp, pieces = D >> 4;
+    const int32_t* table = a.table + size_t(row) * a.ldt;
+    const i64 room = i64(a.width) << c.lp;
+    // the pages of span u's sixteen groups, in lanes 0..15 (and again in the others): whatever the sequence's length
+    auto fetch = [&](int u) {
+        const int pos = u * KV_SPAN + 16 * fr;
+        const int page = pos < room ? table[pos >> c.lp] : -1;
+        return unsigned(page) < unsigned(c.pages) ? page : -1;
+    };
+    int page = -1;
+    if (!DEAL && a.window == 0) page = fetch(chunk);   // on its way with the length
+    const int n = kv_len(a, row), first = kv_first(a, n), u0 = first / KV_SPAN, u1 = (n + KV_SPAN - 1) / KV_SPAN;
+    const int qh = head * a.group + q0 + fr;
+    // queries: sixteen lanes a query, four neighbouring values at a time
+    int4 x[NS];
+    {
+        const int32_t* q = a.Q + size_t(row) * a.ldq + size_t(head * a.group + q0) * D + (tid >> 4) * D + 4 * fr;
+#pragma unroll
+        for (int b = 0; b < NS; ++b) x[b] = (tid >> 4) < nq && (EXACT || 4 * fr + 64 * b < D) ? *reinterpret_cast<const int4*>(q + 64 * b) : make_int4(0, 0, 0, 0);
+    }
+    if (!DEAL && n == 0 && chunk == 0) zero_row(row);
+    // DEAL: spans [u, u_end), one after the other; else u, u + split, ...
+    int u = DEAL ? u0 + int(i64(u1 - u0) * chunk / split) : u0 + chunk;
+    const int u_end = DEAL ? u0 + int(i64(u1 - u0) * (chunk + 1) / split) : u1, step = DEAL ? 1 : split;
+    if (u >= u_end) return;
+    if (DEAL || a.window) page = fetch(u);
+
+    constexpr int KS = EARLY ? 4 : 2;          // subtiles of keys in registers
+    v4i kv[KS][NS][PL], vv[NS][4][PL];
+    uint4 ek, ev;
+    int evb;
+    // a span's group g: where its keys begin (page 0 where there is none)
+    auto group = [&](int pages, int u, int g) { return c.keys(max(__shfl(pages, g), 0), head) + (((u * KV_SPAN + 16 * g) & (P - 1)) >> 4) * c.group_bytes(); };
+    auto load_tiles = [&](int pages, int u, int k0) {      // subtiles k0, k0 + 1, ...
+        const int8_t* kg = group(pages, u, 4 * wave + (fr >> 2)) + (fr & 3) * 16 + fg * 64;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int b = 0; b < NS; ++b)
 #pragma unroll
                 for (int p = 0; p < PL; ++p)
-                    kv[ks][b][p] = 4 * b + fg < pieces ? *reinterpret_cast<const v4i*>(kg + p * 16 * D + ks * 4 * D + b * 256) : v4i{0, 0, 0, 0};
-        const int8_t* vg[4];
+                    kv[ks][b][p] = EXACT || 4 * b + fg < pieces ? *reinterpret_cast<const v4i*>(kg + p * 16 * D + (k0 + ks) * 4 * D + b * 256) : v4i{0, 0, 0, 0};
+    };
+    auto load_keys = [&](int pages, int u) {
+        load_tiles(pages, u, 0);
+        const int pg = __shfl(pages, 4 * wave + fg);
+        const uint8_t* sh = c.shifts(max(pg, 0), head) + ((u * KV_SPAN + 64 * wave + 16 * fg) & (P - 1));
+        ek = *reinterpret_cast<const uint4*>(sh);
+        ev = *reinterpret_cast<const uint4*>(sh + P);
+        evb = sh[P + fr];
+    };
+    auto load_values = [&](int pages, int u) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-            bool ok;
-            vg[kt] = group(4 * kt + fg, ok) + c.half_bytes() + fr * 16;
-        }
-        auto load_values = [&]() {
+            const int8_t* vg = group(pages, u, 4 * kt + fg) + c.half_bytes() + fr * 16 + wave * 256;
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int p = 0; p < PL; ++p)
-                        vv[i][kt][p] = wave + 4 * i < pieces ? *reinterpret_cast<const v4i*>(vg[kt] + p * 16 * D + (wave + 4 * i) * 256) : v4i{0, 0, 0, 0};
-        };
-        if (EARLY) load_values();
+                for (int p = 0; p < PL; ++p) vv[i][kt][p] = EXACT || wave + 4 * i < pieces ? *reinterpret_cast<const v4i*>(vg + p * 16 * D + i * 1024) : v4i{0, 0, 0, 0};
+        }
+    };
+    load_keys(page, u);
 
-        // shifts of the lane's sixteen positions, and which of them count
-        const int p0 = base + 64 * wave + 16 * fg;
-        uint4 ek, ev;
+    // the table, four entries a thread
+    {
+        i64 t[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) t[i] = a.Lexp[4 * tid + i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.table[4 * tid + i] = make_uint2(unsigned(t[i]) + (1u << 14), unsigned(t[i + 1] - t[i]));
+        if (tid == 0) s.table[EXP_N - 1] = make_uint2(0, 0);
+    }
+    {
+        unsigned m = 0;
+#pragma unroll
+        for (int b = 0; b < NS; ++b) m = max(max(m, max(uabs(x[b].x), uabs(x[b].y))), max(uabs(x[b].z), uabs(x[b].w)));
+        m = max(m, unsigned(dpp32<DPP_XOR1>(int(m))));
+        m = max(m, unsigned(dpp32<DPP_XOR2>(int(m))));
+        m = max(m, unsigned(dpp32<DPP_HALF_MIRROR>(int(m))));
+        m = max(m, unsigned(dpp32<DPP_MIRROR>(int(m))));
+        const int e = max(0, 32 - __clz(int(m)) - 14);
+        int total = 0;
+#pragma unroll
+        for (int b = 0; b < NS; ++b) {
+            const int v[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+            unsigned h = 0, l = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = e ? (v[j] >> e) + ((v[j] >> (e - 1)) & 1) : v[j];
+                total += r;
+                h |= unsigned(((r + 128) >> 8) & 255) << (8 * j);
+                l |= unsigned(r & 255) << (8 * j);
+            }
+            *reinterpret_cast<unsigned*>(&qs[0][tid >> 4][4 * fr + 64 * b]) = h;
+            *reinterpret_cast<unsigned*>(&qs[1][tid >> 4][4 * fr + 64 * b]) = l;
+        }
+        total += dpp32<DPP_XOR1>(total);
+        total += dpp32<DPP_XOR2>(total);
+        total += dpp32<DPP_HALF_MIRROR>(total);
+        total += dpp32<DPP_MIRROR>(total);
+        if (fr == 0) {
+            s.scale[tid >> 4] = ldexp(double(a.m), e - a.s);
+            s.qsum[tid >> 4] = total;
+        }
+    }
+    lds_barrier();
+    const double scale = s.scale[fr];
+    const int qsum = s.qsum[fr];
+
+    for (;;) {
+        const int un = u + step;
+        int pagen = -1;
+        if (EARLY) {
+            load_values(page, u);
+            if (un < u_end) pagen = fetch(un);
+        }
+        // which of the lane's sixteen positions count
+        const int p0 = u * KV_SPAN + 64 * wave + 16 * fg;
         unsigned live;
         {
-            const int pg = __shfl(page, 4 * wave + fg);
-            const uint8_t* sh = c.shifts(max(pg, 0), head) + (p0 & (P - 1));
-            ek = *reinterpret_cast<const uint4*>(sh);
-            ev = *reinterpret_cast<const uint4*>(sh + P);
             const int from = min(max(first - p0, 0), 16), to = min(max(n - p0, 0), 16);
-            live = pg >= 0 && to > from ? ((1u << to) - 1) & ~((1u << from) - 1) : 0;
+            live = __shfl(page, 4 * wave + fg) >= 0 && to > from ? ((1u << to) - 1) & ~((1u << from) - 1) : 0;
         }
-        const unsigned* ekw = reinterpret_cast<const unsigned*>(&ek);
-        const unsigned* evw = reinterpret_cast<const unsigned*>(&ev);
+        const bool whole = __ballot(live != 0xffff) == 0;
+        const unsigned ekw[4] = {ek.x, ek.y, ek.z, ek.w};
+        unsigned evw[4] = {ev.x, ev.y, ev.z, ev.w};
+        // the least and the greatest shift of the values, as the greatest of (ev, 255 - ev) in two halves
+        int ends = live >> fr & 1 ? evb | (255 - evb) << 16 : 0;
+        ends = max_u16x2(ends, dpp32<DPP_XOR1>(ends));
+        ends = max_u16x2(ends, dpp32<DPP_XOR2>(ends));
+        ends = max_u16x2(ends, dpp32<DPP_HALF_MIRROR>(ends));
+        ends = max_u16x2(ends, dpp32<DPP_MIRROR>(ends));
+        {
+            auto e16 = __builtin_amdgcn_permlane16_swap(ends, ends, false, false);
+            ends = max_u16x2(int(e16[0]), int(e16[1]));
+            auto e32 = __builtin_amdgcn_permlane32_swap(ends, ends, false, false);
+            ends = max_u16x2(int(e32[0]), int(e32[1]));
+        }
 
         int sc[16];
-        int mx = INT_MIN, lo = 255, hi = 0;
+        int mx = INT_MIN;
+        v4i qd[NS][2];   // lane (fg, fr): the values [64 b + 16 fg, + 16) of query fr
+#pragma unroll
+        for (int b = 0; b < NS; ++b)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) qd[b][p] = *reinterpret_cast<const v4i*>(&qs[p][fr][64 * b + 16 * fg]);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
+            if (!EARLY && ks == KS) load_tiles(page, u, KS);
             v4i h = {0, 0, 0, 0}, mid = {0, 0, 0, 0}, l = {0, 0, 0, 0};
 #pragma unroll
             for (int b = 0; b < NS; ++b) {
-                h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks][b][0], qd[b][0], h, 0, 0, 0);
+                h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][0], h, 0, 0, 0);
                 if constexpr (PL == 1) {
-                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks][b][0], qd[b][1], l, 0, 0, 0);
+                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], l, 0, 0, 0);
                 } else {
-                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks][b][0], qd[b][1], mid, 0, 0, 0);
-                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks][b][1], qd[b][0], mid, 0, 0, 0);
-                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks][b][1], qd[b][1], l, 0, 0, 0);
+                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], mid, 0, 0, 0);
+                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][0], mid, 0, 0, 0);
+                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][1], l, 0, 0, 0);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int i = 4 * ks + j;
                 double S;
                 if constexpr (PL == 1) S = double(256 * h[j] + l[j]);
                 else S = fma(double(h[j]), 65536.0, fma(double(mid[j]), 256.0, double(l[j] + 128 * qsum)));
-                const int e = int((ekw[ks] >> (8 * j)) & 255), f = min(int((evw[ks] >> (8 * j)) & 255), TOP_SHIFT);
-                const double up = __builtin_bit_cast(double, u64(unsigned(1023 + e)) << 52);
-                sc[i] = cvt_sat(floor(fma(S * scale, up, 0.5)));
-                if (live >> i & 1) {
-                    mx = max(mx, sc[i]);
-                    lo = min(lo, f);
-                    hi = max(hi, f);
-                }
+                const double up = __builtin_bit_cast(double, u64(1023 + ((ekw[ks] >> (8 * j)) & 255)) << 52);
+                sc[4 * ks + j] = cvt_sat(floor(fma(S * scale, up, 0.5)));
             }
         }
-        mx = max(mx, __shfl_xor(mx, 16));
-        mx = max(mx, __shfl_xor(mx, 32));
-        lo = min(lo, __shfl_xor(lo, 16));
-        lo = min(lo, __shfl_xor(lo, 32));
-        hi = max(hi, __shfl_xor(hi, 16));
-        hi = max(hi, __shfl_xor(hi, 32));
+        if (!whole)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = live >> i & 1 ? sc[i] : INT_MIN;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = max(mx, sc[i]);
+        mx = across_max(mx);
         if (fg == 0) s.mx[wave][fr] = mx;
-        if (lane == 0) {
-            s.lo[wave] = lo;
-            s.hi[wave] = hi;
-        }
+        if (lane == 0) s.ev[wave] = ends;
+        if (EARLY && un < u_end) load_keys(pagen, un);
         lds_barrier();
         mx = max(max(s.mx[0][fr], s.mx[1][fr]), max(s.mx[2][fr], s.mx[3][fr]));
-        lo = min(min(s.lo[0], s.lo[1]), min(s.lo[2], s.lo[3]));
-        hi = max(max(s.hi[0], s.hi[1]), max(s.hi[2], s.hi[3]));
-        const int digits = __builtin_amdgcn_readfirstlane(hi <= lo ? 2 : 2 + (hi - lo + 7) / 8);   // a span where nothing counts has lo > hi
+        ends = max_u16x2(max_u16x2(s.ev[0], s.ev[1]), max_u16x2(s.ev[2], s.ev[3]));
+        ends = __builtin_amdgcn_readfirstlane(ends);
+        const int lo = 255 - (ends >> 16), hi = max(min(ends & 0xffff, lo + TOP_SHIFT), lo);   // lo = 255 where nothing counts
+        const int digits = 2 + (hi - lo + 7) / 8;
+        const bool small = digits <= 3 && hi <= 30 - 8 * PL;   // weights of 32 bits, sums that a double holds
 
         int sum = 0;
-        i64 xs = 0;
-        unsigned pk[MAX_DIGITS][4];
+        int w[16];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            int w[4];
+        for (int i = 0; i < 16; ++i) w[i] = weight(s, unsigned(mx) - unsigned(sc[i]));
+        if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = 4 * ks + j;
-                w[j] = live >> i & 1 ? weight(s, unsigned(mx) - unsigned(sc[i])) : 0;
-                sum += w[j];
+            for (int i = 0; i < 16; ++i) w[i] = live >> i & 1 ? w[i] : 0;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {   // shifts of what does not count become the least one
+                const unsigned keep = ((live >> (4 * ks) & 15) * 0x00204081u & 0x01010101u) * 255u;
+                evw[ks] = (evw[ks] & keep) | (unsigned(lo) * 0x01010101u & ~keep);
             }
-            if (digits <= 3) {
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += w[i];
+        sum = across_sum(sum);
+        if (fg == 0) s.sum[wave][fr] = sum;
+        i64 xs = 0;
+        int8_t* prow = &s.p[0][fr][64 * wave + 16 * fg];
+        if (small) {
+            unsigned pk[3][4];
+            int xs32 = 0;                      // at most 256 * 2^23 in all
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const unsigned f = evw[ks] - unsigned(lo) * 0x01010101u;   // no byte is below lo
                 unsigned y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int f = min(int((evw[ks] >> (8 * j)) & 255), TOP_SHIFT);
-                    const int x = -int(unsigned(w[j]) << ((f - lo) & 31));
-                    if (PL == 2) xs += x;
-                    y[j] = unsigned(x) + 0x8080u;
+                    const unsigned v = unsigned(w[4 * ks + j]) << (f >> (8 * j) & 31);
+                    if (PL == 2) xs32 -= int(v);
+                    y[j] = 0x8080u - v;
                 }
-                pk[0][ks] = pk[1][ks] = pk[2][ks] = 0;
+                const unsigned p01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400), p23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400);
+                pk[0][ks] = __builtin_amdgcn_perm(p23, p01, 0x05040100) ^ 0x80808080u;
+                pk[1][ks] = __builtin_amdgcn_perm(p23, p01, 0x07060302) ^ 0x80808080u;
+                pk[2][ks] = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602) | __builtin_amdgcn_perm(y[3], y[2], 0x06020c0c);
+            }
+            if (PL == 2) xs = across_sum(xs32);
+            *reinterpret_cast<uint4*>(prow) = make_uint4(pk[0][0], pk[0][1], pk[0][2], pk[0][3]);
+            *reinterpret_cast<uint4*>(prow + sizeof s.p[0]) = make_uint4(pk[1][0], pk[1][1], pk[1][2], pk[1][3]);
+            if (digits == 3) *reinterpret_cast<uint4*>(prow + 2 * sizeof s.p[0]) = make_uint4(pk[2][0], pk[2][1], pk[2][2], pk[2][3]);
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                i64 x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    pk[0][ks] |= (y[j] & 255) << (8 * j);
-                    pk[1][ks] |= (y[j] >> 8 & 255) << (8 * j);
-                    pk[2][ks] |= (y[j] >> 16 & 255) << (8 * j);
+                    x[j] = -i64(u64(unsigned(w[4 * ks + j])) << ((int(evw[ks] >> (8 * j) & 255) - lo) & 31));
+                    xs += x[j];
                 }
-                pk[0][ks] ^= 0x80808080u;
-                pk[1][ks] ^= 0x80808080u;
-                // with two digits the third is the sign of the second: it is not used
-            } else {
+                for (int t = 0; t < digits; ++t) {
+                    unsigned b = 0;
 #pragma unroll
-                for (int t = 0; t < MAX_DIGITS; ++t) pk[t][ks] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int f = min(int((evw[ks] >> (8 * j)) & 255), TOP_SHIFT);
-                    i64 x = -i64(u64(unsigned(w[j])) << ((f - lo) & 63));
-                    if (PL == 2) xs += x;
-#pragma unroll
-                    for (int t = 0; t < MAX_DIGITS; ++t) {
-                        const int b = int(int8_t(x));
-                        pk[t][ks] |= unsigned(b & 255) << (8 * j);
-                        x = (x - b) >> 8;
+                    for (int j = 0; j < 4; ++j) {
+                        const int d = int(int8_t(x[j]));
+                        b |= unsigned(d & 255) << (8 * j);
+                        x[j] = (x[j] - d) >> 8;
                     }
+                    *reinterpret_cast<unsigned*>(prow + t * int(sizeof s.p[0]) + 4 * ks) = b;
                 }
             }
+            if (PL == 2) {
+                xs += shfl_xor64(xs, 16);
+                xs += shfl_xor64(xs, 32);
+            }
         }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        if (PL == 2) {
-            xs += shfl_xor64(xs, 16);
-            xs += shfl_xor64(xs, 32);
-        }
-        if (fg == 0) {
-            s.sum[wave][fr] = sum;
-            if (PL == 2) s.x[wave][fr] = xs;
-        }
-#pragma unroll
-        for (int t = 0; t < MAX_DIGITS; ++t)
-            if (t < digits) *reinterpret_cast<uint4*>(&s.p[t][fr][64 * wave + 16 * fg]) = make_uint4(pk[t][0], pk[t][1], pk[t][2], pk[t][3]);
+        if (PL == 2 && fg == 0) s.x[wave][fr] = xs;
         lds_barrier();
         sum = s.sum[0][fr] + s.sum[1][fr] + s.sum[2][fr] + s.sum[3][fr];
         if (PL == 2) xs = s.x[0][fr] + s.x[1][fr] + s.x[2][fr] + s.x[3][fr];
-        if (!EARLY) load_values();
+        if (!EARLY) load_values(page, u);
 
-        i64 O[NS][4];
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) O[i][j] = 0;
-        for (int t = digits - 1; t >= 0; --t) {
+        int r[NS][4];
+        auto digit = [&](int t, auto add) {    // the products of one digit, handed over dimension by dimension
             v4i pb[4];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) pb[kt] = *reinterpret_cast<const v4i*>(&s.p[t][fr][64 * kt + 16 * fg]);
@@ -321,30 +458,53 @@ __global__ void __launch_bounds__(256) kv_attn_kernel(KvAttnArgs a) {
                     if constexpr (PL == 2) l = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[i][kt][1], pb[kt], l, 0, 0, 0);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) O[i][j] = O[i][j] * 256 + (PL == 1 ? h[j] : 256 * h[j] + l[j]);
+                for (int j = 0; j < 4; ++j) add(i, j, PL == 1 ? h[j] : 256 * h[j] + l[j]);
             }
-        }
-        if (!mine) {
-            // fall through to the barrier-free end of the loop
+        };
+        const double inv = 1.0 / double(max(sum, 1));
+        if (small) {
+            double O[NS][4];
+            const auto set = [&](int i, int j, int v) { O[i][j] = double(v); };
+            const auto add = [&](int i, int j, int v) { O[i][j] = fma(O[i][j], 256.0, double(v)); };
+            if (digits == 3) {
+                digit(2, set);
+                digit(1, add);
+            } else {
+                digit(1, set);
+            }
+            digit(0, add);
+            const double neg = -__builtin_bit_cast(double, u64(1023 + lo) << 52), half = double(sum >> 1), L = double(sum);
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double o = PL == 2 ? fma(double(int(xs)), 128.0, O[i][j]) : O[i][j];
+                    r[i][j] = sum ? div_sat53(fma(o, neg, half), L, inv) : 0;
+                }
         } else {
-            const double inv = 1.0 / double(max(sum, 1));
+            i64 O[NS][4];
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) O[i][j] = 0;
+            for (int t = digits - 1; t >= 0; --t) digit(t, [&](int i, int j, int v) { O[i][j] = O[i][j] * 256 + v; });
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[i][j] = sum ? div_sat(i64(u64(-(O[i][j] + (PL == 2 ? 128 * xs : 0))) << lo) + (sum >> 1), sum, inv) : 0;
+        }
+        if (fr < nq) {
             const bool only = u1 - u0 == 1;
             const size_t at = (size_t(row) * a.Hq + qh) * a.spans + u;
             unsigned big = 0;
             if (!only && wave == 0 && fg == 0) a.stat[at] = make_int2(mx, sum);
+            int32_t* y = (only ? a.out + size_t(row) * a.ldo + size_t(qh) * D : a.part + at * D) + 16 * wave + 4 * fg;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const int d = 16 * (wave + 4 * i) + 4 * fg;
-                if (wave + 4 * i >= pieces) break;
-                int r[4];
+                if (!EXACT && wave + 4 * i >= pieces) break;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const i64 num = -(O[i][j] + (PL == 2 ? 128 * xs : 0));
-                    r[j] = sum ? div_sat(i64(u64(num) << lo) + (sum >> 1), sum, inv) : 0;
-                    big = max(big, uabs(r[j]));
-                }
-                int32_t* y = only ? a.out + size_t(row) * a.ldo + size_t(qh) * D + d : a.part + at * D + d;
-                *reinterpret_cast<int4*>(y) = make_int4(r[0], r[1], r[2], r[3]);
+                for (int j = 0; j < 4; ++j) big = max(big, uabs(r[i][j]));
+                *reinterpret_cast<int4*>(y + 64 * i) = make_int4(r[i][0], r[i][1], r[i][2], r[i][3]);
             }
             if (only && a.rowmax) {
                 big = max(big, unsigned(__shfl_xor(int(big), 16)));
@@ -352,14 +512,41 @@ __global__ void __launch_bounds__(256) kv_attn_kernel(KvAttnArgs a) {
                 if (fg == 0 && big) atomicMax(a.rowmax + row, big);
             }
         }
+        u = un;
+        if (u >= u_end) return;
+        if (EARLY) {
+            page = pagen;
+        } else {
+            asm volatile("" ::: "memory");     // not among the products, whose values fill the registers
+            page = fetch(u);
+            load_keys(page, u);
+        }
     }
 }
 
 // ---------------------------------------------------------------- the join
 
-constexpr int JOIN_CHUNK = 1024;   // spans whose weights stand in LDS at a time
-constexpr int JOIN_D = 32;         // dimensions of a block: eight lanes of four, 32 spans at a time
+template <int CTRL>
+__device__ __forceinline__ i64 dpp64(i64 v) { return i64(u64(unsigned(dpp32<CTRL>(int(v)))) | u64(unsigned(dpp32<CTRL>(int(v >> 32)))) << 32); }
+__device__ __forceinline__ i64 wave_sum64(i64 v) {
+    v += dpp64<DPP_XOR1>(v);
+    v += dpp64<DPP_XOR2>(v);
+    v += dpp64<DPP_HALF_MIRROR>(v);
+    v += dpp64<DPP_MIRROR>(v);
+    const auto l16 = __builtin_amdgcn_permlane16_swap(int(v), int(v), false, false), h16 = __builtin_amdgcn_permlane16_swap(int(v >> 32), int(v >> 32), false, false);
+    v = i64(u64(l16[0]) | u64(h16[0]) << 32) + i64(u64(l16[1]) | u64(h16[1]) << 32);
+    const auto l32 = __builtin_amdgcn_permlane32_swap(int(v), int(v), false, false), h32 = __builtin_amdgcn_permlane32_swap(int(v >> 32), int(v >> 32), false, false);
+    return i64(u64(l32[0]) | u64(h32[0]) << 32) + i64(u64(l32[1]) | u64(h32[1]) << 32);
+}
+__device__ __forceinline__ int wave_max(int v) {
+    v = max(v, dpp32<DPP_XOR1>(v));
+    v = max(v, dpp32<DPP_XOR2>(v));
+    v = max(v, dpp32<DPP_HALF_MIRROR>(v));
+    v = max(v, dpp32<DPP_MIRROR>(v));
+    return across_max(v);
+}
 
+// G of a span; st.y = 0: none
 __device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st) {
     const unsigned d = unsigned(mx) - unsigned(st.x);
     if (st.y == 0 || d >= (1u << 20)) return 0;
@@ -367,96 +554,180 @@ __device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st)
     return ((t + (((t1 - t) * i64(d & 1023)) >> 10) + 64) >> 7) * st.y;
 }
 
-__global__ void __launch_bounds__(256) kv_join_kernel(KvAttnArgs a) {
-    __shared__ int mxs[4];
-    __shared__ i64 sums[4];
-    __shared__ int g[JOIN_CHUNK];
-    __shared__ i64 acc[4][8][4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int D = a.c.D, parts = (D + JOIN_D - 1) / JOIN_D, qh = blockIdx.x / parts, d0 = (blockIdx.x % parts) * JOIN_D, row = blockIdx.y;
-    const int n = int(min(i64(max(min(a.len[row], a.max_len), 0)), i64(a.width) << a.c.lp)), first = a.window > 0 ? max(0, n - a.window) : 0;
-    const int u0 = first / KV_SPAN, u1 = (n + KV_SPAN - 1) / KV_SPAN;
-    if (u1 - u0 <= 1) return;      // the first kernel has written the row
-    const size_t at = (size_t(row) * a.Hq + qh) * a.spans;
-    int mx = INT_MIN;
-    for (int u = u0 + tid; u < u1; u += 256) {
-        const int2 st = a.stat[at + u];
-        if (st.y) mx = max(mx, st.x);
-    }
-    for (int d = 32; d; d >>= 1) mx = max(mx, __shfl_xor(mx, d));
-    if (lane == 0) mxs[wave] = mx;
-    __syncthreads();
-    mx = max(max(mxs[0], mxs[1]), max(mxs[2], mxs[3]));
-    i64 G = 0;
-    for (int u = u0 + tid; u < u1; u += 256) G += join_weight(a, mx, a.stat[at + u]);
-    for (int d = 32; d; d >>= 1) G += shfl_xor64(G, d);
-    if (lane == 0) sums[wave] = G;
-    __syncthreads();
-    G = sums[0] + sums[1] + sums[2] + sums[3];
-    const int h = max(0, 64 - __clzll((long long)G) - 30);
-    const i64 half = (i64(1) << h) >> 1;
-    const int dl = 4 * (tid & 7), k0 = tid >> 3;
-    const bool in = d0 + dl < D;
+constexpr int JOIN_ONE = 64;       // spans that one wave joins: a lane each for their weights
+constexpr int JOIN_WAVES = 16;     // waves of a query head where there are more
+constexpr int JOIN_CHUNK = 1024;   // spans whose weights stand in LDS at a time
+
+// A lane has four neighbouring dimensions of every (64 / lanes of a span)-th span, so that a wave reads up to 1 KB at a time. Spans are
+// weighed by a lane each. Up to JOIN_ONE spans a wave joins a query head by itself, with the first means on their way before their weights
+// are known; beyond that sixteen waves do, and dims of D dimensions a block where the heads alone would leave CUs idle.
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(KvAttnArgs a, int dims) {
+    constexpr int AHEAD = 8;
+    __shared__ int g_lds[WAVES == 1 ? 1 : JOIN_CHUNK];
+    __shared__ int mxs[WAVES];
+    __shared__ i64 sums[2][WAVES];
+    __shared__ i64 acc[WAVES == 1 ? 1 : WAVES][WAVES == 1 ? 1 : 64 + 1][4];
+    touch_args<int(sizeof(KvAttnArgs) + 4)>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int D = a.c.D, parts = (D + dims - 1) / dims, row = blockIdx.y;
+    const int qh = WAVES == 1 ? int(blockIdx.x) * 4 + wave : int(blockIdx.x) / parts, d0 = WAVES == 1 ? 0 : (int(blockIdx.x) % parts) * dims;
+    const int n = kv_len(a, row), u0 = kv_first(a, n) / KV_SPAN, count = (n + KV_SPAN - 1) / KV_SPAN - u0;
+    if (count <= 1 || qh >= a.Hq) return;      // the first kernel has written the row
+    const size_t at = (size_t(row) * a.Hq + qh) * a.spans + u0;
+    const int quads = min(dims, D - d0) / 4, per = quads <= 4 ? 4 : quads <= 8 ? 8 : quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // lanes of a span
+    const int groups = 64 / per, quad = lane & (per - 1), sub = lane / per;
+    const int32_t* part = a.part + at * D + d0 + 4 * min(quad, quads - 1);
     i64 x[4] = {0, 0, 0, 0}, T = 0;
-    for (int c = u0; c < u1; c += JOIN_CHUNK) {
-        const int m = min(JOIN_CHUNK, u1 - c);
-        __syncthreads();
-        for (int k = tid; k < m; k += 256) g[k] = int((join_weight(a, mx, a.stat[at + c + k]) + half) >> h);
-        __syncthreads();
-        for (int k = k0; k < m; k += 32) {
-            const i64 w = g[k];
-            if (in) {
-                const int4 v = *reinterpret_cast<const int4*>(a.part + (at + c + k) * D + d0 + dl);
-                x[0] += w * v.x;
-                x[1] += w * v.y;
-                x[2] += w * v.z;
-                x[3] += w * v.w;
-            }
-            T += w;
-        }
-    }
+    auto add = [&](i64 w, int4 v) {
+        x[0] += w * v.x;
+        x[1] += w * v.y;
+        x[2] += w * v.z;
+        x[3] += w * v.w;
+    };
+    if constexpr (WAVES == 1) {
+        int4 v[AHEAD];
 #pragma unroll
-    for (int d = 8; d < 64; d <<= 1) {
+        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(sub + i * groups, count - 1)) * D);
+        const int2 st = lane < count ? a.stat[at + lane] : make_int2(INT_MIN, 0);
+        const int mx = wave_max(st.y ? st.x : INT_MIN);
+        const i64 G = join_weight(a, mx, st);
+        const int h = max(0, 64 - __clzll((long long)wave_sum64(G)) - 30);
+        const int g = int((G + ((i64(1) << h) >> 1)) >> h);   // 0 in the lanes behind the last span
+        T = wave_sum64(g);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) add(sub + i * groups < count ? __shfl(g, sub + i * groups) : 0, v[i]);
+        for (int k = sub + AHEAD * groups; k - sub < count; k += groups) {
+            const int w = __shfl(g, k);        // k < 64: count <= JOIN_ONE, and groups divides it
+            add(w, *reinterpret_cast<const int4*>(part + size_t(min(k, count - 1)) * D));
+        }
+    } else {
+        // the thread's spans tid + 1024 i: the first one's statistics stay in registers
+        int4 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(wave * groups + sub + i * WAVES * groups, count - 1)) * D);
+        const int2 st0 = tid < count ? a.stat[at + tid] : make_int2(INT_MIN, 0);
+        int mx = st0.y ? st0.x : INT_MIN;
+        for (int k = tid + JOIN_CHUNK; k < count; k += JOIN_CHUNK) {
+            const int2 st = a.stat[at + k];
+            if (st.y) mx = max(mx, st.x);
+        }
+        mx = wave_max(mx);
+        if (lane == 0) mxs[wave] = mx;
+        __syncthreads();
+        mx = wave_max(mxs[lane & (WAVES - 1)]);
+        const i64 G0 = join_weight(a, mx, st0);
+        i64 G = G0;
+        for (int k = tid + JOIN_CHUNK; k < count; k += JOIN_CHUNK) G += join_weight(a, mx, a.stat[at + k]);
+        G = wave_sum64(G);
+        if (lane == 0) sums[0][wave] = G;
+        __syncthreads();
+        G = wave_sum64(lane < WAVES ? sums[0][lane] : 0);
+        const int h = max(0, 64 - __clzll((long long)G) - 30);
+        const i64 half = (i64(1) << h) >> 1;
+        for (int c = 0; c < count; c += JOIN_CHUNK) {
+            const int m = min(JOIN_CHUNK, count - c);
+            if (c) __syncthreads();
+            if (tid < m) {
+                g_lds[tid] = int(((c ? join_weight(a, mx, a.stat[at + c + tid]) : G0) + half) >> h);
+                T += g_lds[tid];
+            }
+            __syncthreads();
+            int k = wave * groups + sub;
+            if (c == 0) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) add(k + i * WAVES * groups < m ? g_lds[k + i * WAVES * groups] : 0, v[i]);
+                k += AHEAD * WAVES * groups;
+            }
+            for (; k < m; k += WAVES * groups) add(g_lds[k], *reinterpret_cast<const int4*>(part + size_t(c + k) * D));
+        }
+        static_assert(JOIN_CHUNK == 64 * WAVES, "a thread a span of a chunk");
+        T = wave_sum64(T);
+        if (lane == 0) sums[1][wave] = T;
+    }
+    for (int d = per; d < 64; d <<= 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] += shfl_xor64(x[j], d);
-        T += shfl_xor64(T, d);
+    if constexpr (WAVES > 1) {
+        if (sub == 0)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[wave][quad][j] = x[j];
+        __syncthreads();
+        if (wave) return;
+        T = wave_sum64(lane < WAVES ? sums[1][lane] : 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = 0;
+            for (int w = 0; w < WAVES; ++w) x[j] += acc[w][quad][j];
+        }
     }
-    if (lane == 0) sums[wave] = T;   // its last readers are two barriers back
-    if (lane < 8)
-        for (int j = 0; j < 4; ++j) acc[wave][lane][j] = x[j];
-    __syncthreads();
-    if (tid >= 32) return;
-    T = sums[0] + sums[1] + sums[2] + sums[3];
-    const int d = d0 + tid;
-    if (d >= D) return;
-    const i64 X = acc[0][tid >> 2][tid & 3] + acc[1][tid >> 2][tid & 3] + acc[2][tid >> 2][tid & 3] + acc[3][tid >> 2][tid & 3];
-    const int r = T ? div_sat(X + (T >> 1), T, 1.0 / double(T)) : 0;
-    a.out[size_t(row) * a.ldo + size_t(qh) * D + d] = r;
-    if (a.rowmax && r) atomicMax(a.rowmax + row, uabs(r));
+    const bool mine = sub == 0 && quad < quads;
+    const double inv = 1.0 / double(T ? T : 1);
+    int r[4];
+    unsigned big = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        r[j] = T ? div_sat(x[j] + (T >> 1), T, inv) : 0;
+        big = max(big, mine ? uabs(r[j]) : 0u);
+    }
+    if (mine) *reinterpret_cast<int4*>(a.out + size_t(row) * a.ldo + size_t(qh) * D + d0 + 4 * quad) = make_int4(r[0], r[1], r[2], r[3]);
+    if (a.rowmax) {
+        for (int d = 1; d < 64; d <<= 1) big = max(big, unsigned(__shfl_xor(int(big), d)));
+        if (lane == 0 && big) atomicMax(a.rowmax + row, big);
+    }
 }
 
-template <int PL>
-void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g) {
+template <int PL, bool EXACT, bool DEAL>
+void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     switch ((a.c.D + 63) / 64) {
-        case 1: kv_attn_kernel<1, PL><<<g, 256, 0, st>>>(a); break;
-        case 2: kv_attn_kernel<2, PL><<<g, 256, 0, st>>>(a); break;
-        case 3: kv_attn_kernel<3, PL><<<g, 256, 0, st>>>(a); break;
-        default: kv_attn_kernel<4, PL><<<g, 256, 0, st>>>(a);
+        case 1: kv_attn_kernel<1, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
+        case 2: kv_attn_kernel<2, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
+        case 3: kv_attn_kernel<3, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
+        default: kv_attn_kernel<4, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks);
     }
+}
+template <bool DEAL>
+void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
+    const bool exact = a.c.D % 64 == 0;
+    if (a.c.planes == 1) exact ? launch_spans<1, true, DEAL>(st, a, g, chunks) : launch_spans<1, false, DEAL>(st, a, g, chunks);
+    else exact ? launch_spans<2, true, DEAL>(st, a, g, chunks) : launch_spans<2, false, DEAL>(st, a, g, chunks);
 }
 
 }  // namespace
 
 hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
-    // blocks a sequence and head: every span one, while that is no more than KV_BLOCKS in all; a block then takes every z-th span
-    constexpr int KV_BLOCKS = 8192;
     const int heads = a.c.heads * a.qtiles;
-    const int split = std::max(1, std::min(a.spans, KV_BLOCKS / std::max(1, heads * a.rows)));
-    const dim3 g(heads, a.rows, split);
-    if (a.c.planes == 1) launch_spans<1>(st, a, g);
-    else launch_spans<2>(st, a, g);
+    const int held = 256 * kv_held(a.c.D, a.c.planes);   // blocks the card holds at a time
+    if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * a.spans > 2 * held) {
+        // Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
+        // of max_len (a run costs its spans and START more), and at least two where the sequences alone are more than the
+        // blocks: then the longest are what is waited for.
+        const float START = 1.5f;
+        const i64 spans = i64(a.rows) * a.spans;
+        int chunks = 0;
+        float least = 0.f;
+        for (int j = i64(a.rows) * heads > held ? 2 : 1; j <= 4; ++j) {
+            const int n = std::max(1, j * held / heads);
+            const i64 most = (spans + n - 1) / n, runs = (a.spans + most - 1) / most * a.rows;
+            const float cost = float((runs * heads + held - 1) / held) * (float(spans) / float(runs) + START);
+            if (!chunks || cost < least) {
+                least = cost;
+                chunks = n;
+            }
+        }
+        launch_spans<true>(st, a, dim3(heads, int(std::min<i64>(chunks + a.rows, spans))), chunks);   // a sequence adds less than one run to them
+    } else {
+        const int split = int(std::max<i64>(1, std::min<i64>(a.spans, 65536 / (heads * i64(a.rows)))));
+        launch_spans<false>(st, a, dim3(heads, a.rows, split), 0);
+    }
     if (hipError_t e = hipGetLastError()) return e;
-    if (a.spans > 1) kv_join_kernel<<<dim3(a.Hq * ((a.c.D + JOIN_D - 1) / JOIN_D), a.rows), 256, 0, st>>>(a);
+    if (a.spans <= 1) return hipSuccess;
+    if (a.spans <= JOIN_ONE) {
+        kv_join_kernel<1><<<dim3((a.Hq + 3) / 4, a.rows), 256, 0, st>>>(a, a.c.D);
+    } else {
+        const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;
+        kv_join_kernel<JOIN_WAVES><<<dim3(a.Hq * ((a.c.D + dims - 1) / dims), a.rows), 64 * JOIN_WAVES, 0, st>>>(a, dims);
+    }
     return hipGetLastError();
 }
 
