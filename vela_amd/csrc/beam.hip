@@ -1,17 +1,22 @@
 // Beam search's selection (vgemm_beam_select): for each row of logits the sum of its weights and its best tokens, a span of 4096
 // tokens at a time, then per group the best continuations. include/vgemm_kv.h states the formulas.
+//
+// The sum of a row's weights is defined by spans, as the attention's is, so that one pass over the logits gives a span's maximum, its sum
+// and its n best tokens; a second, small kernel joins them. The n best of many values are found by a threshold that at least n of them
+// reach -- the n-th greatest of 64 lanes' maxima, found by bits with a ballot each --, and the few that reach it are put in order by counting. Where too many
+// do (ties, or the best ones in few lanes), the best are taken one after the other instead.
 #include <algorithm>
 #include <climits>
 
 #include "kv.h"
 #include "norm_math.h"
+#include "wave.h"
 
 namespace vk {
 
 namespace {
 
 constexpr int EXP_N = 1025;
-constexpr int PER = BEAM_SPAN / 256;   // values of a thread
 
 __device__ __forceinline__ i64 beam_exp(unsigned d, const int64_t* L) {
     if (d >= (1u << 20)) return 0;
@@ -19,102 +24,211 @@ __device__ __forceinline__ i64 beam_exp(unsigned d, const int64_t* L) {
     return a + (((b - a) * i64(d & 1023)) >> 10);
 }
 
-// A logit and its place in the span as one number: greater logits first, then lower places; 0 for what is banned or not there.
-// 32 + 12 bits, and one that tells the least logit from none.
-constexpr int KEY_BITS = 45;
+// A logit and its place in the span as one number: greater logits first, then lower places; 0 for what is banned.
 __device__ __forceinline__ u64 key_of(int z, int at) { return z == INT_MIN ? 0 : (u64(unsigned(z) ^ 0x80000000u) << 12) + u64(BEAM_SPAN - 1 - at) + 1; }
 __device__ __forceinline__ int key_logit(u64 k) { return int(unsigned((k - 1) >> 12) ^ 0x80000000u); }
 __device__ __forceinline__ int key_place(u64 k) { return BEAM_SPAN - 1 - int((k - 1) & (BEAM_SPAN - 1)); }
 
+// A value that at least n lanes' v reach, at most `step` below the greatest such one where that lies within `range` (powers of two) of the greatest v;
+// 1 where fewer than n lanes have any (v = 0: none).
+__device__ __forceinline__ unsigned reached_by(unsigned v, int n, unsigned range, unsigned step) {
+    const unsigned top = unsigned(wave_max(int(v ^ 0x80000000u))) ^ 0x80000000u;
+    auto enough = [&](unsigned u) { return __popcll(__ballot(v >= u)) >= n; };
+    if (top > range && enough(top - range)) {
+        unsigned t = top - range;
+        for (unsigned b = range >> 1; b >= step; b >>= 1)
+            if (enough(t + b)) t += b;
+        return t;
+    }
+    unsigned t = 0;
+    for (unsigned b = 1u << 31; b; b >>= 1)
+        if (enough(t | b)) t |= b;
+    return t > 1 ? t : 1;
+}
+
+// orders the wave's own LDS accesses where no barrier does
+__device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+constexpr int LIST = 192;   // keys of a wave that reach the threshold: n and a few more as a rule, at most 64 where they are taken one by one
+
 struct SpanLds {
-    uint2 table[EXP_N];        // entry i: Lexp[i], Lexp[i + 1] - Lexp[i]; the last one stands for 0
-    u64 list[BEAM_SPAN];       // keys that reach the threshold
+    uint2 table[EXP_N];     // entry i: Lexp[i], Lexp[i + 1] - Lexp[i]; the last one stands for 0
+    u64 list[4][LIST];
     i64 sum[4];
-    u64 floor_[4];
-    int mx[4], count;
+    int mx[4], count[4];
+    unsigned reach[4];
 };
 
-// One span of one row. The n-th greatest of a wave's 64 lane maxima is a key that at least n keys of the wave reach, so the greatest of the
-// four waves' is a threshold that the span's n best reach; found by bits, with a ballot each. The keys that reach it, a few more than n as
-// a rule and at most 16 n a wave, are put in order by counting.
-__global__ void __launch_bounds__(256) beam_span_kernel(BeamArgs a) {
+struct __attribute__((packed, aligned(4))) Quad { int v[4]; };   // sixteen bytes that lie where rows of any length put them
+
+// One span of one row, by WAVES waves of a block of four: one where there are spans for all CUs (a wave's search, sums and order then serve 64
+// values a lane: 200 x 100003 logits 49 -> 22 us), four where the call's own latency counts (4 x 32000: 6.4 us).
+template <int WAVES>
+__global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
+    constexpr int PER = BEAM_SPAN / (64 * WAVES);
     __shared__ SpanLds s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, span = blockIdx.x, n = a.b.n;
+    touch_args<int(sizeof(BeamArgs))>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = a.b.n;
+    const int id = WAVES == 4 ? int(blockIdx.x) : int(blockIdx.x) * 4 + wave, rows = a.b.groups * a.b.beams;
+    const int row = min(id / a.spans, rows - 1), span = id % a.spans;
     const size_t out = size_t(row) * a.spans + span;
-    if (a.b.score[row] == LLONG_MIN) return;   // no such beam: nothing reads its part of the workspace
-    const int base = span * BEAM_SPAN;
+    const bool in = id < rows * a.spans;
+    const i64 score = a.b.score[row];            // on its way with the logits
+    const int base = span * BEAM_SPAN, m = in ? min(BEAM_SPAN, a.b.V - base) : 0, t0 = WAVES == 4 ? tid : lane;
     const int32_t* z = a.b.logits + size_t(row) * a.b.ldz + base;
-    const int m = min(BEAM_SPAN, a.b.V - base);
     int v[PER];
+    if (m == BEAM_SPAN) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = tid + 256 * i < m ? z[tid + 256 * i] : INT_MIN;
-    for (int i = tid; i < EXP_N; i += 256) {
-        const i64 t = a.b.Lexp[i], t1 = a.b.Lexp[min(i + 1, EXP_N - 1)];
-        s.table[i] = i < EXP_N - 1 ? make_uint2(unsigned(t), unsigned(t1 - t)) : make_uint2(0, 0);
-    }
-    if (tid == 0) s.count = 0;
-    u64 best = 0;
+        for (int q = 0; q < PER / 4; ++q) {
+            const Quad x = *reinterpret_cast<const Quad*>(z + 4 * (q * 64 * WAVES + t0));
 #pragma unroll
-    for (int i = 0; i < PER; ++i) best = max(best, key_of(v[i], tid + 256 * i));
-    // the greatest t with at least n lane maxima >= t, 0 where fewer lanes have any
-    u64 t = 0;
-    for (int b = KEY_BITS - 1; b >= 0; --b) {
-        const u64 u = t | (u64(1) << b);
-        if (__popcll(__ballot(best >= u)) >= n) t = u;
+            for (int i = 0; i < 4; ++i) v[4 * q + i] = x.v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = 4 * ((i >> 2) * 64 * WAVES + t0) + (i & 3);
+            v[i] = at < m ? z[at] : INT_MIN;
+        }
     }
-    int mx = best ? key_logit(best) : INT_MIN;
-    for (int d = 32; d; d >>= 1) mx = max(mx, __shfl_xor(mx, d));
+    auto place = [&](int i) { return 4 * ((i >> 2) * 64 * WAVES + t0) + (i & 3); };
+    {
+        i64 t[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) t[i] = a.b.Lexp[4 * tid + i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.table[4 * tid + i] = make_uint2(unsigned(t[i]), unsigned(t[i + 1] - t[i]));
+        if (tid == 0) s.table[EXP_N - 1] = make_uint2(0, 0);
+    }
+    int mx = INT_MIN;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mx = max(mx, v[i]);
+    unsigned reach = reached_by(unsigned(mx) ^ 0x80000000u, n, 1u << 20, 1u << 10);   // 16 of the logits, by steps of 1/64
+    mx = wave_max(mx);
     if (lane == 0) {
         s.mx[wave] = mx;
-        s.floor_[wave] = t;
+        s.reach[wave] = reach;
+        s.count[wave] = 0;
     }
     __syncthreads();
-    mx = max(max(s.mx[0], s.mx[1]), max(s.mx[2], s.mx[3]));
-    t = max(max(max(s.floor_[0], s.floor_[1]), max(s.floor_[2], s.floor_[3])), u64(1));
-    i64 sum = 0;
+    if (!in || score == LLONG_MIN) return;     // no such beam: nothing reads its part of the workspace
+    if constexpr (WAVES == 4) {
+        mx = max(max(s.mx[0], s.mx[1]), max(s.mx[2], s.mx[3]));
+        reach = max(max(s.reach[0], s.reach[1]), max(s.reach[2], s.reach[3]));
+    }
+    const int least = int(reach ^ 0x80000000u);   // above what is banned
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const unsigned d = v[i] == INT_MIN ? ~0u : unsigned(mx) - unsigned(v[i]);
-        const uint2 e = s.table[min(d >> 10, unsigned(EXP_N - 1))];
-        sum += i64(e.x) + ((i64(int(e.y)) * int(d & 1023)) >> 10);
-        const u64 k = key_of(v[i], tid + 256 * i);
-        if (k >= t) s.list[atomicAdd(&s.count, 1)] = k;
+    for (int i = 0; i < PER; ++i)
+        if (v[i] >= least) {
+            const int at = atomicAdd(&s.count[wave], 1);
+            if (at < LIST) s.list[wave][at] = key_of(v[i], place(i));
+        }
+    i64 sum = 0;
+    // what is banned lies far enough below any maximum but those near it
+    const bool low = mx < INT_MIN + (1 << 20);
+#pragma unroll
+    for (int q = 0; q < PER / 8; ++q) {
+#pragma unroll
+        for (int i = 8 * q; i < 8 * q + 8; ++i) {
+            const unsigned d = low && v[i] == INT_MIN ? ~0u : unsigned(mx) - unsigned(v[i]);
+            const uint2 e = s.table[min(d >> 10, unsigned(EXP_N - 1))];
+            sum += e.x + unsigned(int((i64(int(e.y)) * int(d & 1023)) >> 10));
+        }
+        asm volatile("" ::: "memory");   // eight table entries on their way at a time, not 64
     }
-    for (int d = 32; d; d >>= 1) sum += i64(__shfl_xor((long long)sum, d));
+    sum = wave_sum64(sum);
+    wave_lds();
+    if (s.count[wave] > LIST) {                   // one after the other: each the greatest below the last
+        int lz = INT_MAX, lp = -1, k = 0;         // the last one's logit and place
+        for (; k < n; ++k) {
+            int bz = INT_MIN, bp = 0;
+            const int rel = lp - 4 * t0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {       // of equal ones the first: a lane's places rise
+                constexpr int STEP = 4 * 64 * WAVES;
+                const int at = (i >> 2) * STEP + (i & 3);
+                if ((v[i] < lz || (v[i] == lz && at > rel)) && v[i] > bz) {
+                    bz = v[i];
+                    bp = at;
+                }
+            }
+            u64 best = key_of(bz, 4 * t0 + bp);
+            for (int d = 1; d < 64; d <<= 1) best = max(best, u64(__shfl_xor((unsigned long long)best, d)));
+            if (!best) break;
+            if (lane == 0) s.list[wave][k] = best;
+            lz = key_logit(best);
+            lp = key_place(best);
+        }
+        if (lane == 0) s.count[wave] = k;
+        wave_lds();
+    }
     if (lane == 0) s.sum[wave] = sum;
-    __syncthreads();
-    const int c = s.count;
-    if (tid == 0) a.stat[out] = BeamStat{s.sum[0] + s.sum[1] + s.sum[2] + s.sum[3], mx, 0};
     int2* cand = a.cand + out * n;
-    for (int i = tid; i < c; i += 256) {
-        const u64 k = s.list[i];
-        int rank = 0;
-        for (int j = 0; j < c; ++j) rank += s.list[j] > k;
-        if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
+    if constexpr (WAVES == 1) {
+        const int c = s.count[wave];
+        if (lane == 0) a.stat[out] = BeamStat{sum, mx, 0};
+        for (int i = lane; i < c; i += 64) {
+            const u64 k = s.list[wave][i];
+            int rank = 0;
+            for (int j = 0; j < c; ++j) rank += s.list[wave][j] > k;
+            if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
+        }
+        for (int i = c + lane; i < n; i += 64) cand[i] = make_int2(INT_MIN, -1);
+    } else {
+        __syncthreads();
+        if (tid == 0) a.stat[out] = BeamStat{s.sum[0] + s.sum[1] + s.sum[2] + s.sum[3], mx, 0};
+        const int all = s.count[0] + s.count[1] + s.count[2] + s.count[3];
+        for (int i = lane; i < s.count[wave]; i += 64) {
+            const u64 k = s.list[wave][i];
+            int rank = 0;
+            for (int w = 0; w < 4; ++w)
+                for (int j = 0; j < s.count[w]; ++j) rank += s.list[w][j] > k;
+            if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
+        }
+        for (int i = all + tid; i < n; i += 256) cand[i] = make_int2(INT_MIN, -1);
     }
-    for (int i = c + tid; i < n; i += 256) cand[i] = make_int2(INT_MIN, -1);
 }
+
+// ---------------------------------------------------------------- the groups
 
 struct Best { i64 c; int at; };   // score and list: lower lists first among equal scores
 __device__ __forceinline__ bool before(const Best& x, const Best& y) { return x.c > y.c || (x.c == y.c && x.at < y.at); }
 
-// One group: logZ of its beams, a wave a beam, then its spans' lists, each in falling order and all in order of beam and token, merged n
-// times by the best of their heads. LLONG_MIN with a list past the last one stands for none.
-constexpr int LISTS = BEAM_MOST * (BEAM_V / BEAM_SPAN) / 256;   // lists of a thread
-__global__ void __launch_bounds__(256) beam_merge_kernel(BeamArgs a) {
+constexpr int NEAR = 40;      // bits of a score below the group's best one that a key holds
+constexpr int PLACES = 23;    // bits of beam * V + token
+constexpr u64 FAR = (u64(1) << NEAR) - 1;
+constexpr int BEST_LIST = 1024;
+
+// One group: logZ of its beams, a wave a beam, then the best of its spans' lists, each in falling order: a thread a list or two, by a threshold as
+// above over keys of a score's distance from the best one and its place, which the lists' heads give and down to which each list is
+// walked. Where the keys do not tell (scores 2^40 apart, or too many that reach the threshold) the lists are merged n times
+// by the best of their heads.
+template <int THREADS, int LISTS>
+__global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
+    constexpr int WAVES = THREADS / 64, AHEAD = 2;   // entries of a list that are asked for at the start
     __shared__ i64 off[BEAM_MOST];
-    __shared__ Best heads[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, B = a.b.beams, n = a.b.n;
-    for (int b = wave; b < B; b += 4) {
+    __shared__ Best heads[WAVES];
+    __shared__ u64 list[BEST_LIST];
+    __shared__ int count, far;
+    __shared__ unsigned reach_of[WAVES];
+    touch_args<int(sizeof(BeamArgs))>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.x, B = a.b.beams, n = a.b.n;
+    const int lists = B * a.spans;
+    const int2* cand = a.cand + size_t(g) * lists * n;
+    int2 first[LISTS][AHEAD];
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i)
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) first[i][j] = tid + THREADS * i < lists && j < n ? cand[size_t(tid + THREADS * i) * n + j] : make_int2(INT_MIN, -1);
+    if (tid == 0) count = far = 0;
+    for (int b = wave; b < B; b += WAVES) {
         const int row = g * B + b;
         const i64 score = a.b.score[row];
         const bool in = lane < a.spans && score != LLONG_MIN;
         const BeamStat st = in ? a.stat[size_t(row) * a.spans + lane] : BeamStat{0, INT_MIN, 0};
-        int mx = st.mx;
-        for (int d = 32; d; d >>= 1) mx = max(mx, __shfl_xor(mx, d));
+        const int mx = wave_max(st.mx);
         i64 S = in && st.S ? (beam_exp(unsigned(mx) - unsigned(st.mx), a.b.Lexp) * ((st.S + 2048) >> 12) + (1 << 17)) >> 18 : 0;
-        for (int d = 32; d; d >>= 1) S += i64(__shfl_xor((long long)S, d));
-        S = max(S, i64(1));
+        S = max(wave_sum64(S), i64(1));
         const int t = 63 - __clzll((long long)S);
         const i64 f = (t >= 30 ? S >> (t - 30) : S << (30 - t)) - (i64(1) << 30);
         const int i = int(f >> 20);
@@ -122,18 +236,81 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamArgs a) {
         if (lane == 0) off[b] = score == LLONG_MIN ? LLONG_MIN : score - mx - logz;
     }
     __syncthreads();
-    const int lists = B * a.spans;
-    const int2* cand = a.cand + size_t(g) * lists * n;
-    i64 c[LISTS];              // the heads of this thread's lists, tid + 256 i
+    // LLONG_MIN: no beam (its lists hold anything) or no token
+    i64 o[LISTS];
+    int f0[LISTS];                               // a beam's place: beam * V
+    i64 top = LLONG_MIN;
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i) {
+        const int beam = min(tid + THREADS * i, lists - 1) / a.spans;
+        o[i] = off[beam];
+        f0[i] = beam * a.b.V;
+    }
+    auto score_of = [&](int i, int2 k) { return o[i] == LLONG_MIN || k.y < 0 ? LLONG_MIN : o[i] + k.x; };
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i) top = max(top, score_of(i, first[i][0]));
+    top = wave_max64(top);
+    if (lane == 0) heads[wave].c = top;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) top = max(top, heads[w].c);
+    auto key = [&](int i, int2 k) {              // 0: none, or too far below the best
+        const i64 c = score_of(i, k);
+        const u64 d = u64(top) - u64(c);
+        return c == LLONG_MIN || d >= FAR ? u64(0) : ((FAR - d) << PLACES) | u64((1 << PLACES) - 1 - (f0[i] + k.y));
+    };
+    u64 best = 0;
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i) best = max(best, key(i, first[i][0]));
+    constexpr int CUT = NEAR + PLACES - 32;
+    const unsigned reach_own = reached_by(unsigned(best >> CUT), n, 1u << (20 - (CUT - PLACES)), 1u << (10 - (CUT - PLACES)));   // scores 2^20 below the best, by steps of 2^10
+    if (lane == 0) reach_of[wave] = reach_own;
+    __syncthreads();
+    unsigned reach = 1;
+    for (int w = 0; w < WAVES; ++w) reach = max(reach, reach_of[w]);
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i)
+        for (int j = 0; j < n; ++j) {
+            const int2 k = j == 0 ? first[i][0] : j == 1 ? first[i][1] : tid + THREADS * i < lists ? cand[size_t(tid + THREADS * i) * n + j] : make_int2(INT_MIN, -1);
+            const u64 y = key(i, k);
+            if (y == 0 || unsigned(y >> CUT) < reach) {
+                if (y == 0 && score_of(i, k) != LLONG_MIN) far = 1;
+                break;
+            }
+            const int at = atomicAdd(&count, 1);
+            if (at < BEST_LIST) list[at] = y;
+        }
+    __syncthreads();
+    const bool told = count >= n || !far;        // else some of the n best are among the far ones
+    if (told && count <= BEST_LIST) {
+        for (int i = tid; i < max(count, n); i += THREADS) {
+            int rank = i;
+            i64 c = LLONG_MIN;
+            int parent = -1, token = -1;
+            if (i < count) {
+                const u64 y = list[i];
+                rank = 0;
+                for (int j = 0; j < count; ++j) rank += list[j] > y;
+                const int f = (1 << PLACES) - 1 - int(y & ((1 << PLACES) - 1));
+                c = i64(u64(top) - (FAR - (y >> PLACES)));
+                parent = g * B + f / a.b.V;
+                token = f % a.b.V;
+            }
+            if (rank < n) {
+                const size_t to = size_t(g) * n + rank;
+                a.b.out_score[to] = c;
+                a.b.parent[to] = parent;
+                a.b.token[to] = token;
+            }
+        }
+        return;
+    }
+    i64 c[LISTS];              // the heads of this thread's lists, tid + THREADS i
     int at[LISTS];             // and how far they have been taken
     auto head = [&](int i) {
-        const int list = tid + 256 * i;
+        const int l = tid + THREADS * i;
         c[i] = LLONG_MIN;
-        if (list >= lists || at[i] >= n) return;
-        const i64 o = off[list / a.spans];
-        if (o == LLONG_MIN) return;
-        const int2 k = cand[size_t(list) * n + at[i]];
-        if (k.y >= 0) c[i] = o + k.x;
+        if (l >= lists || at[i] >= n) return;
+        c[i] = score_of(i, cand[size_t(l) * n + at[i]]);
     };
 #pragma unroll
     for (int i = 0; i < LISTS; ++i) {
@@ -144,7 +321,7 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamArgs a) {
         Best x{LLONG_MIN, INT_MAX};
 #pragma unroll
         for (int i = 0; i < LISTS; ++i) {
-            const Best y{c[i], tid + 256 * i};
+            const Best y{c[i], tid + THREADS * i};
             if (c[i] != LLONG_MIN && before(y, x)) x = y;
         }
         for (int d = 32; d; d >>= 1) {
@@ -154,24 +331,24 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamArgs a) {
         if (lane == 0) heads[wave] = x;
         __syncthreads();
         x = heads[0];
-        for (int w = 1; w < 4; ++w)
+        for (int w = 1; w < WAVES; ++w)
             if (before(heads[w], x)) x = heads[w];
         __syncthreads();
-        const size_t o = size_t(g) * n + k;
+        const size_t to = size_t(g) * n + k;
         if (x.at == INT_MAX) {
             if (tid == 0) {
-                a.b.out_score[o] = LLONG_MIN;
-                a.b.parent[o] = a.b.token[o] = -1;
+                a.b.out_score[to] = LLONG_MIN;
+                a.b.parent[to] = a.b.token[to] = -1;
             }
             continue;
         }
-        if ((x.at & 255) != tid) continue;
+        if ((x.at & (THREADS - 1)) != tid) continue;
 #pragma unroll
         for (int i = 0; i < LISTS; ++i)
-            if (tid + 256 * i == x.at) {
-                a.b.out_score[o] = x.c;
-                a.b.parent[o] = g * B + x.at / a.spans;
-                a.b.token[o] = cand[size_t(x.at) * n + at[i]].y;
+            if (tid + THREADS * i == x.at) {
+                a.b.out_score[to] = x.c;
+                a.b.parent[to] = g * B + x.at / a.spans;
+                a.b.token[to] = cand[size_t(x.at) * n + at[i]].y;
                 ++at[i];
                 head(i);
             }
@@ -181,9 +358,12 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamArgs a) {
 }  // namespace
 
 hipError_t launch_beam_select(hipStream_t st, const BeamArgs& a) {
-    beam_span_kernel<<<dim3(a.spans, a.b.groups * a.b.beams), 256, 0, st>>>(a);
+    const int spans = a.b.groups * a.b.beams * a.spans;
+    if (spans >= 2048) beam_span_kernel<1><<<(spans + 3) / 4, 256, 0, st>>>(a);
+    else beam_span_kernel<4><<<spans, 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
-    beam_merge_kernel<<<a.b.groups, 256, 0, st>>>(a);
+    if (a.b.beams * a.spans <= 256) beam_merge_kernel<256, 1><<<a.b.groups, 256, 0, st>>>(a);
+    else beam_merge_kernel<1024, 2><<<a.b.groups, 1024, 0, st>>>(a);
     return hipGetLastError();
 }
 

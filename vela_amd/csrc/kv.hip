@@ -4,6 +4,7 @@
 
 #include "kv.h"
 #include "norm_math.h"
+#include "wave.h"
 
 namespace vk {
 
@@ -118,38 +119,66 @@ __global__ void __launch_bounds__(256) kv_plan_kernel(VgemmKvPlan p, int lp) {
 
 // ---------------------------------------------------------------- rows
 
-// the greatest of a 16-lane row's values
-__device__ __forceinline__ unsigned row16_max(unsigned v) {
-    v = max(v, unsigned(dpp32<DPP_XOR1>(int(v))));
-    v = max(v, unsigned(dpp32<DPP_XOR2>(int(v))));
-    v = max(v, unsigned(dpp32<DPP_HALF_MIRROR>(int(v))));
-    return max(v, unsigned(dpp32<DPP_MIRROR>(int(v))));
+constexpr int KV_TOKENS = 16;   // of a block: sixteen lanes a token, four neighbouring values at a time
+
+// Where a row lies: page, and the place in it; there = false where the slot is none.
+struct Place { bool there; int page, at; };
+__device__ __forceinline__ Place place_of(const KvView& c, int slot) {
+    const bool there = slot >= 0 && slot < (c.pages << c.lp);
+    return Place{there, there ? slot >> c.lp : 0, there ? slot & ((1 << c.lp) - 1) : 0};
 }
 
-constexpr int KV_TOKENS = 16;   // of a block: sixteen lanes a token
+// Values lie transposed, sixteen tokens a dimension. A block turns its sixteen tokens over in LDS, so that four tokens whose slots follow one another
+// from a multiple of four are one word in memory, and lanes that follow one another touch 256 neighbouring bytes. The LDS columns are the
+// tokens moved by `off`, which makes a run of tokens that begins anywhere meet those words; tokens of other words go as bytes.
+constexpr int TURN = 20;        // columns of a dimension: sixteen and up to three before them
+struct Turn {
+    int slot[KV_TOKENS];
+    int off;
+};
+__device__ __forceinline__ void turn_init(Turn& t, const KvView& c, const int32_t* slots, int M) {
+    if (threadIdx.x < 64) {     // one wave
+        const int i = threadIdx.x, at = int(blockIdx.x) * KV_TOKENS + i;
+        const int slot = i < KV_TOKENS && at < M ? slots[at] : -1;
+        const bool there = place_of(c, slot).there;
+        const u64 first = __ballot(there);
+        if (i < KV_TOKENS) t.slot[i] = there ? slot : -1;
+        if (first ? i == __ffsll((unsigned long long)first) - 1 : i == 0) t.off = first ? (slot - i) & 3 : 0;
+    }
+}
+// the slot of the first of word w's four tokens where they are one word in memory, else -1
+__device__ __forceinline__ int turn_word(const Turn& t, int w) {
+    const int i = 4 * w - t.off;
+    if (i < 0 || i + 3 >= KV_TOKENS) return -1;
+    const int s = t.slot[i];
+    return s >= 0 && (s & 3) == 0 && t.slot[i + 1] == s + 1 && t.slot[i + 2] == s + 2 && t.slot[i + 3] == s + 3 ? s : -1;
+}
 
-// sixteen tokens of one head, keys or values (blockIdx.z): a token's sixteen lanes hold four neighbouring values at a time
-template <int PL>
+template <int PL, bool RUNS>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvView c, const int32_t* K, const int32_t* V, int ld, const int32_t* slots, int M) {
-    const int l = threadIdx.x & 15, t = int(blockIdx.x) * KV_TOKENS + (threadIdx.x >> 4), head = blockIdx.y, value = blockIdx.z;
-    const int slot = t < M ? slots[t] : -1;
-    const bool there = slot >= 0 && slot < (c.pages << c.lp);
-    const int32_t* x = (value ? V : K) + size_t(there ? t : 0) * ld + head * c.D;
+    __shared__ Turn turn;
+    __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
+    const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;
+    const bool value = blockIdx.z;
+    const Place p = place_of(c, t < M ? slots[t] : -1);
+    const int32_t* x = (value ? V : K) + size_t(p.there ? t : 0) * ld + head * c.D;
     int4 v[4];
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = 4 * l + 64 * i;
-        v[i] = there && d < c.D ? *reinterpret_cast<const int4*>(x + d) : make_int4(0, 0, 0, 0);
+        v[i] = p.there && d < c.D ? *reinterpret_cast<const int4*>(x + d) : make_int4(0, 0, 0, 0);
         m = max(max(m, max(uabs(v[i].x), uabs(v[i].y))), max(uabs(v[i].z), uabs(v[i].w)));
     }
-    m = row16_max(m);
+    if (RUNS && value) {
+        turn_init(turn, c, slots, M);
+        __syncthreads();
+    }
+    m = row_max(m);
     constexpr int BITS = 8 * PL - 1, TOP = (1 << BITS) - 1;
     const int e = max(0, 32 - __clz(int(m)) - BITS);   // __clz(0) is 32
-    if (!there) return;
-    const int page = slot >> c.lp, at = slot & ((1 << c.lp) - 1), t16 = at & 15;
-    int8_t* dst = c.keys(page, head) + (value ? c.half_bytes() : 0) + (at >> 4) * c.group_bytes();
-    if (l == 0) c.shifts(page, head)[(value << c.lp) + at] = uint8_t(e);
+    if (l == 0 && p.there) c.shifts(p.page, head)[(int(value) << c.lp) + p.at] = uint8_t(e);
+    int8_t* keys = c.keys(p.page, head) + (p.at >> 4) * c.group_bytes();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = 4 * l + 64 * i;
@@ -158,52 +187,97 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvView c, const int32_t* 
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[j] = min(max(e ? (q[j] >> e) + ((q[j] >> (e - 1)) & 1) : q[j], -TOP), TOP);
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-            int8_t* plane = dst + p * 16 * c.D;
+        for (int n = 0; n < PL; ++n) {
             char4 b;
             int8_t* bb = reinterpret_cast<int8_t*>(&b);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bb[j] = int8_t(PL == 1 ? q[j] : p == 0 ? q[j] >> 8 : (q[j] & 255) - 128);
-            if (value) {
+            for (int j = 0; j < 4; ++j) bb[j] = int8_t(PL == 1 ? q[j] : n == 0 ? q[j] >> 8 : (q[j] & 255) - 128);
+            if (RUNS && value) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) plane[c.value_at(t16, d + j)] = bb[j];
-            } else {
-                *reinterpret_cast<char4*>(plane + c.key_at(t16, d)) = b;
+                for (int j = 0; j < 4; ++j) vt[(n * c.D + d + j) * TURN + t16 + turn.off] = bb[j];
+            } else if (p.there && value) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d + j)] = bb[j];
+            } else if (p.there) {
+                *reinterpret_cast<char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d)) = b;
+            }
+        }
+    }
+    if (!RUNS || !value) return;
+    __syncthreads();
+    const int words = turn.off ? 5 : 4;
+    for (int w = tid & 3; w < words; w += 4) {
+        const int s = turn_word(turn, w), i0 = 4 * w - turn.off;
+        if (s >= 0) {
+            const Place o = place_of(c, s);
+            int8_t* dst = c.keys(o.page, head) + c.half_bytes() + (o.at >> 4) * c.group_bytes() + (o.at & 15);
+            for (int d = tid >> 2; d < PL * c.D; d += 64) *reinterpret_cast<int*>(dst + 16 * d) = *reinterpret_cast<const int*>(&vt[d * TURN + 4 * w]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i0 + k < 0 || i0 + k >= KV_TOKENS || turn.slot[i0 + k] < 0) continue;
+                const Place o = place_of(c, turn.slot[i0 + k]);
+                int8_t* dst = c.keys(o.page, head) + c.half_bytes() + (o.at >> 4) * c.group_bytes() + (o.at & 15);
+                for (int d = tid >> 2; d < PL * c.D; d += 64) dst[16 * d] = vt[d * TURN + 4 * w + k];
             }
         }
     }
 }
 
-template <int PL>
+template <int PL, bool RUNS>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvView c, const int32_t* slots, int M, int32_t* K, int32_t* V, int ld) {
-    const int l = threadIdx.x & 15, t = int(blockIdx.x) * KV_TOKENS + (threadIdx.x >> 4), head = blockIdx.y;
+    __shared__ Turn turn;
+    __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
+    const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;
     const bool value = K ? blockIdx.z : true;
+    const Place p = place_of(c, t < M ? slots[t] : -1);
+    const int e = p.there ? min(int(c.shifts(p.page, head)[(int(value) << c.lp) + p.at]), 31) : 0;
+    const int8_t* keys = c.keys(p.page, head) + (p.at >> 4) * c.group_bytes();
+    if (RUNS && value) {
+        turn_init(turn, c, slots, M);
+        __syncthreads();
+        const int words = turn.off ? 5 : 4;
+        for (int w = tid & 3; w < words; w += 4) {
+            const int s = turn_word(turn, w), i0 = 4 * w - turn.off;
+            if (s >= 0) {
+                const Place o = place_of(c, s);
+                const int8_t* src = c.keys(o.page, head) + c.half_bytes() + (o.at >> 4) * c.group_bytes() + (o.at & 15);
+                for (int d = tid >> 2; d < PL * c.D; d += 64) *reinterpret_cast<int*>(&vt[d * TURN + 4 * w]) = *reinterpret_cast<const int*>(src + 16 * d);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (i0 + k < 0 || i0 + k >= KV_TOKENS || turn.slot[i0 + k] < 0) continue;
+                    const Place o = place_of(c, turn.slot[i0 + k]);
+                    const int8_t* src = c.keys(o.page, head) + c.half_bytes() + (o.at >> 4) * c.group_bytes() + (o.at & 15);
+                    for (int d = tid >> 2; d < PL * c.D; d += 64) vt[d * TURN + 4 * w + k] = src[16 * d];
+                }
+            }
+        }
+        __syncthreads();
+    }
     if (t >= M) return;
-    const int slot = slots[t];
-    const bool there = slot >= 0 && slot < (c.pages << c.lp);
     int32_t* y = (value ? V : K) + size_t(t) * ld + head * c.D;
-    const int page = there ? slot >> c.lp : 0, at = there ? slot & ((1 << c.lp) - 1) : 0, t16 = at & 15;
-    const int8_t* src = c.keys(page, head) + (value ? c.half_bytes() : 0) + (at >> 4) * c.group_bytes();
-    const int e = there ? min(int(c.shifts(page, head)[(int(value) << c.lp) + at]), 31) : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = 4 * l + 64 * i;
         if (d >= c.D) break;
         int q[4] = {0, 0, 0, 0};
-        if (there) {
+        if (p.there) {
 #pragma unroll
-            for (int p = 0; p < PL; ++p) {
-                const int8_t* plane = src + p * 16 * c.D;
+            for (int n = 0; n < PL; ++n) {
                 char4 b;
                 int8_t* bb = reinterpret_cast<int8_t*>(&b);
-                if (value) {
+                if (RUNS && value) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) bb[j] = plane[c.value_at(t16, d + j)];
+                    for (int j = 0; j < 4; ++j) bb[j] = vt[(n * c.D + d + j) * TURN + t16 + turn.off];
+                } else if (value) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bb[j] = keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d + j)];
                 } else {
-                    b = *reinterpret_cast<const char4*>(plane + c.key_at(t16, d));
+                    b = *reinterpret_cast<const char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d));
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) q[j] = p == 0 ? bb[j] : 256 * q[j] + bb[j] + 128;
+                for (int j = 0; j < 4; ++j) q[j] = n == 0 ? bb[j] : 256 * q[j] + bb[j] + 128;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) q[j] = int(sat32(i64(q[j]) << e));
@@ -252,17 +326,23 @@ hipError_t launch_kv_plan(hipStream_t st, const VgemmKvPlan& p, int lp) {
     return hipGetLastError();
 }
 
+// Few tokens are mostly a decode step's, each in a page of its own: their bytes go one by one, without LDS and its two barriers. Written and read back, 8
+// heads x 128: 24 tokens apart 9.3 us so and 10.1 turned over, 1000 in a row 11.4 and 12.3 (8 bits), 4000 in a row 28.2 and 25.1 (8 bits), 5000 55 and 37 (16 bits).
+constexpr int RUNS_FROM = 4096;   // tokens times planes
+
 hipError_t launch_kv_write(hipStream_t st, const KvView& c, const int32_t* K, const int32_t* V, int ld, const int32_t* slot, int M) {
     const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, 2);
-    if (c.planes == 1) kv_write_kernel<1><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
-    else kv_write_kernel<2><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
+    const bool runs = M >= RUNS_FROM / c.planes;
+    if (c.planes == 1) runs ? kv_write_kernel<1, true><<<g, 256, 0, st>>>(c, K, V, ld, slot, M) : kv_write_kernel<1, false><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
+    else runs ? kv_write_kernel<2, true><<<g, 256, 0, st>>>(c, K, V, ld, slot, M) : kv_write_kernel<2, false><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_read(hipStream_t st, const KvView& c, const int32_t* slot, int M, int32_t* K, int32_t* V, int ld) {
     const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, K && V ? 2 : 1);
-    if (c.planes == 1) kv_read_kernel<1><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
-    else kv_read_kernel<2><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
+    const bool runs = M >= RUNS_FROM / c.planes;
+    if (c.planes == 1) runs ? kv_read_kernel<1, true><<<g, 256, 0, st>>>(c, slot, M, K, V, ld) : kv_read_kernel<1, false><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
+    else runs ? kv_read_kernel<2, true><<<g, 256, 0, st>>>(c, slot, M, K, V, ld) : kv_read_kernel<2, false><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
     return hipGetLastError();
 }
 

@@ -23,6 +23,7 @@
 
 #include "kv.h"
 #include "norm_math.h"
+#include "wave.h"
 
 namespace vk {
 
@@ -39,31 +40,6 @@ constexpr int TOP_SHIFT = 25;         // of an int32 in 8 bits
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ i64 shfl_xor64(i64 v, int d) { return i64(__shfl_xor((long long)v, d)); }
-
-// over the four lanes (fg, fr) of a query, fg = 0..3
-__device__ __forceinline__ int across_max(int v) {
-    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max(int(a[0]), int(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max(int(b[0]), int(b[1]));
-}
-__device__ __forceinline__ int across_sum(int v) {
-    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = int(a[0] + a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return int(b[0] + b[1]);
-}
-
-// inclusive running sum over the wave: within rows of sixteen, then the rows' totals handed on
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3, then 31 into 2 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
 
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int max_u16x2(int a, int b) {
@@ -261,11 +237,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         unsigned m = 0;
 #pragma unroll
         for (int b = 0; b < NS; ++b) m = max(max(m, max(uabs(x[b].x), uabs(x[b].y))), max(uabs(x[b].z), uabs(x[b].w)));
-        m = max(m, unsigned(dpp32<DPP_XOR1>(int(m))));
-        m = max(m, unsigned(dpp32<DPP_XOR2>(int(m))));
-        m = max(m, unsigned(dpp32<DPP_HALF_MIRROR>(int(m))));
-        m = max(m, unsigned(dpp32<DPP_MIRROR>(int(m))));
-        const int e = max(0, 32 - __clz(int(m)) - 14);
+        const int e = max(0, 32 - __clz(int(row_max(m))) - 14);
         int total = 0;
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
@@ -281,10 +253,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
             *reinterpret_cast<unsigned*>(&qs[0][tid >> 4][4 * fr + 64 * b]) = h;
             *reinterpret_cast<unsigned*>(&qs[1][tid >> 4][4 * fr + 64 * b]) = l;
         }
-        total += dpp32<DPP_XOR1>(total);
-        total += dpp32<DPP_XOR2>(total);
-        total += dpp32<DPP_HALF_MIRROR>(total);
-        total += dpp32<DPP_MIRROR>(total);
+        total = row_sum(total);
         if (fr == 0) {
             s.scale[tid >> 4] = ldexp(double(a.m), e - a.s);
             s.qsum[tid >> 4] = total;
@@ -526,26 +495,6 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
 
 // ---------------------------------------------------------------- the join
 
-template <int CTRL>
-__device__ __forceinline__ i64 dpp64(i64 v) { return i64(u64(unsigned(dpp32<CTRL>(int(v)))) | u64(unsigned(dpp32<CTRL>(int(v >> 32)))) << 32); }
-__device__ __forceinline__ i64 wave_sum64(i64 v) {
-    v += dpp64<DPP_XOR1>(v);
-    v += dpp64<DPP_XOR2>(v);
-    v += dpp64<DPP_HALF_MIRROR>(v);
-    v += dpp64<DPP_MIRROR>(v);
-    const auto l16 = __builtin_amdgcn_permlane16_swap(int(v), int(v), false, false), h16 = __builtin_amdgcn_permlane16_swap(int(v >> 32), int(v >> 32), false, false);
-    v = i64(u64(l16[0]) | u64(h16[0]) << 32) + i64(u64(l16[1]) | u64(h16[1]) << 32);
-    const auto l32 = __builtin_amdgcn_permlane32_swap(int(v), int(v), false, false), h32 = __builtin_amdgcn_permlane32_swap(int(v >> 32), int(v >> 32), false, false);
-    return i64(u64(l32[0]) | u64(h32[0]) << 32) + i64(u64(l32[1]) | u64(h32[1]) << 32);
-}
-__device__ __forceinline__ int wave_max(int v) {
-    v = max(v, dpp32<DPP_XOR1>(v));
-    v = max(v, dpp32<DPP_XOR2>(v));
-    v = max(v, dpp32<DPP_HALF_MIRROR>(v));
-    v = max(v, dpp32<DPP_MIRROR>(v));
-    return across_max(v);
-}
-
 // G of a span; st.y = 0: none
 __device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st) {
     const unsigned d = unsigned(mx) - unsigned(st.x);
@@ -697,32 +646,33 @@ void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
 
 hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     const int heads = a.c.heads * a.qtiles;
+    const int spans = a.window > 0 ? std::min(a.spans, a.window / KV_SPAN + 2) : a.spans;   // that a sequence may have
     const int held = 256 * kv_held(a.c.D, a.c.planes);   // blocks the card holds at a time
-    if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * a.spans > 2 * held) {
+    if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * spans > 2 * held) {
         // Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
         // of max_len (a run costs its spans and START more), and at least two where the sequences alone are more than the
         // blocks: then the longest are what is waited for.
         const float START = 1.5f;
-        const i64 spans = i64(a.rows) * a.spans;
+        const i64 all = i64(a.rows) * spans;
         int chunks = 0;
         float least = 0.f;
         for (int j = i64(a.rows) * heads > held ? 2 : 1; j <= 4; ++j) {
             const int n = std::max(1, j * held / heads);
-            const i64 most = (spans + n - 1) / n, runs = (a.spans + most - 1) / most * a.rows;
-            const float cost = float((runs * heads + held - 1) / held) * (float(spans) / float(runs) + START);
+            const i64 most = (all + n - 1) / n, runs = (spans + most - 1) / most * a.rows;
+            const float cost = float((runs * heads + held - 1) / held) * (float(all) / float(runs) + START);
             if (!chunks || cost < least) {
                 least = cost;
                 chunks = n;
             }
         }
-        launch_spans<true>(st, a, dim3(heads, int(std::min<i64>(chunks + a.rows, spans))), chunks);   // a sequence adds less than one run to them
+        launch_spans<true>(st, a, dim3(heads, int(std::min<i64>(chunks + a.rows, all))), chunks);   // a sequence adds less than one run to them
     } else {
-        const int split = int(std::max<i64>(1, std::min<i64>(a.spans, 65536 / (heads * i64(a.rows)))));
+        const int split = int(std::max<i64>(1, std::min<i64>(spans, 65536 / (heads * i64(a.rows)))));
         launch_spans<false>(st, a, dim3(heads, a.rows, split), 0);
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (a.spans <= 1) return hipSuccess;
-    if (a.spans <= JOIN_ONE) {
+    if (spans <= JOIN_ONE) {
         kv_join_kernel<1><<<dim3((a.Hq + 3) / 4, a.rows), 256, 0, st>>>(a, a.c.D);
     } else {
         const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;
