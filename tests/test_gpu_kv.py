@@ -668,3 +668,149 @@ def test_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for x, w in zip(a, want):
         assert_equal(to_np(x.d["out"]), w)
+
+
+# ---------------------------------------------------------------- every form of the kernels
+
+DEALT = 1 << 16   # a max_len that makes every call one whose spans are dealt over the card's blocks, whatever the lengths
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("D", [16, 64, 80, 128, 144, 192, 208, 256])
+@pytest.mark.parametrize("window", [0, 300])
+def test_attention_dealt(gpu, bits, D, window):
+    """Heads of every register form, sizes that fill their pieces and that do not; rows without tokens among the others."""
+    rng = np.random.default_rng(D + bits)
+    lens = rng.integers(0, 900, 20)
+    lens[[0, 7, 19]] = 0
+    a = Attend(rng, lens, 16, 2, D, bits, 6)
+    a.check(window=window)
+    a.check(window=window, max_len=DEALT if not window else 900)
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 700, 2048, 2049])
+def test_attention_dealt_over_many_rows(gpu, rows):
+    """Running sums of one and of several rows a thread, up to the most that are dealt and past them."""
+    rng = np.random.default_rng(rows)
+    lens = np.where(rng.random(rows) < 0.5, 0, rng.integers(0, 300, rows))
+    lens[rng.integers(0, rows, 3)] = [1500, 900, 513]
+    a = Attend(rng, lens, 64, 1, 16, 8, 1)
+    a.check(max_len=DEALT)
+    a.check(window=400)
+
+
+def test_attention_dealt_without_any_tokens(gpu):
+    a = Attend(np.random.default_rng(50), np.zeros(300, np.int64), 16, 4, 64, 8, 8)
+    a.check(max_len=DEALT)
+
+
+def test_attention_dealt_over_absent_pages(gpu):
+    a = Attend(np.random.default_rng(51), [1000, 800, 600, 300, 20], 16, 2, 64, 8, 4)
+    a.table[0, 3], a.table[0, 20], a.table[0, 62] = -1, a.cache.c.pages, -(1 << 31)
+    a.table[1, 16:32] = -1
+    a.table[2, :38] = 1 << 30
+    a.check(max_len=DEALT)
+
+
+@pytest.mark.parametrize("D", [16, 48, 80, 128, 256])
+@pytest.mark.parametrize("rows,Hq", [(5, 2), (130, 2)])
+def test_attention_joins(gpu, D, rows, Hq):
+    """Heads cut into dimensions where few join many spans, and whole; more spans than a block weighs at a time."""
+    rng = np.random.default_rng(D + rows)
+    lens = rng.integers(0, 600, rows)
+    lens[rows // 2] = 5000 if rows > 5 else 140000 if D == 16 else 20000
+    a = Attend(rng, lens, 256, 1, D, 8, Hq)
+    a.check(max_len=max(20000, int(lens.max())), pad=4)
+
+
+@pytest.mark.parametrize("kind", ["random", "equal", "two", "banned", "lane", "last"])
+def test_select_of_many_spans(gpu, kind):
+    """A wave a span, its best ones by threshold and one after the other."""
+    rng = np.random.default_rng(52)
+    groups, beams, n, V = 70, 4, 12, 33003
+    z = logits(rng, groups * beams, V)
+    if kind == "equal":
+        z[...] = -5
+    if kind == "two":
+        z[...] = np.where(rng.random(z.shape) < 0.5, 5, 6)
+    if kind == "banned":
+        z[rng.random(z.shape) < 0.999] = km.LOW
+        z[1] = z[4:8] = km.LOW
+    if kind == "lane":
+        z[:, 8:12] += 1 << 24
+        z[:, 264:268] += 1 << 24
+        z[:, 520:524] += 1 << 24
+        z[:, 776:780] += 1 << 24
+    if kind == "last":
+        z[:, -5:] = 1 << 29
+    check_select(z, scores(rng, groups * beams, 0.2), groups, beams, n, pad=1)
+
+
+def test_select_of_scores_far_apart(gpu):
+    """The best beams have fewer tokens than are asked for, the next lies 2^40 and more below: no key tells them apart."""
+    rng = np.random.default_rng(53)
+    for V in (3, 20):
+        s = np.array([0, -(1 << 41), -(1 << 50), (1 << 61) - 1, 5, 5, 5, -(1 << 61) + 1], np.int64)
+        check_select(logits(rng, 8, V), s, 2, 4, 4 * V if 4 * V <= 64 else 64)
+        check_select(logits(rng, 8, V), np.array([0, -(1 << 40), -(1 << 40) + 1, -(1 << 40) - 1] * 2, np.int64), 2, 4, min(4 * V, 64))
+
+
+def test_select_of_more_ties_than_are_kept(gpu):
+    rng = np.random.default_rng(54)
+    z = np.full((64, 9001), 4, np.int32)
+    check_select(z, np.zeros(64, np.int64), 2, 32, 64)
+    z[:, 7::50] = 5
+    check_select(z, np.repeat([0, 1], 32).astype(np.int64), 2, 32, 64)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("D", [16, 80, 128, 256])
+@pytest.mark.parametrize("M", [2047, 4100])
+def test_rows_of_prompts(gpu, bits, D, M):
+    """Runs of tokens that begin at every place of a group, with rows left out, and tokens in any order: words and single bytes."""
+    rng = np.random.default_rng(D + M)
+    page, heads = 32, 2
+    pages = M // page + 20
+    order = rng.permutation(pages)
+    slot, t = [], 0
+    while len(slot) < M:
+        run = int(rng.integers(1, 70))
+        at = int(rng.integers(0, 4)) + t
+        slot += [int(order[p // page]) * page + p % page for p in range(at, at + run) if p < pages * page]
+        t = at + run
+        if t >= pages * page - 80:
+            break
+    rest = rng.permutation(np.setdiff1d(np.arange(pages * page), slot))
+    slot = np.concatenate([np.array(slot[:M]), rest[:max(0, M - len(slot))]]).astype(np.int32)
+    M = len(slot)
+    slot[rng.random(M) < 0.05] = -1
+    k, v = (rows_of(rng, M, heads, D, True).reshape(M, -1) for _ in range(2))
+    C, ds = Cache(pages, page, heads, D, bits), dev(slot)
+    before = C.values()
+    vk.k_kv_write(C.c, dev(k), dev(v), heads * D, ds, M)
+    after = C.values()
+    there = slot >= 0
+    ko, vo = full((M, heads * D)), full((M, heads * D))
+    vk.k_kv_read(C.c, ds, M, ko, vo, heads * D)
+    for x, o, i in ((k, ko, 0), (v, vo, 2)):
+        q, e = km.quant(x.reshape(M, heads, D), bits)
+        before[i][slot[there]], before[i + 1][slot[there]] = q[there], e[there]
+        assert_equal(after[i], before[i])
+        assert_equal(after[i + 1], before[i + 1])
+        assert_equal(to_np(o), np.where(there[:, None], lm.sat32(q << e[..., None]).reshape(M, -1), 0))
+
+
+def test_shared_pages(gpu):
+    """The same pages in the tables of several sequences, twice in one table, and the same slot read many times."""
+    a = Attend(np.random.default_rng(55), [300, 300, 64, 300], 16, 2, 64, 8, 4)
+    a.table[1] = a.table[0]
+    a.table[3, :19] = np.repeat(a.table[0, :1], 19)
+    a.table[2, 1] = a.table[2, 0]
+    a.check()
+    M = 40
+    ds, ko, vo = dev(np.full(M, int(a.table[0, 0]) * 16 + 5, np.int32)), full((M, 128)), full((M, 128))
+    vk.k_kv_read(a.cache.c, ds, M, ko, vo, 128)
+    kq, ek, vq, ev = a.cache.values()
+    s = int(a.table[0, 0]) * 16 + 5
+    assert_equal(to_np(ko), np.repeat((kq[s] << ek[s][:, None]).reshape(1, -1), M, 0))
+    assert_equal(to_np(vo), np.repeat((vq[s] << ev[s][:, None]).reshape(1, -1), M, 0))

@@ -155,7 +155,7 @@ __device__ __forceinline__ int turn_word(const Turn& t, int w) {
 }
 
 template <int PL, bool RUNS>
-__global__ void __launch_bounds__(256) kv_write_kernel(KvView c, const int32_t* K, const int32_t* V, int ld, const int32_t* slots, int M) {
+__global__ void __launch_bounds__(256, 8) kv_write_kernel(KvView c, const int32_t* K, const int32_t* V, int ld, const int32_t* slots, int M) {
     __shared__ Turn turn;
     __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
     const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvView c, const int32_t* 
 }
 
 template <int PL, bool RUNS>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvView c, const int32_t* slots, int M, int32_t* K, int32_t* V, int ld) {
+__global__ void __launch_bounds__(256, 8) kv_read_kernel(KvView c, const int32_t* slots, int M, int32_t* K, int32_t* V, int ld) {
     __shared__ Turn turn;
     __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
     const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;

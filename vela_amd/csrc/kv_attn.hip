@@ -504,8 +504,8 @@ __device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st)
 }
 
 constexpr int JOIN_ONE = 64;       // spans that one wave joins: a lane each for their weights
-constexpr int JOIN_WAVES = 16;     // waves of a query head where there are more
-constexpr int JOIN_CHUNK = 1024;   // spans whose weights stand in LDS at a time
+constexpr int JOIN_WAVES = 8;     // waves of a query head where there are more
+constexpr int JOIN_CHUNK = 64 * JOIN_WAVES;   // spans whose weights stand in LDS at a time
 
 // A lane has four neighbouring dimensions of every (64 / lanes of a span)-th span, so that a wave reads up to 1 KB at a time. Spans are
 // weighed by a lane each. Up to JOIN_ONE spans a wave joins a query head by itself, with the first means on their way before their weights
