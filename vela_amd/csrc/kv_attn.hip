@@ -62,6 +62,12 @@ __device__ __forceinline__ int div_sat53(double n, double l, double inv) {
     return cvt_sat(q);
 }
 
+// 1 / l: an estimate and a step of Newton's, off by a few units of the last place; the quotients below are corrected
+__device__ __forceinline__ double recip(double l) {
+    const double r = __builtin_amdgcn_rcp(l);
+    return fma(fma(-l, r, 1.0), r, r);
+}
+
 struct Lds {
     uint2 table[EXP_N];                        // entry i: Lexp[i] + 2^14, Lexp[i + 1] - Lexp[i]; the last one stands for 0
     int8_t p[MAX_DIGITS][16][P_LD];
@@ -81,84 +87,105 @@ __device__ __forceinline__ int weight(const Lds& s, unsigned d) {
 // blocks of four waves that a CU holds at a time, by their registers
 constexpr int kv_held(int D, int planes) { return D <= 128 && planes == 1 ? 3 : (D + 63) / 64 * planes > 4 ? 1 : 2; }
 
-constexpr int DEAL_ROWS = 2048;   // sequences whose spans are dealt evenly: their running sums stand where the weights will
+constexpr int DEAL_ROWS = 2048;   // sequences whose spans are dealt evenly: every wave goes through their lengths, 64 at a time
 
 __device__ __forceinline__ int kv_len(const KvAttnArgs& a, int row) { return int(min(i64(max(min(a.len[row], a.max_len), 0)), i64(a.width) << a.c.lp)); }
 __device__ __forceinline__ int kv_first(const KvAttnArgs& a, int n) { return a.window > 0 ? max(0, n - a.window) : 0; }
 
-// EXACT: D == 64 NS, so that the loads' offsets are constants. DEAL: blocks take runs of spans of one sequence and key head, as even as
-// the lengths allow, so that there are about `chunks` runs a head over all sequences; every block counts them from the lengths. Else a block has
-// one span, or each gridDim.z-th.
-template <int NS, int PL, bool EXACT, bool DEAL>
+// the one of F parts of four that a lane takes: x[KT * sub + t], t < KT = 4 / F
+template <int F, class T>
+__device__ __forceinline__ T part_of(const T& x0, const T& x1, const T& x2, const T& x3, int sub, int t) {
+    if constexpr (F == 1) return t == 0 ? x0 : t == 1 ? x1 : t == 2 ? x2 : x3;
+    if constexpr (F == 2) return t == 0 ? (sub ? x2 : x0) : (sub ? x3 : x1);
+    const T lo = sub & 1 ? x1 : x0, hi = sub & 1 ? x3 : x2;
+    return sub & 2 ? hi : lo;
+}
+// over a lane's F parts, 16 / F lanes apart in a row of sixteen
+template <int F>
+__device__ __forceinline__ int parts_max(int v) {
+    if constexpr (F >= 2) v = max(v, dpp32<0x128>(v));   // row_ror 8, then 4
+    if constexpr (F == 4) v = max(v, dpp32<0x124>(v));
+    return v;
+}
+template <int F>
+__device__ __forceinline__ int parts_sum(int v) {
+    if constexpr (F >= 2) v += dpp32<0x128>(v);
+    if constexpr (F == 4) v += dpp32<0x124>(v);
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void load_words(unsigned (&w)[N], const void* p) {
+    if constexpr (N == 4) {
+        const uint4 v = *static_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *static_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        w[0] = *static_cast<const unsigned*>(p);
+    }
+}
+template <int N, class T>
+__device__ __forceinline__ void store_words(void* p, const T (&w)[N]) {
+    if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(unsigned(w[0]), unsigned(w[1]), unsigned(w[2]), unsigned(w[3]));
+    else if constexpr (N == 2) *static_cast<uint2*>(p) = make_uint2(unsigned(w[0]), unsigned(w[1]));
+    else *static_cast<unsigned*>(p) = unsigned(w[0]);
+}
+
+// EXACT: D == 64 NS, so that the loads' offsets are constants. F: up to 16 / F query heads share a key head; each stands in F columns, whose
+// lanes take a F-th of its scores, weights and results (the matrix instructions give all of them in every column).
+// chunks > 0: blocks take runs of spans of one sequence and key head, as even as the lengths allow, so that there are about `chunks` runs
+// a head over all sequences; every block counts them from the lengths. chunks = 0: a block has one span, or each gridDim.z-th.
+template <int NS, int PL, bool EXACT, int F>
 __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAttnArgs a, int chunks) {
+    constexpr int QT = 16 / F, KT = 4 / F, NK = 16 / F, JN = 4 / F;   // queries; a lane's subtiles, keys, and dimensions of four
     constexpr bool EARLY = NS * PL <= 4;       // values asked for beside the keys, and the next span's keys during the softmax: 32 NS PL registers for both
     __shared__ __attribute__((aligned(16))) Lds s;
     __shared__ __attribute__((aligned(16))) int8_t qs[2][16][64 * NS + 16];
     touch_args<int(sizeof(KvAttnArgs) + 4)>();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
+    const int qi = fr & (QT - 1), sub = fr / QT;   // the lane's query, and which part of it
+    const bool deal = chunks > 0;
     const int head = blockIdx.x / a.qtiles, q0 = (blockIdx.x % a.qtiles) * 16, nq = min(16, a.group - q0);   // key head, its first query head here and their number
     int row = blockIdx.y, chunk = blockIdx.z, split = gridDim.z;
     auto zero_row = [&](int r) {               // a sequence without tokens
         for (int i = tid; i < nq * (EXACT ? 64 * NS : a.c.D); i += 256) a.out[size_t(r) * a.ldo + size_t(head * a.group + q0) * (EXACT ? 64 * NS : a.c.D) + i] = 0;
     };
-    if constexpr (DEAL) {
-        static_assert(DEAL_ROWS * 4 <= int(sizeof s.p), "running sums");
-        constexpr int EACH = DEAL_ROWS / 256;
-        int* start = reinterpret_cast<int*>(&s.p[0][0][0]);
-        const int each = (a.rows + 255) >> 8;      // sequences of a thread: tid, tid + 256, ...
-        int count[EACH], sum = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            count[i] = 0;
-            if (i >= each) break;
-            const int r = tid + 256 * i, n = r < a.rows ? kv_len(a, r) : 0;
-            count[i] = (n + KV_SPAN - 1) / KV_SPAN - kv_first(a, n) / KV_SPAN;
-            sum += count[i];
-        }
-        // runs of at most m spans, inv = 1 / m: below 2^16 the product is off by less than 0.5 / m
-        auto runs_of = [](int n, int m, float inv) { return int((float(n + m - 1) + 0.5f) * inv); };
-        // the sum over the threads before this one, and over all
-        auto block_sum = [&](int slot, int v, int& total) {
-            const int run = wave_scan(v);
-            if (lane == 63) s.sum[slot][wave] = run;
-            __syncthreads();
-            const int w0 = s.sum[slot][0], w1 = s.sum[slot][1], w2 = s.sum[slot][2], w3 = s.sum[slot][3];
-            total = w0 + w1 + w2 + w3;
-            return run - v + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
-        };
-        int total;
-        block_sum(0, sum, total);
-        const int most = max(1, (total + chunks - 1) / chunks);   // spans of a run
-        sum = 0;
-        const float inv = 1.f / float(most);
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            if (i >= each) break;
-            count[i] = runs_of(count[i], most, inv);
-            sum += count[i];
-        }
-        int run = block_sum(1, sum, total);
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {           // in the order of threads
-            if (i >= each) break;
-            start[tid * each + i] = run;
-            run += count[i];
-        }
-        __syncthreads();
+    int n = 0;
+    auto zero_rows = [&]() {                   // of dealt spans: sequences without tokens, which no run covers
         for (int r = blockIdx.y; r < a.rows; r += int(gridDim.y))
             if (kv_len(a, r) == 0) zero_row(r);
-        if (int(blockIdx.y) >= total) return;
-        int lo = 0, hi = 256 * each;               // the last sequence whose runs begin at or before this one
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (start[mid] <= int(blockIdx.y)) lo = mid;
-            else hi = mid;
+    };
+    if (deal) {
+        // Every wave for itself, without a barrier: a lane has the sequences lane, lane + 64, ...; runs are numbered in the order of lanes.
+        auto spans_of = [&](int len) { return (len + KV_SPAN - 1) / KV_SPAN - kv_first(a, len) / KV_SPAN; };
+        const int n0 = lane < a.rows ? kv_len(a, lane) : 0, count0 = spans_of(n0);
+        int count = count0;
+#pragma unroll 4
+        for (int r = lane + 64; r < a.rows; r += 64) count += spans_of(kv_len(a, r));
+        const int most = max(1, (wave_sum(count) + chunks - 1) / chunks);   // spans of a run
+        // runs of at most `most` spans: below 2^16 the product is off by less than 0.5 / most
+        const float inv = 1.f / float(most);
+        auto runs_of = [&](int spans) { return int((float(spans + most - 1) + 0.5f) * inv); };
+        const int runs0 = runs_of(count0);
+        int runs = runs0;
+#pragma unroll 4
+        for (int r = lane + 64; r < a.rows; r += 64) runs += runs_of(spans_of(kv_len(a, r)));
+        const int end = wave_scan(runs), y = blockIdx.y;
+        if (y >= __builtin_amdgcn_readlane(end, 63)) {
+            zero_rows();
+            return;
         }
-        const int t = each == 1 ? lo : lo / each;
-        row = __builtin_amdgcn_readfirstlane(t + (lo - t * each) * 256);
-        chunk = __builtin_amdgcn_readfirstlane(int(blockIdx.y) - start[lo]);
-        split = __builtin_amdgcn_readfirstlane((lo + 1 < 256 * each ? start[lo + 1] : total) - start[lo]);
-        __syncthreads();
+        row = __ffsll((unsigned long long)__ballot(end > y)) - 1;           // the first lane whose runs end behind this one
+        chunk = y - __builtin_amdgcn_readlane(end - runs, row);
+        split = __builtin_amdgcn_readlane(runs0, row);
+        n = __builtin_amdgcn_readlane(n0, row);
+        while (chunk >= split) {               // not that lane's first sequence
+            chunk -= split;
+            row += 64;
+            n = __builtin_amdgcn_readfirstlane(kv_len(a, row));
+            split = __builtin_amdgcn_readfirstlane(runs_of(spans_of(n)));
+        }
     }
     const KvView& c = a.c;
     const int D = EXACT ? 64 * NS : c.D, P = 1 << c.lp, pieces = D >> 4;
@@ -171,9 +198,10 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         return unsigned(page) < unsigned(c.pages) ? page : -1;
     };
     int page = -1;
-    if (!DEAL && a.window == 0) page = fetch(chunk);   // on its way with the length
-    const int n = kv_len(a, row), first = kv_first(a, n), u0 = first / KV_SPAN, u1 = (n + KV_SPAN - 1) / KV_SPAN;
-    const int qh = head * a.group + q0 + fr;
+    if (!deal && a.window == 0) page = fetch(chunk);   // on its way with the length
+    if (!deal) n = kv_len(a, row);
+    const int first = kv_first(a, n), u0 = first / KV_SPAN, u1 = (n + KV_SPAN - 1) / KV_SPAN;
+    const int qh = head * a.group + q0 + qi;
     // queries: sixteen lanes a query, four neighbouring values at a time
     int4 x[NS];
     {
@@ -181,16 +209,16 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
 #pragma unroll
         for (int b = 0; b < NS; ++b) x[b] = (tid >> 4) < nq && (EXACT || 4 * fr + 64 * b < D) ? *reinterpret_cast<const int4*>(q + 64 * b) : make_int4(0, 0, 0, 0);
     }
-    if (!DEAL && n == 0 && chunk == 0) zero_row(row);
-    // DEAL: spans [u, u_end), one after the other; else u, u + split, ...
-    int u = DEAL ? u0 + int(i64(u1 - u0) * chunk / split) : u0 + chunk;
-    const int u_end = DEAL ? u0 + int(i64(u1 - u0) * (chunk + 1) / split) : u1, step = DEAL ? 1 : split;
+    if (!deal && n == 0 && chunk == 0) zero_row(row);
+    // dealt: spans [u, u_end), one after the other; else u, u + split, ...
+    int u = deal ? u0 + int(i64(u1 - u0) * chunk / split) : u0 + chunk;
+    const int u_end = deal ? u0 + int(i64(u1 - u0) * (chunk + 1) / split) : u1, step = deal ? 1 : split;
     if (u >= u_end) return;
-    if (DEAL || a.window) page = fetch(u);
+    if (deal || a.window) page = fetch(u);
 
     constexpr int KS = EARLY ? 4 : 2;          // subtiles of keys in registers
     v4i kv[KS][NS][PL], vv[NS][4][PL];
-    uint4 ek, ev;
+    unsigned ek[KT], ev[KT];
     int evb;
     // a span's group g: where its keys begin (page 0 where there is none)
     auto group = [&](int pages, int u, int g) { return c.keys(max(__shfl(pages, g), 0), head) + (((u * KV_SPAN + 16 * g) & (P - 1)) >> 4) * c.group_bytes(); };
@@ -208,8 +236,8 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         load_tiles(pages, u, 0);
         const int pg = __shfl(pages, 4 * wave + fg);
         const uint8_t* sh = c.shifts(max(pg, 0), head) + ((u * KV_SPAN + 64 * wave + 16 * fg) & (P - 1));
-        ek = *reinterpret_cast<const uint4*>(sh);
-        ev = *reinterpret_cast<const uint4*>(sh + P);
+        load_words(ek, sh + NK * sub);
+        load_words(ev, sh + P + NK * sub);
         evb = sh[P + fr];
     };
     auto load_values = [&](int pages, int u) {
@@ -223,6 +251,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         }
     };
     load_keys(page, u);
+    if (deal) zero_rows();
 
     // the table, four entries a thread
     {
@@ -260,8 +289,8 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         }
     }
     lds_barrier();
-    const double scale = s.scale[fr];
-    const int qsum = s.qsum[fr];
+    const double scale = s.scale[qi];
+    const int qsum = s.qsum[qi];
 
     for (;;) {
         const int un = u + step;
@@ -270,18 +299,24 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
             load_values(page, u);
             if (un < u_end) pagen = fetch(un);
         }
-        // which of the lane's sixteen positions count
+        // which of the lane's positions count
         const int p0 = u * KV_SPAN + 64 * wave + 16 * fg;
+        const bool there = __shfl(page, 4 * wave + fg) >= 0;
         unsigned live;
         {
-            const int from = min(max(first - p0, 0), 16), to = min(max(n - p0, 0), 16);
-            live = __shfl(page, 4 * wave + fg) >= 0 && to > from ? ((1u << to) - 1) & ~((1u << from) - 1) : 0;
+            const int from = min(max(first - p0 - NK * sub, 0), NK), to = min(max(n - p0 - NK * sub, 0), NK);
+            live = there && to > from ? ((1u << to) - 1) & ~((1u << from) - 1) : 0;
         }
-        const bool whole = __ballot(live != 0xffff) == 0;
-        const unsigned ekw[4] = {ek.x, ek.y, ek.z, ek.w};
-        unsigned evw[4] = {ev.x, ev.y, ev.z, ev.w};
-        // the least and the greatest shift of the values, as the greatest of (ev, 255 - ev) in two halves
-        int ends = live >> fr & 1 ? evb | (255 - evb) << 16 : 0;
+        const bool whole = __ballot(live != (1u << NK) - 1) == 0;
+        unsigned evw[KT];
+        unsigned ekw[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            ekw[t] = ek[t];
+            evw[t] = ev[t];
+        }
+        // the least and the greatest shift of the values, as the greatest of (ev, 255 - ev) in two halves; a lane a position
+        int ends = there && p0 + fr >= first && p0 + fr < n ? evb | (255 - evb) << 16 : 0;
         ends = max_u16x2(ends, dpp32<DPP_XOR1>(ends));
         ends = max_u16x2(ends, dpp32<DPP_XOR2>(ends));
         ends = max_u16x2(ends, dpp32<DPP_HALF_MIRROR>(ends));
@@ -293,48 +328,65 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
             ends = max_u16x2(int(e32[0]), int(e32[1]));
         }
 
-        int sc[16];
+        int sc[NK];
         int mx = INT_MIN;
-        v4i qd[NS][2];   // lane (fg, fr): the values [64 b + 16 fg, + 16) of query fr
+        v4i qd[NS][2];   // lane (fg, fr): the values [64 b + 16 fg, + 16) of its query
 #pragma unroll
         for (int b = 0; b < NS; ++b)
 #pragma unroll
-            for (int p = 0; p < 2; ++p) qd[b][p] = *reinterpret_cast<const v4i*>(&qs[p][fr][64 * b + 16 * fg]);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            if (!EARLY && ks == KS) load_tiles(page, u, KS);
-            v4i h = {0, 0, 0, 0}, mid = {0, 0, 0, 0}, l = {0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < NS; ++b) {
-                h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][0], h, 0, 0, 0);
-                if constexpr (PL == 1) {
-                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], l, 0, 0, 0);
-                } else {
-                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], mid, 0, 0, 0);
-                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][0], mid, 0, 0, 0);
-                    l = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][1], l, 0, 0, 0);
-                }
-            }
+            for (int p = 0; p < 2; ++p) qd[b][p] = *reinterpret_cast<const v4i*>(&qs[p][qi][64 * b + 16 * fg]);
+        v4i h[4], mid[4], l[4];
+        auto scores = [&](int t, const v4i& h, const v4i& mid, const v4i& l) {   // subtile t of the lane's
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 double S;
                 if constexpr (PL == 1) S = double(256 * h[j] + l[j]);
                 else S = fma(double(h[j]), 65536.0, fma(double(mid[j]), 256.0, double(l[j] + 128 * qsum)));
-                const double up = __builtin_bit_cast(double, u64(1023 + ((ekw[ks] >> (8 * j)) & 255)) << 52);
-                sc[4 * ks + j] = cvt_sat(floor(fma(S * scale, up, 0.5)));
+                const double up = __builtin_bit_cast(double, u64(1023 + ((ekw[t] >> (8 * j)) & 255)) << 52);
+                sc[4 * t + j] = cvt_sat(floor(fma(S * scale, up, 0.5)));
+            }
+        };
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            if (!EARLY && ks == KS) load_tiles(page, u, KS);
+            h[ks] = mid[ks] = l[ks] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NS; ++b) {
+                h[ks] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][0], h[ks], 0, 0, 0);
+                if constexpr (PL == 1) {
+                    l[ks] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], l[ks], 0, 0, 0);
+                } else {
+                    mid[ks] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][0], qd[b][1], mid[ks], 0, 0, 0);
+                    mid[ks] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][0], mid[ks], 0, 0, 0);
+                    l[ks] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv[ks % KS][b][1], qd[b][1], l[ks], 0, 0, 0);
+                }
+            }
+            if (F == 1) scores(ks, h[ks], mid[ks], l[ks]);
+        }
+        if constexpr (F > 1) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                v4i ht, mt = {0, 0, 0, 0}, lt;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    ht[j] = part_of<F>(h[0][j], h[1][j], h[2][j], h[3][j], sub, t);
+                    lt[j] = part_of<F>(l[0][j], l[1][j], l[2][j], l[3][j], sub, t);
+                    if (PL == 2) mt[j] = part_of<F>(mid[0][j], mid[1][j], mid[2][j], mid[3][j], sub, t);
+                }
+                scores(t, ht, mt, lt);
             }
         }
         if (!whole)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] = live >> i & 1 ? sc[i] : INT_MIN;
+            for (int i = 0; i < NK; ++i) sc[i] = live >> i & 1 ? sc[i] : INT_MIN;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = max(mx, sc[i]);
-        mx = across_max(mx);
-        if (fg == 0) s.mx[wave][fr] = mx;
+        for (int i = 0; i < NK; ++i) mx = max(mx, sc[i]);
+        mx = parts_max<F>(across_max(mx));
+        if (fg == 0) s.mx[wave][qi] = mx;
         if (lane == 0) s.ev[wave] = ends;
         if (EARLY && un < u_end) load_keys(pagen, un);
         lds_barrier();
-        mx = max(max(s.mx[0][fr], s.mx[1][fr]), max(s.mx[2][fr], s.mx[3][fr]));
+        mx = max(max(s.mx[0][qi], s.mx[1][qi]), max(s.mx[2][qi], s.mx[3][qi]));
         ends = max_u16x2(max_u16x2(s.ev[0], s.ev[1]), max_u16x2(s.ev[2], s.ev[3]));
         ends = __builtin_amdgcn_readfirstlane(ends);
         const int lo = 255 - (ends >> 16), hi = max(min(ends & 0xffff, lo + TOP_SHIFT), lo);   // lo = 255 where nothing counts
@@ -342,82 +394,81 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         const bool small = digits <= 3 && hi <= 30 - 8 * PL;   // weights of 32 bits, sums that a double holds
 
         int sum = 0;
-        int w[16];
+        int w[NK];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = weight(s, unsigned(mx) - unsigned(sc[i]));
+        for (int i = 0; i < NK; ++i) w[i] = weight(s, unsigned(mx) - unsigned(sc[i]));
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = live >> i & 1 ? w[i] : 0;
+            for (int i = 0; i < NK; ++i) w[i] = live >> i & 1 ? w[i] : 0;
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {   // shifts of what does not count become the least one
-                const unsigned keep = ((live >> (4 * ks) & 15) * 0x00204081u & 0x01010101u) * 255u;
-                evw[ks] = (evw[ks] & keep) | (unsigned(lo) * 0x01010101u & ~keep);
+            for (int t = 0; t < KT; ++t) {     // shifts of what does not count become the least one
+                const unsigned keep = ((live >> (4 * t) & 15) * 0x00204081u & 0x01010101u) * 255u;
+                evw[t] = (evw[t] & keep) | (unsigned(lo) * 0x01010101u & ~keep);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += w[i];
-        sum = across_sum(sum);
-        if (fg == 0) s.sum[wave][fr] = sum;
+        for (int i = 0; i < NK; ++i) sum += w[i];
+        sum = parts_sum<F>(across_sum(sum));
+        if (fg == 0) s.sum[wave][qi] = sum;
         i64 xs = 0;
-        int8_t* prow = &s.p[0][fr][64 * wave + 16 * fg];
+        int8_t* prow = &s.p[0][qi][64 * wave + 16 * fg + NK * sub];
         if (small) {
-            unsigned pk[3][4];
+            unsigned pk[3][KT];
             int xs32 = 0;                      // at most 256 * 2^23 in all
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                const unsigned f = evw[ks] - unsigned(lo) * 0x01010101u;   // no byte is below lo
+            for (int t = 0; t < KT; ++t) {
+                const unsigned f = evw[t] - unsigned(lo) * 0x01010101u;   // no byte is below lo
                 unsigned y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const unsigned v = unsigned(w[4 * ks + j]) << (f >> (8 * j) & 31);
+                    const unsigned v = unsigned(w[4 * t + j]) << (f >> (8 * j) & 31);
                     if (PL == 2) xs32 -= int(v);
                     y[j] = 0x8080u - v;
                 }
                 const unsigned p01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400), p23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400);
-                pk[0][ks] = __builtin_amdgcn_perm(p23, p01, 0x05040100) ^ 0x80808080u;
-                pk[1][ks] = __builtin_amdgcn_perm(p23, p01, 0x07060302) ^ 0x80808080u;
-                pk[2][ks] = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602) | __builtin_amdgcn_perm(y[3], y[2], 0x06020c0c);
+                pk[0][t] = __builtin_amdgcn_perm(p23, p01, 0x05040100) ^ 0x80808080u;
+                pk[1][t] = __builtin_amdgcn_perm(p23, p01, 0x07060302) ^ 0x80808080u;
+                pk[2][t] = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602) | __builtin_amdgcn_perm(y[3], y[2], 0x06020c0c);
             }
-            if (PL == 2) xs = across_sum(xs32);
-            *reinterpret_cast<uint4*>(prow) = make_uint4(pk[0][0], pk[0][1], pk[0][2], pk[0][3]);
-            *reinterpret_cast<uint4*>(prow + sizeof s.p[0]) = make_uint4(pk[1][0], pk[1][1], pk[1][2], pk[1][3]);
-            if (digits == 3) *reinterpret_cast<uint4*>(prow + 2 * sizeof s.p[0]) = make_uint4(pk[2][0], pk[2][1], pk[2][2], pk[2][3]);
+            if (PL == 2) xs = parts_sum<F>(across_sum(xs32));
+            store_words(prow, pk[0]);
+            store_words(prow + sizeof s.p[0], pk[1]);
+            if (digits == 3) store_words(prow + 2 * sizeof s.p[0], pk[2]);
         } else {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
+            for (int t = 0; t < KT; ++t) {
                 i64 x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[j] = -i64(u64(unsigned(w[4 * ks + j])) << ((int(evw[ks] >> (8 * j) & 255) - lo) & 31));
+                    x[j] = -i64(u64(unsigned(w[4 * t + j])) << ((int(evw[t] >> (8 * j) & 255) - lo) & 31));
                     xs += x[j];
                 }
-                for (int t = 0; t < digits; ++t) {
+                for (int d = 0; d < digits; ++d) {
                     unsigned b = 0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int d = int(int8_t(x[j]));
-                        b |= unsigned(d & 255) << (8 * j);
-                        x[j] = (x[j] - d) >> 8;
+                        const int y = int(int8_t(x[j]));
+                        b |= unsigned(y & 255) << (8 * j);
+                        x[j] = (x[j] - y) >> 8;
                     }
-                    *reinterpret_cast<unsigned*>(prow + t * int(sizeof s.p[0]) + 4 * ks) = b;
+                    *reinterpret_cast<unsigned*>(prow + d * int(sizeof s.p[0]) + 4 * t) = b;
                 }
             }
             if (PL == 2) {
-                xs += shfl_xor64(xs, 16);
-                xs += shfl_xor64(xs, 32);
+                for (int d = QT; d < 64; d <<= 1) xs += shfl_xor64(xs, d);
             }
         }
-        if (PL == 2 && fg == 0) s.x[wave][fr] = xs;
+        if (PL == 2 && fg == 0) s.x[wave][qi] = xs;
         lds_barrier();
-        sum = s.sum[0][fr] + s.sum[1][fr] + s.sum[2][fr] + s.sum[3][fr];
-        if (PL == 2) xs = s.x[0][fr] + s.x[1][fr] + s.x[2][fr] + s.x[3][fr];
+        sum = s.sum[0][qi] + s.sum[1][qi] + s.sum[2][qi] + s.sum[3][qi];
+        if (PL == 2) xs = s.x[0][qi] + s.x[1][qi] + s.x[2][qi] + s.x[3][qi];
         if (!EARLY) load_values(page, u);
 
-        int r[NS][4];
-        auto digit = [&](int t, auto add) {    // the products of one digit, handed over dimension by dimension
+        int r[NS][JN];
+        auto digit = [&](int t, auto add) {    // the products of one digit, handed over dimension by dimension: the lane's of each four
             v4i pb[4];
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) pb[kt] = *reinterpret_cast<const v4i*>(&s.p[t][fr][64 * kt + 16 * fg]);
+            for (int kt = 0; kt < 4; ++kt) pb[kt] = *reinterpret_cast<const v4i*>(&s.p[t][qi][64 * kt + 16 * fg]);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 v4i h = {0, 0, 0, 0}, l = {0, 0, 0, 0};
@@ -426,60 +477,79 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
                     h = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[i][kt][0], pb[kt], h, 0, 0, 0);
                     if constexpr (PL == 2) l = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[i][kt][1], pb[kt], l, 0, 0, 0);
                 }
+                if constexpr (PL == 2)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) add(i, j, PL == 1 ? h[j] : 256 * h[j] + l[j]);
+                    for (int j = 0; j < 4; ++j) h[j] = 256 * h[j] + l[j];
+#pragma unroll
+                for (int j = 0; j < JN; ++j) add(i, j, part_of<F>(h[0], h[1], h[2], h[3], sub, j));
             }
         };
-        const double inv = 1.0 / double(max(sum, 1));
+        const double inv = recip(double(max(sum, 1)));
         if (small) {
-            double O[NS][4];
-            const auto set = [&](int i, int j, int v) { O[i][j] = double(v); };
-            const auto add = [&](int i, int j, int v) { O[i][j] = fma(O[i][j], 256.0, double(v)); };
-            if (digits == 3) {
-                digit(2, set);
-                digit(1, add);
+            // the lower two digits' sums of up to 2^30 are one integer
+            int low[NS][JN];
+            const auto set = [&](int i, int j, int v) { low[i][j] = v; };
+            const auto add = [&](int i, int j, int v) { low[i][j] = low[i][j] * 256 + v; };
+            double O[NS][JN];
+            if (PL == 2) {                     // sums of two planes: up to 2^30 each
+                const auto set2 = [&](int i, int j, int v) { O[i][j] = double(v); };
+                const auto add2 = [&](int i, int j, int v) { O[i][j] = fma(O[i][j], 256.0, double(v)); };
+                if (digits == 3) {
+                    digit(2, set2);
+                    digit(1, add2);
+                } else {
+                    digit(1, set2);
+                }
+                digit(0, add2);
             } else {
                 digit(1, set);
+                digit(0, add);
+                if (digits == 3) {
+                    digit(2, [&](int i, int j, int v) { O[i][j] = fma(double(v), 65536.0, double(low[i][j])); });
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NS; ++i)
+#pragma unroll
+                        for (int j = 0; j < JN; ++j) O[i][j] = double(low[i][j]);
+                }
             }
-            digit(0, add);
             const double neg = -__builtin_bit_cast(double, u64(1023 + lo) << 52), half = double(sum >> 1), L = double(sum);
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < JN; ++j) {
                     const double o = PL == 2 ? fma(double(int(xs)), 128.0, O[i][j]) : O[i][j];
                     r[i][j] = sum ? div_sat53(fma(o, neg, half), L, inv) : 0;
                 }
         } else {
-            i64 O[NS][4];
+            i64 O[NS][JN];
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) O[i][j] = 0;
+                for (int j = 0; j < JN; ++j) O[i][j] = 0;
             for (int t = digits - 1; t >= 0; --t) digit(t, [&](int i, int j, int v) { O[i][j] = O[i][j] * 256 + v; });
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[i][j] = sum ? div_sat(i64(u64(-(O[i][j] + (PL == 2 ? 128 * xs : 0))) << lo) + (sum >> 1), sum, inv) : 0;
+                for (int j = 0; j < JN; ++j) r[i][j] = sum ? div_sat(i64(u64(-(O[i][j] + (PL == 2 ? 128 * xs : 0))) << lo) + (sum >> 1), sum, inv) : 0;
         }
-        if (fr < nq) {
-            const bool only = u1 - u0 == 1;
+        const bool only = u1 - u0 == 1;
+        unsigned big = 0;
+        if (qi < nq) {
             const size_t at = (size_t(row) * a.Hq + qh) * a.spans + u;
-            unsigned big = 0;
-            if (!only && wave == 0 && fg == 0) a.stat[at] = make_int2(mx, sum);
-            int32_t* y = (only ? a.out + size_t(row) * a.ldo + size_t(qh) * D : a.part + at * D) + 16 * wave + 4 * fg;
+            if (!only && wave == 0 && fg == 0 && sub == 0) a.stat[at] = make_int2(mx, sum);
+            int32_t* y = (only ? a.out + size_t(row) * a.ldo + size_t(qh) * D : a.part + at * D) + 16 * wave + 4 * fg + JN * sub;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 if (!EXACT && wave + 4 * i >= pieces) break;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) big = max(big, uabs(r[i][j]));
-                *reinterpret_cast<int4*>(y + 64 * i) = make_int4(r[i][0], r[i][1], r[i][2], r[i][3]);
+                for (int j = 0; j < JN; ++j) big = max(big, uabs(r[i][j]));
+                store_words(y + 64 * i, r[i]);
             }
-            if (only && a.rowmax) {
-                big = max(big, unsigned(__shfl_xor(int(big), 16)));
-                big = max(big, unsigned(__shfl_xor(int(big), 32)));
-                if (fg == 0 && big) atomicMax(a.rowmax + row, big);
-            }
+        }
+        if (only && a.rowmax) {
+            for (int d = 1; d < 64; d <<= 1) big = max(big, unsigned(__shfl_xor(int(big), d)));
+            if (lane == 0 && big) atomicMax(a.rowmax + row, big);
         }
         u = un;
         if (u >= u_end) return;
@@ -626,20 +696,25 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
     }
 }
 
-template <int PL, bool EXACT, bool DEAL>
+template <int PL, bool EXACT, int F>
 void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     switch ((a.c.D + 63) / 64) {
-        case 1: kv_attn_kernel<1, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
-        case 2: kv_attn_kernel<2, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
-        case 3: kv_attn_kernel<3, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks); break;
-        default: kv_attn_kernel<4, PL, EXACT, DEAL><<<g, 256, 0, st>>>(a, chunks);
+        case 1: kv_attn_kernel<1, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
+        case 2: kv_attn_kernel<2, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
+        case 3: kv_attn_kernel<3, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
+        default: kv_attn_kernel<4, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks);
     }
 }
-template <bool DEAL>
+template <int F>
 void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     const bool exact = a.c.D % 64 == 0;
-    if (a.c.planes == 1) exact ? launch_spans<1, true, DEAL>(st, a, g, chunks) : launch_spans<1, false, DEAL>(st, a, g, chunks);
-    else exact ? launch_spans<2, true, DEAL>(st, a, g, chunks) : launch_spans<2, false, DEAL>(st, a, g, chunks);
+    if (a.c.planes == 1) exact ? launch_spans<1, true, F>(st, a, g, chunks) : launch_spans<1, false, F>(st, a, g, chunks);
+    else exact ? launch_spans<2, true, F>(st, a, g, chunks) : launch_spans<2, false, F>(st, a, g, chunks);
+}
+void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
+    if (a.group <= 4) launch_spans<4>(st, a, g, chunks);
+    else if (a.group <= 8) launch_spans<2>(st, a, g, chunks);
+    else launch_spans<1>(st, a, g, chunks);
 }
 
 }  // namespace
@@ -665,10 +740,10 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
                 chunks = n;
             }
         }
-        launch_spans<true>(st, a, dim3(heads, int(std::min<i64>(chunks + a.rows, all))), chunks);   // a sequence adds less than one run to them
+        launch_spans(st, a, dim3(heads, int(std::min<i64>(chunks + a.rows, all))), chunks);   // a sequence adds less than one run to them
     } else {
         const int split = int(std::max<i64>(1, std::min<i64>(spans, 65536 / (heads * i64(a.rows)))));
-        launch_spans<false>(st, a, dim3(heads, a.rows, split), 0);
+        launch_spans(st, a, dim3(heads, a.rows, split), 0);
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (a.spans <= 1) return hipSuccess;
