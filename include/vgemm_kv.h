@@ -64,7 +64,8 @@ int vgemm_kv_plan(void* stream, const VgemmKvPlan* P);
 int vgemm_kv_write(void* stream, const VgemmKv* C, const int32_t* K, const int32_t* V, int ld, const int32_t* slot, int M);
 /* The rows q 2^e of slots slot[t], saturated to 32 bits; rows of 0 where the slot lies outside [0, pages * page). K or V may be NULL. */
 int vgemm_kv_read(void* stream, const VgemmKv* C, const int32_t* slot, int M, int32_t* K, int32_t* V, int ld);
-/* Page dst[i] becomes a copy of page src[i], i < n, data and shifts; pairs with a number outside [0, pages) are left out. No page is the dst of two pairs, or the dst of one and the src of another. */
+/* Page dst[i] becomes a copy of page src[i], i < n <= 2^23, data and shifts; pairs with a number outside [0, pages) are left out. No page is the dst of
+ * two pairs, or the dst of one and the src of another. */
 int vgemm_kv_copy(void* stream, const VgemmKv* C, const int32_t* src, const int32_t* dst, int n);
 
 /* Attention of one new token for each of `rows` sequences. Q [rows x ldq]: Hq heads of D values (Hq a multiple of the cache's

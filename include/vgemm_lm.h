@@ -1,8 +1,8 @@
 /*
  * vgemm_lm -- operators of a language model's decode step in the library's exact integer arithmetic: part of
  * libvgemm.so, beside the W8A16 products, norms and GEGLU blocks of vgemm.h. No counterparts in the reference. Of such a
- * step these are the norms, the projections and the feed-forward layers, dense or of experts; rotary positions, attention over a
- * cache and sampling are not there, and no engine block or container of vgemm_engine.h / vgemm_model.h uses them.
+ * step these are the norms, the projections and the feed-forward layers, dense or of experts; the key-value cache, its attention and beam search are in
+ * vgemm_kv.h, rotary positions and sampling are not there, and no engine block or container of vgemm_engine.h / vgemm_model.h uses them.
  *
  *   vgemm_rmsnorm_q     residual addition, root-mean-square norm, 8-bit rows (or the int16 view)
  *   vgemm_w4_pack       4-bit weights with group scales and zero points, laid out for the products

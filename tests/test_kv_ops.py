@@ -92,7 +92,7 @@ def test_row_refusals(change, rc, msg):
 
 
 @pytest.mark.parametrize("src,dst,n,rc,msg", [(None, FAKE, 3, -1, "src and dst"), (FAKE, None, 3, -1, "src and dst"), (FAKE, FAKE, -1, -1, "bad arguments"),
-                                              (FAKE, FAKE, (1 << 24) + 1, -3, "at most 16777216")])
+                                              (FAKE, FAKE, (1 << 23) + 1, -3, "at most 8388608")])
 def test_copy_refusals(src, dst, n, rc, msg):
     assert _lib.load().vgemm_kv_copy(None, ctypes.byref(cache()), src, dst, n) == rc
     assert msg in last()

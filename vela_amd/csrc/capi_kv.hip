@@ -99,7 +99,7 @@ int vgemm_kv_copy(void* stream, const VgemmKv* C, const int32_t* src, const int3
     if (n < 0) return fail(VGEMM_ERR_ARG, "kv_copy: bad arguments");
     if (n == 0) return ok();
     if (!src || !dst) return fail(VGEMM_ERR_ARG, "kv_copy: src and dst required");
-    if (n > (1 << 24)) return fail(VGEMM_ERR_UNSUPPORTED, "kv_copy: at most %d pages a call, not %d", 1 << 24, n);
+    if (n > (1 << 23)) return fail(VGEMM_ERR_UNSUPPORTED, "kv_copy: at most %d pages a call, not %d", 1 << 23, n);   // what a grid holds
     return hip_status(vk::launch_kv_copy(static_cast<hipStream_t>(stream), kv_view(*C), src, dst, n), "kv_copy launch");
 }
 

@@ -2,11 +2,12 @@
 //
 // The weights of a softmax need the row's maximum before their sum, and a rounded weight cannot be rescaled exactly. The
 // operator is therefore defined on spans of 256 positions: a span's weights are relative to its own maximum, its mean is rounded to 32 bits, and the means
-// are joined with the spans' weights. A span needs one pass over its keys and values, any split of the sequence into spans gives the same
-// numbers, and what goes from the first kernel to the join is 4 D bytes a span and query head beside 512 D planes of cache.
+// are joined with the spans' weights. A span needs one pass over its keys and values, the numbers do not depend on which block takes which
+// span, and what goes from the first kernel to the join is 4 D bytes a span and query head beside the 512 D bytes of its 8-bit keys and values.
 //
-// A block of four waves takes a span of one sequence and key head with up to sixteen of its query heads, one a column of the 16x16x64 int8
-// matrix instruction.
+// A block of four waves takes a span of one sequence and key head with up to sixteen of its query heads, the columns of the 16x16x64 int8
+// matrix instruction. What bounds it is memory: two sequences of 131072 tokens (8 x 128 heads, 8 bits, 32 query heads) take 111 us, 4.8 TB/s of
+// cache, against 5.0 for a copy; a span alone is a chain of two loads and ~3.5 us of work, 5.8 us for a sequence of 500 tokens (16 x 64, 16 bits).
 //   * Scores: wave w has the positions [64 w, 64 w + 64). The keys are the A operand; row i of subtile ks is position 16 (i / 4) + 4 ks + i % 4, so that
 //     lane (fg, query) ends with the scores of the 16 positions from 16 fg on, in order. Quarters of four tokens
 //     lie together in a page (vgemm_kv.h), so a load touches four runs of 256 bytes.
@@ -30,8 +31,6 @@ namespace vk {
 namespace {
 
 constexpr int EXP_N = 1025;
-
-
 constexpr int MAX_DIGITS = 6;         // 15 bits and shifts up to 25 apart
 constexpr int P_LD = KV_SPAN + 16;    // bytes of a query's weights in LDS, one digit: rows 4 banks apart
 constexpr int TOP_SHIFT = 25;         // of an int32 in 8 bits
@@ -75,6 +74,7 @@ struct Lds {
     i64 x[4][16];
     double scale[16];
     int qsum[16];
+    unsigned big[4];
 };
 
 // rshr(lutexp(d), 15), at most 32767
@@ -133,7 +133,8 @@ __device__ __forceinline__ void store_words(void* p, const T (&w)[N]) {
 }
 
 // EXACT: D == 64 NS, so that the loads' offsets are constants. F: up to 16 / F query heads share a key head; each stands in F columns, whose
-// lanes take a F-th of its scores, weights and results (the matrix instructions give all of them in every column).
+// lanes take a F-th of its scores, weights and results (the matrix instructions give all of them in every column): 780 vector instructions a wave and
+// span for 128 values in 8 bits with F = 1, about 450 with 4; four queries a key, 32 x 8192 tokens of 64 values 82 -> 73 us, of 128 89 % of the time.
 // chunks > 0: blocks take runs of spans of one sequence and key head, as even as the lengths allow, so that there are about `chunks` runs
 // a head over all sequences; every block counts them from the lengths. chunks = 0: a block has one span, or each gridDim.z-th.
 template <int NS, int PL, bool EXACT, int F>
@@ -211,8 +212,8 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
     }
     if (!deal && n == 0 && chunk == 0) zero_row(row);
     // dealt: spans [u, u_end), one after the other; else u, u + split, ...
-    int u = deal ? u0 + int(i64(u1 - u0) * chunk / split) : u0 + chunk;
-    const int u_end = deal ? u0 + int(i64(u1 - u0) * (chunk + 1) / split) : u1, step = deal ? 1 : split;
+    int u = deal ? u0 + (u1 - u0) * chunk / split : u0 + chunk;   // at most 2^15 spans: the products stay below 2^30
+    const int u_end = deal ? u0 + (u1 - u0) * (chunk + 1) / split : u1, step = deal ? 1 : split;
     if (u >= u_end) return;
     if (deal || a.window) page = fetch(u);
 
@@ -547,9 +548,12 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
                 store_words(y + 64 * i, r[i]);
             }
         }
-        if (only && a.rowmax) {
-            for (int d = 1; d < 64; d <<= 1) big = max(big, unsigned(__shfl_xor(int(big), d)));
-            if (lane == 0 && big) atomicMax(a.rowmax + row, big);
+        if (only && a.rowmax) {                // one atomic a block; its only span
+            big = unsigned(wave_max(int(big ^ 0x80000000u))) ^ 0x80000000u;
+            if (lane == 0) s.big[wave] = big;
+            lds_barrier();
+            big = max(max(s.big[0], s.big[1]), max(s.big[2], s.big[3]));
+            if (tid == 0 && big) atomicMax(a.rowmax + row, big);
         }
         u = un;
         if (u >= u_end) return;
@@ -579,7 +583,7 @@ constexpr int JOIN_CHUNK = 64 * JOIN_WAVES;   // spans whose weights stand in LD
 
 // A lane has four neighbouring dimensions of every (64 / lanes of a span)-th span, so that a wave reads up to 1 KB at a time. Spans are
 // weighed by a lane each. Up to JOIN_ONE spans a wave joins a query head by itself, with the first means on their way before their weights
-// are known; beyond that sixteen waves do, and dims of D dimensions a block where the heads alone would leave CUs idle.
+// are known; beyond that eight waves do, and dims of D dimensions a block where the heads alone would leave CUs idle.
 template <int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(KvAttnArgs a, int dims) {
     constexpr int AHEAD = 8;
@@ -591,9 +595,9 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int D = a.c.D, parts = (D + dims - 1) / dims, row = blockIdx.y;
     const int qh = WAVES == 1 ? int(blockIdx.x) * 4 + wave : int(blockIdx.x) / parts, d0 = WAVES == 1 ? 0 : (int(blockIdx.x) % parts) * dims;
-    const int n = kv_len(a, row), u0 = kv_first(a, n) / KV_SPAN, count = (n + KV_SPAN - 1) / KV_SPAN - u0;
-    if (count <= 1 || qh >= a.Hq) return;      // the first kernel has written the row
-    const size_t at = (size_t(row) * a.Hq + qh) * a.spans + u0;
+    // without a window the first loads do not wait for the length: they stay within max_len's spans, and what lies behind the sequence's has no weight
+    const int n = kv_len(a, row), u0 = a.window ? kv_first(a, n) / KV_SPAN : 0, count = (n + KV_SPAN - 1) / KV_SPAN - u0, most = a.window ? max(count, 1) : a.spans;
+    const size_t at = (size_t(row) * a.Hq + min(qh, a.Hq - 1)) * a.spans + u0;
     const int quads = min(dims, D - d0) / 4, per = quads <= 4 ? 4 : quads <= 8 ? 8 : quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // lanes of a span
     const int groups = 64 / per, quad = lane & (per - 1), sub = lane / per;
     const int32_t* part = a.part + at * D + d0 + 4 * min(quad, quads - 1);
@@ -607,8 +611,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
     if constexpr (WAVES == 1) {
         int4 v[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(sub + i * groups, count - 1)) * D);
-        const int2 st = lane < count ? a.stat[at + lane] : make_int2(INT_MIN, 0);
+        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(sub + i * groups, most - 1)) * D);
+        int2 st = a.stat[at + min(lane, most - 1)];
+        if (count <= 1) return;                // the first kernel has written the row
+        if (lane >= count) st = make_int2(INT_MIN, 0);
         const int mx = wave_max(st.y ? st.x : INT_MIN);
         const i64 G = join_weight(a, mx, st);
         const int h = max(0, 64 - __clzll((long long)wave_sum64(G)) - 30);
@@ -621,11 +627,13 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
             add(w, *reinterpret_cast<const int4*>(part + size_t(min(k, count - 1)) * D));
         }
     } else {
-        // the thread's spans tid + 1024 i: the first one's statistics stay in registers
+        // the thread's spans tid + 512 i: the first one's statistics stay in registers
         int4 v[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(wave * groups + sub + i * WAVES * groups, count - 1)) * D);
-        const int2 st0 = tid < count ? a.stat[at + tid] : make_int2(INT_MIN, 0);
+        for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const int4*>(part + size_t(min(wave * groups + sub + i * WAVES * groups, most - 1)) * D);
+        int2 st0 = a.stat[at + min(tid, most - 1)];
+        if (count <= 1) return;
+        if (tid >= count) st0 = make_int2(INT_MIN, 0);
         int mx = st0.y ? st0.x : INT_MIN;
         for (int k = tid + JOIN_CHUNK; k < count; k += JOIN_CHUNK) {
             const int2 st = a.stat[at + k];
@@ -680,7 +688,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
             for (int w = 0; w < WAVES; ++w) x[j] += acc[w][quad][j];
         }
     }
-    const bool mine = sub == 0 && quad < quads;
+    const bool mine = sub == 0 && quad < quads && qh < a.Hq;
     const double inv = 1.0 / double(T ? T : 1);
     int r[4];
     unsigned big = 0;
@@ -690,8 +698,15 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
         big = max(big, mine ? uabs(r[j]) : 0u);
     }
     if (mine) *reinterpret_cast<int4*>(a.out + size_t(row) * a.ldo + size_t(qh) * D + d0 + 4 * quad) = make_int4(r[0], r[1], r[2], r[3]);
-    if (a.rowmax) {
-        for (int d = 1; d < 64; d <<= 1) big = max(big, unsigned(__shfl_xor(int(big), d)));
+    if (!a.rowmax) return;
+    big = unsigned(wave_max(int(big ^ 0x80000000u))) ^ 0x80000000u;
+    if constexpr (WAVES == 1) {                // one atomic a block: 32 of them on a row's word cost 2 us
+        __shared__ unsigned bigs[4];
+        if (lane == 0) bigs[wave] = big;
+        __syncthreads();
+        big = max(max(bigs[0], bigs[1]), max(bigs[2], bigs[3]));
+        if (tid == 0 && big) atomicMax(a.rowmax + row, big);
+    } else {
         if (lane == 0 && big) atomicMax(a.rowmax + row, big);
     }
 }
