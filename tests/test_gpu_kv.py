@@ -814,3 +814,16 @@ def test_shared_pages(gpu):
     s = int(a.table[0, 0]) * 16 + 5
     assert_equal(to_np(ko), np.repeat((kq[s] << ek[s][:, None]).reshape(1, -1), M, 0))
     assert_equal(to_np(vo), np.repeat((vq[s] << ev[s][:, None]).reshape(1, -1), M, 0))
+
+
+def test_attention_over_two_million_tokens(gpu):
+    """A table that names the same pages again and again: 8192 spans."""
+    rng = np.random.default_rng(56)
+    a = Attend(rng, [700, 300], 256, 1, 16, 8, 2)
+    n = (1 << 21) - 100
+    pages = a.table[0, :3].copy()
+    a.table = np.full((2, n // 256 + 1), -1, np.int32)
+    a.table[0] = rng.choice(pages, a.table.shape[1])
+    a.table[1, :2] = pages[:2]
+    a.lens, a.width = np.array([n, 300]), a.table.shape[1]
+    a.check()

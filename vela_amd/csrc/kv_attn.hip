@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         int count = count0;
 #pragma unroll 4
         for (int r = lane + 64; r < a.rows; r += 64) count += spans_of(kv_len(a, r));
-        const int most = max(1, (wave_sum(count) + chunks - 1) / chunks);   // spans of a run
+        const int most = min(max(1, (wave_sum(count) + chunks - 1) / chunks), KV_MAX_LEN / KV_SPAN);   // spans of a run
         // runs of at most `most` spans: below 2^16 the product is off by less than 0.5 / most
         const float inv = 1.f / float(most);
         auto runs_of = [&](int spans) { return int((float(spans + most - 1) + 0.5f) * inv); };
@@ -577,8 +577,8 @@ __device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st)
     return ((t + (((t1 - t) * i64(d & 1023)) >> 10) + 64) >> 7) * st.y;
 }
 
-constexpr int JOIN_ONE = 64;       // spans that one wave joins: a lane each for their weights
-constexpr int JOIN_WAVES = 8;     // waves of a query head where there are more
+constexpr int JOIN_ONE = 64;       // spans that one wave joins, a lane each for their weights: 8 spans 13.0 us a pass so and 19.2 with eight waves, 64 of 32 sequences 242 and 244
+constexpr int JOIN_WAVES = 8;      // waves of a query head where there are more
 constexpr int JOIN_CHUNK = 64 * JOIN_WAVES;   // spans whose weights stand in LDS at a time
 
 // A lane has four neighbouring dimensions of every (64 / lanes of a span)-th span, so that a wave reads up to 1 KB at a time. Spans are
@@ -739,8 +739,9 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     const int spans = a.window > 0 ? std::min(a.spans, a.window / KV_SPAN + 2) : a.spans;   // that a sequence may have
     const int held = 256 * kv_held(a.c.D, a.c.planes);   // blocks the card holds at a time
     if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * spans > 2 * held) {
-        // Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
-        // of max_len (a run costs its spans and START more), and at least two where the sequences alone are more than the
+        // Blocks with more than two spans each take them as dealt (32 x 4096 tokens 80.6 us a pass, 85.7 with a block a span; 16 x 2000, 1.3 spans a block,
+        // 29.3 and 28.0). Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
+        // of max_len (a run costs its spans and START more; 64 x 8192 tokens in two runs a block 256 us, in one 282), and at least two where the sequences alone are more than the
         // blocks: then the longest are what is waited for.
         const float START = 1.5f;
         const i64 all = i64(a.rows) * spans;
@@ -765,7 +766,7 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     if (spans <= JOIN_ONE) {
         kv_join_kernel<1><<<dim3((a.Hq + 3) / 4, a.rows), 256, 0, st>>>(a, a.c.D);
     } else {
-        const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;
+        const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;   // 64 heads of 128: 10.4 us so, 16.4 with a block a head
         kv_join_kernel<JOIN_WAVES><<<dim3(a.Hq * ((a.c.D + dims - 1) / dims), a.rows), 64 * JOIN_WAVES, 0, st>>>(a, dims);
     }
     return hipGetLastError();
