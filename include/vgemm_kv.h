@@ -71,7 +71,7 @@ int vgemm_kv_copy(void* stream, const VgemmKv* C, const int32_t* src, const int3
 /* Attention of one new token for each of `rows` sequences. Q [rows x ldq]: Hq heads of D values (Hq a multiple of the cache's
  * heads; query head h reads head h / (Hq / heads)). Sequence r holds n = min(max(len[r], 0), max_len, width * page) tokens (the new one among them,
  * written before), token j in page table[r, j / page]; with window > 0 only the last `window` of them count, and none
- * whose table entry lies outside [0, pages). For a query head:
+ * whose table entry lies outside [0, pages); the slots of those that count have been written by vgemm_kv_write (or copied). For a query head:
  *   q = rshr(x, eq), eq the least shift >= 0 with max |x| < 2^(14 + eq)
  *   s_j = rshr(m sum_d q_d k_jd, s - eq - ek_j)                         1 <= m <= 32768, -64 <= s <= 128
  * Tokens go in spans of 256 positions, [256 u, 256 u + 256). In a span, over the tokens that count:

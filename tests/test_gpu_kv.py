@@ -821,7 +821,7 @@ def test_attention_over_two_million_tokens(gpu):
     rng = np.random.default_rng(56)
     a = Attend(rng, [700, 300], 256, 1, 16, 8, 2)
     n = (1 << 21) - 100
-    pages = a.table[0, :3].copy()
+    pages = a.table[0, :2].copy()      # the filled ones: a slot that no call has written has no value
     a.table = np.full((2, n // 256 + 1), -1, np.int32)
     a.table[0] = rng.choice(pages, a.table.shape[1])
     a.table[1, :2] = pages[:2]
