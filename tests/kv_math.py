@@ -70,8 +70,8 @@ def attend(q, k, ek, v, ev, ok, heads, m, s, L):
         S = np.rint(k[at, g].astype(np.float64) @ x.astype(np.float64)).astype(I64)
         z = lm.rshr(S * m, s - eq - ek[at, g].astype(I64))
         mx, Ls, As = [], [], []
-        for u in np.unique(at // SPAN):
-            i = at // SPAN == u
+        ends = np.flatnonzero(np.diff(at // SPAN, append=-1)) + 1
+        for i in map(slice, np.concatenate([[0], ends[:-1]]), ends):
             top = z[i].max()
             P = np.minimum(32767, (lutexp(top - z[i], L) + (1 << 14)) >> 15)
             w = int(P.sum())
