@@ -53,18 +53,46 @@ constexpr int LIST = 192;   // keys of a wave that reach the threshold: n and a 
 
 struct SpanLds {
     uint2 table[EXP_N];     // entry i: Lexp[i], Lexp[i + 1] - Lexp[i]; the last one stands for 0
-    u64 list[4][LIST];
+    u64 list[4 * LIST];     // a wave's own part, or a block's
     i64 sum[4];
-    int mx[4], count[4];
+    int mx[4], count;
     unsigned reach[4];
 };
+
+// lanes below this one among those of mask
+__device__ __forceinline__ int below(u64 mask) { return int(__builtin_amdgcn_mbcnt_hi(unsigned(mask >> 32), __builtin_amdgcn_mbcnt_lo(unsigned(mask), 0))); }
+
+// use(key, rank) for each of c keys, its rank the number of greater ones, by `rows` rows of sixteen lanes. Up to 64 keys a row takes one, a lane four of the
+// others (4 x 32000 logits: 6.9 -> 5.7 us); beyond that a lane takes one and goes through all.
+template <class U>
+__device__ __forceinline__ void by_rank(const u64* list, int c, int row, int rows, int l, U use) {
+    if (c <= 64) {
+        for (int i0 = 0; i0 < c; i0 += rows) {   // whole rows: every lane takes part in the sums
+            const int i = i0 + row;
+            const u64 k = list[min(i, c - 1)];
+            int rank = 0;
+#pragma unroll
+            for (int j = 0; j < 64; j += 16)
+                if (j < c) rank += j + l < c && list[min(j + l, c - 1)] > k;
+            rank = row_sum(rank);
+            if (l == 0 && i < c) use(k, rank);
+        }
+    } else {
+        for (int i = row * 16 + l; i < c; i += rows * 16) {
+            const u64 k = list[i];
+            int rank = 0;
+            for (int j = 0; j < c; ++j) rank += list[j] > k;
+            use(k, rank);
+        }
+    }
+}
 
 struct __attribute__((packed, aligned(4))) Quad { int v[4]; };   // sixteen bytes that lie where rows of any length put them
 
 // One span of one row, by WAVES waves of a block of four: one where there are spans for all CUs (a wave's search, sums and order then serve 64
-// values a lane: 200 x 100003 logits 49 -> 22 us), four where the call's own latency counts (4 x 32000: 6.4 us).
+// values a lane: 200 x 100003 logits 49 -> 22 us, 3.6 TB/s, 13 of them the read alone), four where the call's own latency counts (4 x 32000: 5.8 us).
 template <int WAVES>
-__global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(256, WAVES == 1 ? 5 : 4) beam_span_kernel(BeamArgs a) {
     constexpr int PER = BEAM_SPAN / (64 * WAVES);
     __shared__ SpanLds s;
     touch_args<int(sizeof(BeamArgs))>();
@@ -100,6 +128,7 @@ __global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
         for (int i = 0; i < 4; ++i) s.table[4 * tid + i] = make_uint2(unsigned(t[i]), unsigned(t[i + 1] - t[i]));
         if (tid == 0) s.table[EXP_N - 1] = make_uint2(0, 0);
     }
+    if (tid == 0) s.count = 0;
     int mx = INT_MIN;
 #pragma unroll
     for (int i = 0; i < PER; ++i) mx = max(mx, v[i]);
@@ -108,7 +137,6 @@ __global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
     if (lane == 0) {
         s.mx[wave] = mx;
         s.reach[wave] = reach;
-        s.count[wave] = 0;
     }
     __syncthreads();
     if (!in || score == LLONG_MIN) return;     // no such beam: nothing reads its part of the workspace
@@ -117,12 +145,29 @@ __global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
         reach = max(max(s.reach[0], s.reach[1]), max(s.reach[2], s.reach[3]));
     }
     const int least = int(reach ^ 0x80000000u);   // above what is banned
+    // what reaches the threshold, one after the other in the wave's part of the list, or in the block's from where the wave's begin
+    u64* list = WAVES == 4 ? s.list : s.list + wave * LIST;
+    int found = 0, at = 0;
+    if (WAVES == 4) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (v[i] >= least) {
-            const int at = atomicAdd(&s.count[wave], 1);
-            if (at < LIST) s.list[wave][at] = key_of(v[i], place(i));
+        for (int i = 0; i < PER; ++i) found += __popcll(__ballot(v[i] >= least));
+        if (found <= LIST) {
+            if (lane == 0) at = atomicAdd(&s.count, found);
+            at = __builtin_amdgcn_readfirstlane(at);
         }
+        found = found <= LIST ? 0 : found;        // to be counted again, or too many
+    }
+    if (found == 0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const u64 mask = __ballot(v[i] >= least);
+            if (!mask) continue;
+            const int to = found + below(mask);
+            if (v[i] >= least && to < LIST) list[at + to] = key_of(v[i], place(i));
+            found += __popcll(mask);
+        }
+    }
+    const bool over = found > LIST;
     i64 sum = 0;
     // what is banned lies far enough below any maximum but those near it
     const bool low = mx < INT_MIN + (1 << 20);
@@ -137,10 +182,13 @@ __global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
         asm volatile("" ::: "memory");   // eight table entries on their way at a time, not 64
     }
     sum = wave_sum64(sum);
-    wave_lds();
-    if (s.count[wave] > LIST) {                   // one after the other: each the greatest below the last
-        int lz = INT_MAX, lp = -1, k = 0;         // the last one's logit and place
-        for (; k < n; ++k) {
+    if (over) {                                   // one after the other: each the greatest below the last
+        if (WAVES == 4) {
+            if (lane == 0) at = atomicAdd(&s.count, n);
+            at = __builtin_amdgcn_readfirstlane(at);
+        }
+        int lz = INT_MAX, lp = -1;                // the last one's logit and place
+        for (int k = 0; k < n; ++k) {             // LIST of them there are, and more
             int bz = INT_MIN, bp = 0;
             const int rel = lp - 4 * t0;
 #pragma unroll
@@ -154,38 +202,28 @@ __global__ void __launch_bounds__(256, 4) beam_span_kernel(BeamArgs a) {
             }
             u64 best = key_of(bz, 4 * t0 + bp);
             for (int d = 1; d < 64; d <<= 1) best = max(best, u64(__shfl_xor((unsigned long long)best, d)));
-            if (!best) break;
-            if (lane == 0) s.list[wave][k] = best;
+            if (lane == 0) list[at + k] = best;
             lz = key_logit(best);
             lp = key_place(best);
         }
-        if (lane == 0) s.count[wave] = k;
-        wave_lds();
+        found = n;
     }
-    if (lane == 0) s.sum[wave] = sum;
     int2* cand = a.cand + out * n;
+    auto put = [&](u64 k, int rank) {
+        if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
+    };
     if constexpr (WAVES == 1) {
-        const int c = s.count[wave];
+        wave_lds();
         if (lane == 0) a.stat[out] = BeamStat{sum, mx, 0};
-        for (int i = lane; i < c; i += 64) {
-            const u64 k = s.list[wave][i];
-            int rank = 0;
-            for (int j = 0; j < c; ++j) rank += s.list[wave][j] > k;
-            if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
-        }
-        for (int i = c + lane; i < n; i += 64) cand[i] = make_int2(INT_MIN, -1);
+        by_rank(list, found, lane >> 4, 4, lane & 15, put);
+        for (int i = found + lane; i < n; i += 64) cand[i] = make_int2(INT_MIN, -1);
     } else {
+        if (lane == 0) s.sum[wave] = sum;
         __syncthreads();
         if (tid == 0) a.stat[out] = BeamStat{s.sum[0] + s.sum[1] + s.sum[2] + s.sum[3], mx, 0};
-        const int all = s.count[0] + s.count[1] + s.count[2] + s.count[3];
-        for (int i = lane; i < s.count[wave]; i += 64) {
-            const u64 k = s.list[wave][i];
-            int rank = 0;
-            for (int w = 0; w < 4; ++w)
-                for (int j = 0; j < s.count[w]; ++j) rank += s.list[w][j] > k;
-            if (rank < n) cand[rank] = make_int2(key_logit(k), base + key_place(k));
-        }
-        for (int i = all + tid; i < n; i += 256) cand[i] = make_int2(INT_MIN, -1);
+        const int c = s.count;
+        by_rank(list, c, tid >> 4, 16, tid & 15, put);
+        for (int i = c + tid; i < n; i += 256) cand[i] = make_int2(INT_MIN, -1);
     }
 }
 
@@ -267,41 +305,54 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
     __syncthreads();
     unsigned reach = 1;
     for (int w = 0; w < WAVES; ++w) reach = max(reach, reach_of[w]);
+    // each list's first entries that reach the threshold: all of a wave's get their places at once
+    u64 y[LISTS][AHEAD];
+    int mine = 0;
 #pragma unroll
     for (int i = 0; i < LISTS; ++i)
-        for (int j = 0; j < n; ++j) {
-            const int2 k = j == 0 ? first[i][0] : j == 1 ? first[i][1] : tid + THREADS * i < lists ? cand[size_t(tid + THREADS * i) * n + j] : make_int2(INT_MIN, -1);
-            const u64 y = key(i, k);
-            if (y == 0 || unsigned(y >> CUT) < reach) {
-                if (y == 0 && score_of(i, k) != LLONG_MIN) far = 1;
-                break;
-            }
-            const int at = atomicAdd(&count, 1);
-            if (at < BEST_LIST) list[at] = y;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            y[i][j] = key(i, first[i][j]);
+            mine += y[i][j] && unsigned(y[i][j] >> CUT) >= reach;
         }
+    const int upto = wave_scan(mine);
+    int slot = 0;
+    if (lane == 63) slot = upto ? atomicAdd(&count, upto) : 0;
+    slot = __builtin_amdgcn_readlane(slot, 63) + upto - mine;
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i) {
+        bool more = true;                        // a list falls: what follows one that does not reach it does not either
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            more = y[i][j] && unsigned(y[i][j] >> CUT) >= reach;
+            if (more && slot < BEST_LIST) list[slot] = y[i][j];
+            slot += more;
+            if (y[i][j] == 0 && score_of(i, first[i][j]) != LLONG_MIN) far = 1;
+        }
+        for (int j = AHEAD; more && j < n; ++j) {
+            const int2 k = cand[size_t(tid + THREADS * i) * n + j];
+            const u64 z = key(i, k);
+            more = z && unsigned(z >> CUT) >= reach;
+            if (z == 0 && score_of(i, k) != LLONG_MIN) far = 1;
+            if (!more) break;
+            const int to = atomicAdd(&count, 1);
+            if (to < BEST_LIST) list[to] = z;
+        }
+    }
     __syncthreads();
     const bool told = count >= n || !far;        // else some of the n best are among the far ones
     if (told && count <= BEST_LIST) {
-        for (int i = tid; i < max(count, n); i += THREADS) {
-            int rank = i;
-            i64 c = LLONG_MIN;
-            int parent = -1, token = -1;
-            if (i < count) {
-                const u64 y = list[i];
-                rank = 0;
-                for (int j = 0; j < count; ++j) rank += list[j] > y;
-                const int f = (1 << PLACES) - 1 - int(y & ((1 << PLACES) - 1));
-                c = i64(u64(top) - (FAR - (y >> PLACES)));
-                parent = g * B + f / a.b.V;
-                token = f % a.b.V;
-            }
-            if (rank < n) {
-                const size_t to = size_t(g) * n + rank;
-                a.b.out_score[to] = c;
-                a.b.parent[to] = parent;
-                a.b.token[to] = token;
-            }
-        }
+        auto put = [&](int rank, i64 c, int parent, int token) {
+            const size_t to = size_t(g) * n + rank;
+            a.b.out_score[to] = c;
+            a.b.parent[to] = parent;
+            a.b.token[to] = token;
+        };
+        by_rank(list, count, tid >> 4, THREADS / 16, tid & 15, [&](u64 y, int rank) {
+            const int f = (1 << PLACES) - 1 - int(y & ((1 << PLACES) - 1));
+            if (rank < n) put(rank, i64(u64(top) - (FAR - (y >> PLACES))), g * B + f / a.b.V, f % a.b.V);
+        });
+        for (int i = count + tid; i < n; i += THREADS) put(i, LLONG_MIN, -1, -1);
         return;
     }
     i64 c[LISTS];              // the heads of this thread's lists, tid + THREADS i
@@ -359,7 +410,7 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
 
 hipError_t launch_beam_select(hipStream_t st, const BeamArgs& a) {
     const int spans = a.b.groups * a.b.beams * a.spans;
-    // 512 spans 37.9 us a pass with four waves each and 41.0 with one, 2048 20.1 both, 5000 32.2 and 30.3
+    // 512 spans 37.9 us a pass with four waves each and 41.0 with one, 2048 20.1 both, 5000 32.2 and 30.3 (an earlier merge included)
     if (spans >= 2048) beam_span_kernel<1><<<(spans + 3) / 4, 256, 0, st>>>(a);
     else beam_span_kernel<4><<<spans, 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
