@@ -83,10 +83,7 @@ def attend(q, k, ek, v, ev, ok, heads, m, s, L):
         live = mx[Ls > 0]
         if live.size == 0:
             continue
-        if len(mx) == 1:      # the join of one span is its mean
-            out[h] = lm.sat32(As[0])
-            continue
-        G = ((lutexp(np.maximum(live.max() - mx, 0), L) + 64) >> 7) * Ls
+        G = np.maximum((lutexp(np.maximum(live.max() - mx, 0), L) + 64) >> 7, mx == live.max()) * Ls
         down = max(0, int(G.sum()).bit_length() - 30)
         w = (G + ((1 << down) >> 1)) >> down
         T = int(w.sum())

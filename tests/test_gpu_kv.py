@@ -827,3 +827,29 @@ def test_attention_over_two_million_tokens(gpu):
     a.table[1, :2] = pages[:2]
     a.lens, a.width = np.array([n, 300]), a.table.shape[1]
     a.check()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("D", [16, 64, 80, 128, 192, 256])
+@pytest.mark.parametrize("Hq", [2, 10, 24, 40])
+def test_attention_of_few_spans(gpu, bits, D, Hq):
+    """Sequences whose spans one block takes two at a time and joins: every number of them up to four, some without tokens, a team without a span."""
+    rng = np.random.default_rng(D + Hq)
+    a = Attend(rng, [0, 1, 256, 257, 512, 513, 768, 769, 1024, 300], 32, 2, D, bits, Hq, extreme=Hq == 10)
+    a.check(pad=4)
+    a.check(window=300)
+    a.check(window=1)
+    a.check(max_len=400)
+
+
+def test_attention_of_few_spans_that_are_absent(gpu):
+    a = Attend(np.random.default_rng(57), [1000, 1000, 600, 300, 20], 16, 2, 64, 8, 4)
+    a.table[0, 16:32] = -1                      # spans between, first, last and all
+    a.table[1, :16] = a.table[1, 48:] = -1
+    a.table[2, :38] = 1 << 30
+    a.table[3, 16:] = a.cache.c.pages
+    a.check()
+    a.lexp = np.zeros(1025, np.int64)
+    a.check()
+    a.lexp = (np.arange(1025) % 2 * (2**31 - 1)).astype(np.int64)
+    a.check()

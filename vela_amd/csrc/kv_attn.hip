@@ -7,7 +7,8 @@
 //
 // A block of four waves takes a span of one sequence and key head with up to sixteen of its query heads, the columns of the 16x16x64 int8
 // matrix instruction. What bounds it is memory: two sequences of 131072 tokens (8 x 128 heads, 8 bits, 32 query heads) take 111 us, 4.8 TB/s of
-// cache, against 5.0 for a copy; a span alone is a chain of two loads and ~3.5 us of work, 5.8 us for a sequence of 500 tokens (16 x 64, 16 bits).
+// cache, against 5.0 for a copy; a span alone is a chain of two loads and ~3.5 us of work, 5.6 us for a sequence of 500 tokens (16 x 64, 16 bits) without its
+// join.
 //   * Scores: wave w has the positions [64 w, 64 w + 64). The keys are the A operand; row i of subtile ks is position 16 (i / 4) + 4 ks + i % 4, so that
 //     lane (fg, query) ends with the scores of the 16 positions from 16 fg on, in order. Quarters of four tokens
 //     lie together in a page (vgemm_kv.h), so a load touches four runs of 256 bytes.
@@ -92,6 +93,17 @@ constexpr int DEAL_ROWS = 2048;   // sequences whose spans are dealt evenly: eve
 __device__ __forceinline__ int kv_len(const KvAttnArgs& a, int row) { return int(min(i64(max(min(a.len[row], a.max_len), 0)), i64(a.width) << a.c.lp)); }
 __device__ __forceinline__ int kv_first(const KvAttnArgs& a, int n) { return a.window > 0 ? max(0, n - a.window) : 0; }
 
+// G of a span; st.y = 0: none. The greatest has a weight with any table, so that one span alone joins to its own mean.
+__device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st) {
+    const unsigned d = unsigned(mx) - unsigned(st.x);
+    if (st.y == 0 || d >= (1u << 20)) return 0;
+    const i64 t = a.Lexp[d >> 10], t1 = a.Lexp[(d >> 10) + 1];
+    const i64 f = (t + (((t1 - t) * i64(d & 1023)) >> 10) + 64) >> 7;
+    return (d == 0 && f == 0 ? 1 : f) * st.y;
+}
+
+constexpr int SHORT_SPANS = 4;   // that a block of eight waves takes and joins by itself
+
 // the one of F parts of four that a lane takes: x[KT * sub + t], t < KT = 4 / F
 template <int F, class T>
 __device__ __forceinline__ T part_of(const T& x0, const T& x1, const T& x2, const T& x3, int sub, int t) {
@@ -137,18 +149,25 @@ __device__ __forceinline__ void store_words(void* p, const T (&w)[N]) {
 // span for 128 values in 8 bits with F = 1, about 450 with 4; four queries a key, 32 x 8192 tokens of 64 values 82 -> 73 us, of 128 89 % of the time.
 // chunks > 0: blocks take runs of spans of one sequence and key head, as even as the lengths allow, so that there are about `chunks` runs
 // a head over all sequences; every block counts them from the lengths. chunks = 0: a block has one span, or each gridDim.z-th.
-template <int NS, int PL, bool EXACT, int F>
-__global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAttnArgs a, int chunks) {
+// SHORT: a block of eight waves takes a sequence of at most SHORT_SPANS spans, two at a time, each by four waves as elsewhere, and joins them itself.
+template <int NS, int PL, bool EXACT, int F, bool SHORT>
+__global__ void __launch_bounds__(SHORT ? 512 : 256, SHORT ? 2 : kv_held(64 * NS, PL)) kv_attn_kernel(KvAttnArgs a, int chunks) {
     constexpr int QT = 16 / F, KT = 4 / F, NK = 16 / F, JN = 4 / F;   // queries; a lane's subtiles, keys, and dimensions of four
     constexpr bool EARLY = NS * PL <= 4;       // values asked for beside the keys, and the next span's keys during the softmax: 32 NS PL registers for both
-    __shared__ __attribute__((aligned(16))) Lds s;
-    __shared__ __attribute__((aligned(16))) int8_t qs[2][16][64 * NS + 16];
+    constexpr int TEAMS = SHORT ? 2 : 1;       // of four waves
+    __shared__ __attribute__((aligned(16))) Lds s_of[TEAMS];
+    __shared__ __attribute__((aligned(16))) int8_t qs_of[TEAMS][2][16][64 * NS + 16];
+    __shared__ __attribute__((aligned(16))) int means[SHORT ? SHORT_SPANS : 1][SHORT ? 16 : 1][SHORT ? 64 * NS : 4];
+    __shared__ int2 stats[SHORT ? SHORT_SPANS : 1][SHORT ? 16 : 1];
     touch_args<int(sizeof(KvAttnArgs) + 4)>();
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
+    const int team = SHORT ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+    Lds& s = s_of[team];
+    auto& qs = qs_of[team];
+    const int tid = SHORT ? threadIdx.x & 255 : threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fg = lane >> 4;
     const int qi = fr & (QT - 1), sub = fr / QT;   // the lane's query, and which part of it
-    const bool deal = chunks > 0;
+    const bool deal = !SHORT && chunks > 0;
     const int head = blockIdx.x / a.qtiles, q0 = (blockIdx.x % a.qtiles) * 16, nq = min(16, a.group - q0);   // key head, its first query head here and their number
-    int row = blockIdx.y, chunk = blockIdx.z, split = gridDim.z;
+    int row = blockIdx.y, chunk = SHORT ? team : blockIdx.z, split = SHORT ? TEAMS : gridDim.z;
     auto zero_row = [&](int r) {               // a sequence without tokens
         for (int i = tid; i < nq * (EXACT ? 64 * NS : a.c.D); i += 256) a.out[size_t(r) * a.ldo + size_t(head * a.group + q0) * (EXACT ? 64 * NS : a.c.D) + i] = 0;
     };
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
     // dealt: spans [u, u_end), one after the other; else u, u + split, ...
     int u = deal ? u0 + (u1 - u0) * chunk / split : u0 + chunk;   // at most 2^15 spans: the products stay below 2^30
     const int u_end = deal ? u0 + (u1 - u0) * (chunk + 1) / split : u1, step = deal ? 1 : split;
-    if (u >= u_end) return;
+    if (SHORT ? n == 0 : u >= u_end) return;   // SHORT: a team without a span left goes along, with nothing that counts
     if (deal || a.window) page = fetch(u);
 
     constexpr int KS = EARLY ? 4 : 2;          // subtiles of keys in registers
@@ -538,17 +557,22 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
         unsigned big = 0;
         if (qi < nq) {
             const size_t at = (size_t(row) * a.Hq + qh) * a.spans + u;
-            if (!only && wave == 0 && fg == 0 && sub == 0) a.stat[at] = make_int2(mx, sum);
+            if (!only && wave == 0 && fg == 0 && sub == 0 && !SHORT) a.stat[at] = make_int2(mx, sum);
             int32_t* y = (only ? a.out + size_t(row) * a.ldo + size_t(qh) * D : a.part + at * D) + 16 * wave + 4 * fg + JN * sub;
+            if (SHORT) {
+                y = &means[min(u - u0, SHORT_SPANS - 1)][qi][16 * wave + 4 * fg + JN * sub];
+                if (u < u1 && wave == 0 && fg == 0 && sub == 0) stats[u - u0][qi] = make_int2(mx, sum);
+            }
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 if (!EXACT && wave + 4 * i >= pieces) break;
+                if (SHORT && u >= u1) break;
 #pragma unroll
                 for (int j = 0; j < JN; ++j) big = max(big, uabs(r[i][j]));
                 store_words(y + 64 * i, r[i]);
             }
         }
-        if (only && a.rowmax) {                // one atomic a block; its only span
+        if (!SHORT && only && a.rowmax) {      // one atomic a block; its only span
             big = unsigned(wave_max(int(big ^ 0x80000000u))) ^ 0x80000000u;
             if (lane == 0) s.big[wave] = big;
             lds_barrier();
@@ -556,7 +580,7 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
             if (tid == 0 && big) atomicMax(a.rowmax + row, big);
         }
         u = un;
-        if (u >= u_end) return;
+        if (SHORT ? u - team >= u1 : u >= u_end) break;
         if (EARLY) {
             page = pagen;
         } else {
@@ -565,17 +589,57 @@ __global__ void __launch_bounds__(256, kv_held(64 * NS, PL)) kv_attn_kernel(KvAt
             load_keys(page, u);
         }
     }
+    if constexpr (SHORT) {
+        __syncthreads();
+        const int count = u1 - u0;
+        unsigned big = 0;
+        for (int i = threadIdx.x; i < nq * (D >> 2); i += 512) {   // four dimensions of a query head
+            const int q = i / (D >> 2), d = 4 * (i % (D >> 2));
+            int mx = INT_MIN;
+#pragma unroll
+            for (int k = 0; k < SHORT_SPANS; ++k)
+                if (k < count && stats[k][q].y) mx = max(mx, stats[k][q].x);
+            i64 G[SHORT_SPANS], all = 0;
+#pragma unroll
+            for (int k = 0; k < SHORT_SPANS; ++k) {
+                G[k] = k < count ? join_weight(a, mx, stats[k][q]) : 0;
+                all += G[k];
+            }
+            const int h = max(0, 64 - __clzll((long long)all) - 30);
+            const i64 half = (i64(1) << h) >> 1;
+            i64 x[4] = {0, 0, 0, 0}, T = 0;
+#pragma unroll
+            for (int k = 0; k < SHORT_SPANS; ++k) {
+                if (k >= count) break;
+                const int w = int((G[k] + half) >> h);
+                const int4 v = *reinterpret_cast<const int4*>(&means[k][q][d]);
+                x[0] += i64(w) * v.x;
+                x[1] += i64(w) * v.y;
+                x[2] += i64(w) * v.z;
+                x[3] += i64(w) * v.w;
+                T += w;
+            }
+            const double inv = recip(double(max(T, i64(1))));
+            int r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                r[j] = T ? div_sat(x[j] + (T >> 1), T, inv) : 0;
+                big = max(big, uabs(r[j]));
+            }
+            store_words(a.out + size_t(row) * a.ldo + size_t(head * a.group + q0 + q) * D + d, r);
+        }
+        if (!a.rowmax) return;
+        big = unsigned(wave_max(int(big ^ 0x80000000u))) ^ 0x80000000u;
+        if (lane == 0) s.big[wave] = big;
+        __syncthreads();
+        if (threadIdx.x) return;
+        for (int t = 0; t < TEAMS; ++t)
+            for (int w = 0; w < 4; ++w) big = max(big, s_of[t].big[w]);
+        if (big) atomicMax(a.rowmax + row, big);
+    }
 }
 
 // ---------------------------------------------------------------- the join
-
-// G of a span; st.y = 0: none
-__device__ __forceinline__ i64 join_weight(const KvAttnArgs& a, int mx, int2 st) {
-    const unsigned d = unsigned(mx) - unsigned(st.x);
-    if (st.y == 0 || d >= (1u << 20)) return 0;
-    const i64 t = a.Lexp[d >> 10], t1 = a.Lexp[(d >> 10) + 1];
-    return ((t + (((t1 - t) * i64(d & 1023)) >> 10) + 64) >> 7) * st.y;
-}
 
 constexpr int JOIN_ONE = 64;       // spans that one wave joins, a lane each for their weights: 8 spans 13.0 us a pass so and 19.2 with eight waves, 64 of 32 sequences 242 and 244
 constexpr int JOIN_WAVES = 8;      // waves of a query head where there are more
@@ -711,13 +775,25 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
     }
 }
 
+constexpr bool kv_short(int D, int planes) { return (D + 63) / 64 * planes <= 4; }   // eight waves' registers are there
+
+template <int NS, int PL, bool EXACT, int F>
+void launch_form(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
+    if constexpr (kv_short(64 * NS, PL)) {
+        if (chunks < 0) {
+            kv_attn_kernel<NS, PL, EXACT, F, true><<<g, 512, 0, st>>>(a, 0);
+            return;
+        }
+    }
+    kv_attn_kernel<NS, PL, EXACT, F, false><<<g, 256, 0, st>>>(a, chunks);
+}
 template <int PL, bool EXACT, int F>
 void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     switch ((a.c.D + 63) / 64) {
-        case 1: kv_attn_kernel<1, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
-        case 2: kv_attn_kernel<2, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
-        case 3: kv_attn_kernel<3, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks); break;
-        default: kv_attn_kernel<4, PL, EXACT, F><<<g, 256, 0, st>>>(a, chunks);
+        case 1: launch_form<1, PL, EXACT, F>(st, a, g, chunks); break;
+        case 2: launch_form<2, PL, EXACT, F>(st, a, g, chunks); break;
+        case 3: launch_form<3, PL, EXACT, F>(st, a, g, chunks); break;
+        default: launch_form<4, PL, EXACT, F>(st, a, g, chunks);
     }
 }
 template <int F>
@@ -726,6 +802,7 @@ void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     if (a.c.planes == 1) exact ? launch_spans<1, true, F>(st, a, g, chunks) : launch_spans<1, false, F>(st, a, g, chunks);
     else exact ? launch_spans<2, true, F>(st, a, g, chunks) : launch_spans<2, false, F>(st, a, g, chunks);
 }
+// chunks: the kernel's; -1: SHORT
 void launch_spans(hipStream_t st, const KvAttnArgs& a, dim3 g, int chunks) {
     if (a.group <= 4) launch_spans<4>(st, a, g, chunks);
     else if (a.group <= 8) launch_spans<2>(st, a, g, chunks);
@@ -738,6 +815,12 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     const int heads = a.c.heads * a.qtiles;
     const int spans = a.window > 0 ? std::min(a.spans, a.window / KV_SPAN + 2) : a.spans;   // that a sequence may have
     const int held = 256 * kv_held(a.c.D, a.c.planes);   // blocks the card holds at a time
+    // Few spans a sequence, and a CU for each sequence and head: one launch (500 tokens of 16 heads 9.4 us a pass, 13 with the join's launch; 32 x 1000 of 8 heads
+    // 17.5 and 21.1). With twice as many, sequences of unequal length wait for the longest twice (64 ragged ones up to 1000: 21.9 and 16.3).
+    if (spans > 1 && spans <= SHORT_SPANS && kv_short(a.c.D, a.c.planes) && i64(heads) * a.rows <= 256) {
+        launch_spans(st, a, dim3(heads, a.rows), -1);
+        return hipGetLastError();
+    }
     if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * spans > 2 * held) {
         // Blocks with more than two spans each take them as dealt (32 x 4096 tokens 80.6 us a pass, 85.7 with a block a span; 16 x 2000, 1.3 spans a block,
         // 29.3 and 28.0). Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
