@@ -159,51 +159,59 @@ __global__ void __launch_bounds__(256, 8) kv_write_kernel(KvView c, const int32_
     __shared__ Turn turn;
     __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
     const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;
-    const bool value = blockIdx.z;
     const Place p = place_of(c, t < M ? slots[t] : -1);
-    const int32_t* x = (value ? V : K) + size_t(p.there ? t : 0) * ld + head * c.D;
-    int4 v[4];
-    unsigned m = 0;
+    const size_t from = size_t(p.there ? t : 0) * ld + head * c.D;
+    // RUNS: keys and values by one block, all their rows asked for at once; else by two
+    constexpr int BOTH = RUNS ? 2 : 1;
+    int4 v[BOTH][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = 4 * l + 64 * i;
-        v[i] = p.there && d < c.D ? *reinterpret_cast<const int4*>(x + d) : make_int4(0, 0, 0, 0);
-        m = max(max(m, max(uabs(v[i].x), uabs(v[i].y))), max(uabs(v[i].z), uabs(v[i].w)));
-    }
-    if (RUNS && value) {
+    for (int b = 0; b < BOTH; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 4 * l + 64 * i;
+            const int32_t* x = ((RUNS ? b : int(blockIdx.z)) ? V : K) + from;
+            v[b][i] = p.there && d < c.D ? *reinterpret_cast<const int4*>(x + d) : make_int4(0, 0, 0, 0);
+        }
+    if (RUNS) {
         turn_init(turn, c, slots, M);
         __syncthreads();
     }
-    m = row_max(m);
     constexpr int BITS = 8 * PL - 1, TOP = (1 << BITS) - 1;
-    const int e = max(0, 32 - __clz(int(m)) - BITS);   // __clz(0) is 32
-    if (l == 0 && p.there) c.shifts(p.page, head)[(int(value) << c.lp) + p.at] = uint8_t(e);
     int8_t* keys = c.keys(p.page, head) + (p.at >> 4) * c.group_bytes();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = 4 * l + 64 * i;
-        if (d >= c.D) break;
-        int q[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int b = 0; b < BOTH; ++b) {
+        const bool value = RUNS ? b : blockIdx.z;
+        unsigned m = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = min(max(e ? (q[j] >> e) + ((q[j] >> (e - 1)) & 1) : q[j], -TOP), TOP);
+        for (int i = 0; i < 4; ++i) m = max(max(m, max(uabs(v[b][i].x), uabs(v[b][i].y))), max(uabs(v[b][i].z), uabs(v[b][i].w)));
+        const int e = max(0, 32 - __clz(int(row_max(m))) - BITS);   // __clz(0) is 32
+        if (l == 0 && p.there) c.shifts(p.page, head)[(int(value) << c.lp) + p.at] = uint8_t(e);
 #pragma unroll
-        for (int n = 0; n < PL; ++n) {
-            char4 b;
-            int8_t* bb = reinterpret_cast<int8_t*>(&b);
+        for (int i = 0; i < 4; ++i) {
+            const int d = 4 * l + 64 * i;
+            if (d >= c.D) break;
+            int q[4] = {v[b][i].x, v[b][i].y, v[b][i].z, v[b][i].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bb[j] = int8_t(PL == 1 ? q[j] : n == 0 ? q[j] >> 8 : (q[j] & 255) - 128);
-            if (RUNS && value) {
+            for (int j = 0; j < 4; ++j) q[j] = min(max(e ? (q[j] >> e) + ((q[j] >> (e - 1)) & 1) : q[j], -TOP), TOP);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) vt[(n * c.D + d + j) * TURN + t16 + turn.off] = bb[j];
-            } else if (p.there && value) {
+            for (int n = 0; n < PL; ++n) {
+                char4 y;
+                int8_t* bb = reinterpret_cast<int8_t*>(&y);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d + j)] = bb[j];
-            } else if (p.there) {
-                *reinterpret_cast<char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d)) = b;
+                for (int j = 0; j < 4; ++j) bb[j] = int8_t(PL == 1 ? q[j] : n == 0 ? q[j] >> 8 : (q[j] & 255) - 128);
+                if (RUNS && value) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vt[(n * c.D + d + j) * TURN + t16 + turn.off] = bb[j];
+                } else if (p.there && value) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d + j)] = bb[j];
+                } else if (p.there) {
+                    *reinterpret_cast<char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d)) = y;
+                }
             }
         }
     }
-    if (!RUNS || !value) return;
+    if (!RUNS) return;
     __syncthreads();
     const int words = turn.off ? 5 : 4;
     for (int w = tid & 3; w < words; w += 4) {
@@ -331,8 +339,8 @@ hipError_t launch_kv_plan(hipStream_t st, const VgemmKvPlan& p, int lp) {
 constexpr int RUNS_FROM = 4096;   // tokens times planes
 
 hipError_t launch_kv_write(hipStream_t st, const KvView& c, const int32_t* K, const int32_t* V, int ld, const int32_t* slot, int M) {
-    const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, 2);
     const bool runs = M >= RUNS_FROM / c.planes;
+    const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, runs ? 1 : 2);
     if (c.planes == 1) runs ? kv_write_kernel<1, true><<<g, 256, 0, st>>>(c, K, V, ld, slot, M) : kv_write_kernel<1, false><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
     else runs ? kv_write_kernel<2, true><<<g, 256, 0, st>>>(c, K, V, ld, slot, M) : kv_write_kernel<2, false><<<g, 256, 0, st>>>(c, K, V, ld, slot, M);
     return hipGetLastError();
