@@ -92,6 +92,21 @@ def test_plan_with_fewer_rows_than_tokens(gpu, rows):
     check_plan(length, add, table, free, pages, 16, width, rows)
 
 
+def test_plan_of_the_most_rows(gpu):
+    """2^31 - 1 of them: the rows behind the tokens get -1 by all blocks."""
+    tokens, length, add = (1 << 31) - 1, [3, 20], [40, 7]
+    table, free = np.array([[5, -1, -1], [2, 0, -1]], np.int32), np.array([1, 7, 3], np.int32)
+    d = [dev(np.asarray(v, np.int32)) for v in (length, add, table, free, [3])]
+    slot = full(tokens + 1)
+    P = vk.KvPlan(R=2, tokens=tokens, pages=8, page=16, width=3, ldt=3, len=vg.ptr(d[0]), add=vg.ptr(d[1]), table=vg.ptr(d[2]), free=vg.ptr(d[3]), nfree=vg.ptr(d[4]),
+                  slot=vg.ptr(slot))
+    vk.k_kv_plan(P)
+    want = km.plan(length, add, table, free, 8, 16, 3, 50)
+    assert_equal(to_np(d[2]), want[0])
+    assert_equal(to_np(slot[:50]), want[3])
+    assert int(slot[50:tokens].amax()) == int(slot[50:tokens].amin()) == -1 and int(slot[tokens]) == JUNK
+
+
 @pytest.mark.parametrize("nfree", [0, 1, 5, -4])
 def test_plan_past_the_free_list(gpu, nfree):
     length, add, table, free, pages, width = random_plan(np.random.default_rng(5), 12, 70, 90, 16)

@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) beam_tables_kernel(VgemmBeamTables t, int
 
 hipError_t launch_kv_plan(hipStream_t st, const VgemmKvPlan& p, int lp) {
     // 256 token rows a block, or 1024 new pages where the rows are few; block 0 alone where there are none
-    const int blocks = std::max(1, std::min((p.tokens + 255) / 256, 1024));
+    const int blocks = std::max(1, std::min(int((int64_t(p.tokens) + 255) / 256), 1024));
     kv_plan_kernel<<<blocks, 256, size_t(p.R) * 8, st>>>(p, lp);
     return hipGetLastError();
 }
