@@ -76,10 +76,10 @@ int vgemm_kv_copy(void* stream, const VgemmKv* C, const int32_t* src, const int3
  *   s_j = rshr(m sum_d q_d k_jd, s - eq - ek_j)                         1 <= m <= 32768, -64 <= s <= 128
  * Tokens go in spans of 256 positions, [256 u, 256 u + 256). In a span, over the tokens that count:
  *   mx_u = max s_j; P_j = min(32767, rshr(lutexp(mx_u - s_j), 15)); L_u = sum P_j
- *   A_u = floor((sum P_j v_j 2^ev_j + floor(L_u / 2)) / L_u), 0 where L_u = 0
+ *   A_u = sat32(floor((sum P_j v_j 2^ev_j + floor(L_u / 2)) / L_u)), 0 where L_u = 0
  * and over the spans with L_u > 0:
  *   mx = max mx_u; G_u = rshr(lutexp(mx - mx_u), 7) L_u, at least L_u where mx_u = mx; h = the least shift >= 0 with sum G_u < 2^(30 + h); g_u = floor(G_u / 2^h + 1/2)
- *   out = floor((sum g_u A_u + floor(T / 2)) / T), T = sum g_u; 0 where no token counts.
+ *   out = sat32(floor((sum g_u A_u + floor(T / 2)) / T)), T = sum g_u; 0 where no token counts.
  * out [rows x ldo]; rowmax[r] = max(rowmax[r], max |out|) if not NULL. Q and out 16-byte aligned, ldq % 4 == ldo % 4 == 0. rows <= 65535, 0 <= max_len <= 2^23,
  * Hq <= 4096. ws: vgemm_kv_attention_workspace_bytes(), 16-byte aligned, of any content (none up to 256 tokens); calls, or replays of captured ones, that share one must not run at the
  * same time. */
