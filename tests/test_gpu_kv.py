@@ -815,6 +815,28 @@ def test_rows_of_prompts(gpu, bits, D, M):
         assert_equal(to_np(o), np.where(there[:, None], lm.sat32(q << e[..., None]).reshape(M, -1), 0))
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("M", [70, 4200])
+def test_rows_read_alone(gpu, bits, M):
+    """Keys without values and values without keys, of few and of many tokens; the other output and what lies between the rows stay."""
+    rng = np.random.default_rng(M)
+    page, heads, D, pad = 64, 3, 80, 12
+    pages = M // page + 2
+    slot = rng.permutation(pages * page)[:M].astype(np.int32)
+    slot[50:] = np.sort(slot[50:])
+    slot[::17] = -1
+    k, v = (rows_of(rng, M, heads, D).reshape(M, -1) for _ in range(2))
+    C, ds = Cache(pages, page, heads, D, bits), dev(slot)
+    vk.k_kv_write(C.c, dev(k), dev(v), heads * D, ds, M)
+    for x, i in ((k, 0), (v, 1)):
+        o = full((M, heads * D + pad))
+        vk.k_kv_read(C.c, ds, M, o if i == 0 else None, None if i == 0 else o, heads * D + pad)
+        q, e = km.quant(x.reshape(M, heads, D), bits)
+        want = np.full((M, heads * D + pad), JUNK, np.int64)
+        want[:, :heads * D] = np.where((slot >= 0)[:, None], lm.sat32(q << e[..., None]).reshape(M, -1), 0)
+        assert_equal(to_np(o), want)
+
+
 def test_shared_pages(gpu):
     """The same pages in the tables of several sequences, twice in one table, and the same slot read many times."""
     a = Attend(np.random.default_rng(55), [300, 300, 64, 300], 16, 2, 64, 8, 4)

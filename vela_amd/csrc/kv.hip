@@ -232,15 +232,25 @@ __global__ void __launch_bounds__(256, 8) kv_write_kernel(KvView c, const int32_
     }
 }
 
+// With RUNS a block reads keys and values where both are asked for (as the write does), the keys' words on their way while the values are turned over.
 template <int PL, bool RUNS>
 __global__ void __launch_bounds__(256, 8) kv_read_kernel(KvView c, const int32_t* slots, int M, int32_t* K, int32_t* V, int ld) {
     __shared__ Turn turn;
     __shared__ __attribute__((aligned(16))) int8_t vt[RUNS ? PL * 256 * TURN : 16];
     const int tid = threadIdx.x, l = tid & 15, t16 = tid >> 4, t = int(blockIdx.x) * KV_TOKENS + t16, head = blockIdx.y;
-    const bool value = K ? blockIdx.z : true;
+    const bool key = RUNS ? K != nullptr : K && !blockIdx.z, value = RUNS ? V != nullptr : !key;
     const Place p = place_of(c, t < M ? slots[t] : -1);
-    const int e = p.there ? min(int(c.shifts(p.page, head)[(int(value) << c.lp) + p.at]), 31) : 0;
+    const uint8_t* sh = c.shifts(p.page, head) + p.at;
+    const int ek = min(int(sh[0]), 31), ev = min(int(sh[1 << c.lp]), 31);
     const int8_t* keys = c.keys(p.page, head) + (p.at >> 4) * c.group_bytes();
+    char4 k[4][PL];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < PL; ++n) {
+            const int d = 4 * l + 64 * i;
+            k[i][n] = key && p.there && d < c.D ? *reinterpret_cast<const char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d)) : char4{0, 0, 0, 0};
+        }
     if (RUNS && value) {
         turn_init(turn, c, slots, M);
         __syncthreads();
@@ -261,37 +271,32 @@ __global__ void __launch_bounds__(256, 8) kv_read_kernel(KvView c, const int32_t
                 }
             }
         }
-        __syncthreads();
     }
-    if (t >= M) return;
-    int32_t* y = (value ? V : K) + size_t(t) * ld + head * c.D;
+    auto put = [&](int32_t* rows, int e, auto byte) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = 4 * l + 64 * i;
-        if (d >= c.D) break;
-        int q[4] = {0, 0, 0, 0};
-        if (p.there) {
+        for (int i = 0; i < 4; ++i) {
+            const int d = 4 * l + 64 * i;
+            if (d >= c.D) break;
+            int q[4] = {0, 0, 0, 0};
+            if (p.there) {
 #pragma unroll
-            for (int n = 0; n < PL; ++n) {
-                char4 b;
-                int8_t* bb = reinterpret_cast<int8_t*>(&b);
-                if (RUNS && value) {
+                for (int n = 0; n < PL; ++n)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) bb[j] = vt[(n * c.D + d + j) * TURN + t16 + turn.off];
-                } else if (value) {
+                    for (int j = 0; j < 4; ++j) q[j] = n == 0 ? byte(i, n, j) : 256 * q[j] + byte(i, n, j) + 128;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) bb[j] = keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d + j)];
-                } else {
-                    b = *reinterpret_cast<const char4*>(keys + n * 16 * c.D + c.key_at(p.at & 15, d));
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) q[j] = n == 0 ? bb[j] : 256 * q[j] + bb[j] + 128;
+                for (int j = 0; j < 4; ++j) q[j] = int(sat32(i64(q[j]) << e));
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = int(sat32(i64(q[j]) << e));
+            *reinterpret_cast<int4*>(rows + size_t(t) * ld + head * c.D + d) = make_int4(q[0], q[1], q[2], q[3]);
         }
-        *reinterpret_cast<int4*>(y + d) = make_int4(q[0], q[1], q[2], q[3]);
-    }
+    };
+    if (key && t < M) put(K, ek, [&](int i, int n, int j) { return int(reinterpret_cast<const int8_t*>(&k[i][n])[j]); });
+    if (!value) return;
+    if (RUNS) __syncthreads();
+    if (t >= M) return;
+    put(V, ev, [&](int i, int n, int j) {
+        const int d = 4 * l + 64 * i + j;
+        return int(RUNS ? vt[(n * c.D + d) * TURN + t16 + turn.off] : keys[c.half_bytes() + n * 16 * c.D + c.value_at(p.at & 15, d)]);
+    });
 }
 
 // ---------------------------------------------------------------- pages and tables by parent
@@ -335,8 +340,9 @@ hipError_t launch_kv_plan(hipStream_t st, const VgemmKvPlan& p, int lp) {
 }
 
 // Few tokens are mostly a decode step's, each in a page of its own: their bytes go one by one, without LDS and its two barriers. Written and read back, 8
-// heads x 128: 24 tokens apart 9.3 us so and 10.1 turned over, 1000 in a row 11.4 and 12.3 (8 bits), 4000 in a row 28.2 and 25.1 (8 bits), 5000 55 and 37 (16 bits).
-constexpr int RUNS_FROM = 4096;   // tokens times planes
+// heads x 128: 24 tokens apart 10.4 us so and 10.9 turned over (the host's time for two calls); in a row, 8 bits, 1000 11.3 and 12.5, 2000 16.6 and 16.4, 4000 27.5 and 22.8; 16 bits,
+// 1000 15.1 and 13.7, 5000 55 and 33.
+constexpr int RUNS_FROM = 2048;   // tokens times planes
 
 hipError_t launch_kv_write(hipStream_t st, const KvView& c, const int32_t* K, const int32_t* V, int ld, const int32_t* slot, int M) {
     const bool runs = M >= RUNS_FROM / c.planes;
@@ -347,8 +353,8 @@ hipError_t launch_kv_write(hipStream_t st, const KvView& c, const int32_t* K, co
 }
 
 hipError_t launch_kv_read(hipStream_t st, const KvView& c, const int32_t* slot, int M, int32_t* K, int32_t* V, int ld) {
-    const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, K && V ? 2 : 1);
     const bool runs = M >= RUNS_FROM / c.planes;
+    const dim3 g((M + KV_TOKENS - 1) / KV_TOKENS, c.heads, K && V && !runs ? 2 : 1);
     if (c.planes == 1) runs ? kv_read_kernel<1, true><<<g, 256, 0, st>>>(c, slot, M, K, V, ld) : kv_read_kernel<1, false><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
     else runs ? kv_read_kernel<2, true><<<g, 256, 0, st>>>(c, slot, M, K, V, ld) : kv_read_kernel<2, false><<<g, 256, 0, st>>>(c, slot, M, K, V, ld);
     return hipGetLastError();
