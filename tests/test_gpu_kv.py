@@ -890,3 +890,33 @@ def test_attention_of_few_spans_that_are_absent(gpu):
     a.check()
     a.lexp = (np.arange(1025) % 2 * (2**31 - 1)).astype(np.int64)
     a.check()
+
+
+class Turns(Attend):
+    """Sequences of any length over a few filled pages, whose tables name them in turn."""
+
+    def __init__(self, rng, lens, D, bits, Hq, filled=80):
+        super().__init__(rng, [16 * filled], 16, 1, D, bits, Hq)
+        self.lens = np.asarray(lens)
+        pages = self.table[0, :filled].copy()
+        self.width = -(-int(self.lens.max()) // 16)
+        self.table = rng.choice(pages, (len(lens), self.width)).astype(np.int32)
+        self.q = rows_of(rng, len(lens), Hq, D)
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 128, 144, 256])
+@pytest.mark.parametrize("window", [0, 4400])
+def test_attention_joins_every_number_of_spans(gpu, D, window):
+    """From two spans a sequence up to the 64 that a wave joins, each with a ragged last one: the weight of every span reaches every lane."""
+    rng = np.random.default_rng(D + window)
+    lens = 256 * np.arange(1, 64) + rng.integers(1, 257, 63)
+    a = Turns(rng, lens, D, 8 if D % 32 else 16, 2)
+    a.check(window=window, max_len=16384)
+    if window:
+        a.check(window=window, max_len=40000)   # a workspace of more spans than the window has
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 128])
+@pytest.mark.parametrize("n", [2049, 2400, 4097, 4352, 4353, 7200, 7425, 9000, 16384])
+def test_attention_joins_one_sequence(gpu, D, n):
+    Turns(np.random.default_rng(n), [n], D, 8, 6).check(max_len=16384)

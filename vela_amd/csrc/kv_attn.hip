@@ -685,7 +685,10 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) kv_join_kernel(
         const int g = int((G + ((i64(1) << h) >> 1)) >> h);   // 0 in the lanes behind the last span
         T = wave_sum64(g);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) add(sub + i * groups < count ? __shfl(g, sub + i * groups) : 0, v[i]);
+        for (int i = 0; i < AHEAD; ++i) {      // every lane takes part: what a lane that is switched off holds reads as 0
+            const int k = sub + i * groups, w = __shfl(g, k & 63);
+            add(k < count ? w : 0, v[i]);
+        }
         for (int k = sub + AHEAD * groups; k - sub < count; k += groups) {
             const int w = __shfl(g, k);        // k < 64: count <= JOIN_ONE, and groups divides it
             add(w, *reinterpret_cast<const int4*>(part + size_t(min(k, count - 1)) * D));
