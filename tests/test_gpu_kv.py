@@ -920,3 +920,26 @@ def test_attention_joins_every_number_of_spans(gpu, D, window):
 @pytest.mark.parametrize("n", [2049, 2400, 4097, 4352, 4353, 7200, 7425, 9000, 16384])
 def test_attention_joins_one_sequence(gpu, D, n):
     Turns(np.random.default_rng(n), [n], D, 8, 6).check(max_len=16384)
+
+
+@pytest.mark.parametrize("below", [1, 2, 100, 254, 255, 256, 257, 258, 1000])
+@pytest.mark.parametrize("beams,n", [(2, 2), (2, 1), (5, 5), (32, 40), (3, 64)])
+def test_select_of_scores_at_the_end_of_the_keys(gpu, below, beams, n):
+    """One token a beam, the first beam's score 2^40 - below above the others', and below their neighbours': those that a key can hold and those that it cannot."""
+    z = np.zeros((2 * beams, 1), np.int32)
+    s = np.zeros((2, beams), np.int64)
+    s[0, 1:] = below - (1 << 40)
+    s[1, 1:] = below - (1 << 40) + np.arange(beams - 1) * 100 - 200
+    check_select(z, s.reshape(-1), 2, beams, n)
+
+
+@pytest.mark.parametrize("V,n", [(3, 6), (4, 8), (40, 64), (9000, 64)])
+def test_select_of_lists_across_the_end_of_the_keys(gpu, V, n):
+    """Lists whose entries lie on both sides of what a key holds, behind ones that no key holds, with banned tokens so that all of them are asked for."""
+    rng = np.random.default_rng(V)
+    z = np.full((4, V), km.LOW, np.int32)
+    for r in range(4):
+        at = rng.permutation(V)[:min(V, 20)]
+        z[r, at] = -20 * rng.integers(0, 20, at.size)
+    for below in (100, 300, 500):
+        check_select(z, np.array([0, below - (1 << 40), 0, below - (1 << 40) - 7], np.int64), 2, 2, n)

@@ -232,14 +232,15 @@ __global__ void __launch_bounds__(256, WAVES == 1 ? 5 : 4) beam_span_kernel(Beam
 struct Best { i64 c; int at; };   // score and list: lower lists first among equal scores
 __device__ __forceinline__ bool before(const Best& x, const Best& y) { return x.c > y.c || (x.c == y.c && x.at < y.at); }
 
-constexpr int NEAR = 40;      // bits of a score below the group's best one that a key holds
+constexpr int NEAR = 40;      // bits of a score below the group's best one in a key
 constexpr int PLACES = 23;    // bits of beam * V + token
-constexpr u64 FAR = (u64(1) << NEAR) - 1;
+constexpr int CUT = NEAR + PLACES - 32;   // a key's upper 32 bits are what thresholds compare: at least 1 in every key that holds something
+constexpr u64 FAR = (u64(1) << NEAR) - 1, HELD = FAR - (u64(1) << (CUT - PLACES));   // distances above HELD are too far for a key
 constexpr int BEST_LIST = 1024;
 
 // One group: logZ of its beams, a wave a beam, then the best of its spans' lists, each in falling order: a thread a list or two, by a threshold as
 // above over keys of a score's distance from the best one and its place, which the lists' heads give and down to which each list is
-// walked. Where the keys do not tell (scores 2^40 apart, or too many that reach the threshold) the lists are merged n times
+// walked. Where the keys do not tell (scores about 2^40 apart, or too many that reach the threshold) the lists are merged n times
 // by the best of their heads.
 template <int THREADS, int LISTS>
 __global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
@@ -294,12 +295,11 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
     auto key = [&](int i, int2 k) {              // 0: none, or too far below the best
         const i64 c = score_of(i, k);
         const u64 d = u64(top) - u64(c);
-        return c == LLONG_MIN || d >= FAR ? u64(0) : ((FAR - d) << PLACES) | u64((1 << PLACES) - 1 - (f0[i] + k.y));
+        return c == LLONG_MIN || d > HELD ? u64(0) : ((FAR - d) << PLACES) | u64((1 << PLACES) - 1 - (f0[i] + k.y));
     };
     u64 best = 0;
 #pragma unroll
     for (int i = 0; i < LISTS; ++i) best = max(best, key(i, first[i][0]));
-    constexpr int CUT = NEAR + PLACES - 32;
     const unsigned reach_own = reached_by(unsigned(best >> CUT), n, 1u << (20 - (CUT - PLACES)), 1u << (10 - (CUT - PLACES)));   // scores 2^20 below the best, by steps of 2^10
     if (lane == 0) reach_of[wave] = reach_own;
     __syncthreads();
