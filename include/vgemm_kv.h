@@ -119,7 +119,9 @@ int vgemm_beam_select(void* stream, const VgemmBeam* B);
 
 /* Row r continues row parent[r]: n = len[parent[r]] (below 0: 0, at most width * page); out_len[r] = n; out_table[r, j] = table[parent[r], j] for the
  * whole pages j < n / page; a partly filled last page becomes fresh[r], with the pair (src[r], dst[r]) = (its page, fresh[r]) for vgemm_kv_copy, else
- * (-1, -1); the entries behind are -1. parent[r] outside [0, rows): n = 0. Tables [rows x ldt], width <= ldt. rows <= 65535, page as in VgemmKv. */
+ * (-1, -1); one that is no page (an entry below 0, as vgemm_kv_plan writes where its list has ended) becomes -1, without a pair: its tokens do not count
+ * afterwards either. Last pages' entries from 0 on are pages of the cache. The entries behind are -1. parent[r] outside [0, rows): n = 0.
+ * Tables [rows x ldt], width <= ldt. rows <= 65535, page as in VgemmKv. */
 typedef struct VgemmBeamTables {
     int rows, page, width, ldt;
     const int32_t *parent, *len, *table, *fresh;

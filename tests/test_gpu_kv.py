@@ -943,3 +943,46 @@ def test_select_of_lists_across_the_end_of_the_keys(gpu, V, n):
         z[r, at] = -20 * rng.integers(0, 20, at.size)
     for below in (100, 300, 500):
         check_select(z, np.array([0, below - (1 << 40), 0, below - (1 << 40) - 7], np.int64), 2, 2, n)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_tables_by_parent_of_absent_pages(gpu, page):
+    """A partly filled last page that is none (a plan's list had ended) stays none: a fresh page in its place would hold nothing that was written."""
+    rng = np.random.default_rng(page)
+    rows, width = 60, 6
+    length = rng.integers(0, width * page + 1, rows)
+    parent = rng.integers(0, rows, rows)
+    table, fresh = rng.integers(0, 999, (rows, width)), rng.integers(0, 999, rows)
+    table[rng.random(table.shape) < 0.4] = -1
+    table[length == 0] = -1
+    table[7] = -(1 << 31)
+    parent[:4] = 7
+    length[7] = 3 * page + 5
+    d = {k: dev(np.asarray(v, np.int32)) for k, v in dict(parent=parent, len=length, table=table, fresh=fresh).items()}
+    o = dict(out_len=full(rows), out_table=full((rows, width)), src=full(rows), dst=full(rows))
+    vb.k_beam_tables(vb.BeamTables(rows=rows, page=page, width=width, ldt=width, **{k: vg.ptr(v) for k, v in {**d, **o}.items()}))
+    out, new, src, dst = km.beam_tables(parent, length, table, fresh, page, width)
+    absent = (new % page > 0) & (src < 0)
+    assert absent[:4].all() and absent.sum() > 10 and (dst >= 0).sum() > 10
+    out[absent, new[absent] // page] = src[absent] = dst[absent] = -1
+    for name, w in (("out_table", out), ("out_len", new), ("src", src), ("dst", dst)):
+        assert_equal(to_np(o[name]), w, name)
+
+
+def test_attention_after_tables_of_absent_pages(gpu):
+    """Tokens that found no page do not count before their beams are reordered, and do not after it."""
+    a = Attend(np.random.default_rng(60), [40, 40, 300, 300], 16, 2, 64, 8, 4)
+    a.table[1, 2] = a.table[3, 18] = -1
+    a.check()
+    spare = np.setdiff1d(np.arange(a.cache.c.pages), a.table[a.table >= 0])   # pages that hold anything
+    parent = np.array([1, 1, 3, 2], np.int32)
+    d = dict(parent=dev(parent), len=dev(a.lens.astype(np.int32)), table=dev(a.table), fresh=dev(np.resize(spare, 4).astype(np.int32)))
+    o = dict(out_len=full(4), out_table=full(a.table.shape), src=full(4), dst=full(4))
+    vb.k_beam_tables(vb.BeamTables(rows=4, page=16, width=a.width, ldt=a.table.shape[1], **{k: vg.ptr(v) for k, v in {**d, **o}.items()}))
+    vk.k_kv_copy(a.cache.c, o["src"], o["dst"], 4)
+    want = a.want()[[1, 1, 3, 2]]            # of the parents' queries
+    a.q, a.lens = a.q[parent], to_np(o["out_len"])
+    a.table[:, :a.width] = to_np(o["out_table"])[:, :a.width]
+    out = a.want()
+    assert_equal(out, want, "tables")
+    a.check()

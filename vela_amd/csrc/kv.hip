@@ -315,18 +315,19 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvView c, const int32_t* s
 }
 
 __global__ void __launch_bounds__(256) beam_tables_kernel(VgemmBeamTables t, int lp) {
-    const int r = blockIdx.x, p = t.parent[r];
+    const int r = blockIdx.x, p = t.parent[r], own = t.fresh[r];
     const bool there = unsigned(p) < unsigned(t.rows);
     const int n = there ? int(min(i64(max(t.len[p], 0)), i64(t.width) << lp)) : 0;
     const int full = n >> lp;
-    const bool part = n & (t.page - 1);
     const int32_t* old = t.table + size_t(there ? p : 0) * t.ldt;
+    const int last = n & (t.page - 1) ? old[full] : -1;   // the partly filled page; a fresh one instead of none would hold what nobody has written
+    const int fresh = last >= 0 ? own : -1;
     int32_t* row = t.out_table + size_t(r) * t.ldt;
-    for (int j = threadIdx.x; j < t.width; j += 256) row[j] = j < full ? old[j] : (j == full && part ? t.fresh[r] : -1);
+    for (int j = threadIdx.x; j < t.width; j += 256) row[j] = j < full ? old[j] : (j == full ? fresh : -1);
     if (threadIdx.x == 0) {
         t.out_len[r] = n;
-        t.src[r] = part ? old[full] : -1;
-        t.dst[r] = part ? t.fresh[r] : -1;
+        t.src[r] = max(last, -1);
+        t.dst[r] = fresh;
     }
 }
 
