@@ -90,7 +90,7 @@ __device__ __forceinline__ void by_rank(const u64* list, int c, int row, int row
 struct __attribute__((packed, aligned(4))) Quad { int v[4]; };   // sixteen bytes that lie where rows of any length put them
 
 // One span of one row, by WAVES waves of a block of four: one where there are spans for all CUs (a wave's search, sums and order then serve 64
-// values a lane: 200 x 100003 logits 49 -> 22 us, 3.6 TB/s, 13 of them the read alone), four where the call's own latency counts (4 x 32000: 5.8 us).
+// values a lane; 200 x 100003 logits take 22 us, 3.6 TB/s, 13 of them the read alone), four where the call's own latency counts (4 x 32000: 5.9 us).
 template <int WAVES>
 __global__ void __launch_bounds__(256, WAVES == 1 ? 5 : 4) beam_span_kernel(BeamArgs a) {
     constexpr int PER = BEAM_SPAN / (64 * WAVES);
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(BeamArgs a) {
 
 hipError_t launch_beam_select(hipStream_t st, const BeamArgs& a) {
     const int spans = a.b.groups * a.b.beams * a.spans;
-    // 512 spans 37.9 us a pass with four waves each and 41.0 with one, 2048 20.1 both, 5000 32.2 and 30.3 (an earlier merge included)
+    // 512 spans 10.7 us a pass with four waves each and 13.5 with one, 2048 16.8 and 17.7, 4096 23.5 and 22.9, 5000 28.4 and 28.2
     if (spans >= 2048) beam_span_kernel<1><<<(spans + 3) / 4, 256, 0, st>>>(a);
     else beam_span_kernel<4><<<spans, 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError()) return e;

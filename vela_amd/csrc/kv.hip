@@ -334,15 +334,15 @@ __global__ void __launch_bounds__(256) beam_tables_kernel(VgemmBeamTables t, int
 }  // namespace
 
 hipError_t launch_kv_plan(hipStream_t st, const VgemmKvPlan& p, int lp) {
-    // 256 token rows a block, or 1024 new pages where the rows are few; block 0 alone where there are none
+    // 256 token rows a block, 1024 blocks at most; the new pages, never more than the tokens, are dealt over the same blocks. Without rows one block writes them all.
     const int blocks = std::max(1, std::min(int((int64_t(p.tokens) + 255) / 256), 1024));
     kv_plan_kernel<<<blocks, 256, size_t(p.R) * 8, st>>>(p, lp);
     return hipGetLastError();
 }
 
 // Few tokens are mostly a decode step's, each in a page of its own: their bytes go one by one, without LDS and its two barriers. Written and read back, 8
-// heads x 128: 24 tokens apart 10.4 us so and 10.9 turned over (the host's time for two calls); in a row, 8 bits, 1000 11.3 and 12.5, 2000 16.6 and 16.4, 4000 27.5 and 22.8; 16 bits,
-// 1000 15.1 and 13.7, 5000 55 and 33.
+// heads x 128: 24 tokens apart 10.1 us so and 10.7 turned over (the host's time for two calls); in a row, 8 bits, 1000 11.2 and 12.4, 2000 16.5 and 16.2, 4000 27.2 and 22.4; 16 bits,
+// 500 9.9 and 10.7, 1000 15.2 and 13.7, 5000 55 and 35.
 constexpr int RUNS_FROM = 2048;   // tokens times planes
 
 hipError_t launch_kv_write(hipStream_t st, const KvView& c, const int32_t* K, const int32_t* V, int ld, const int32_t* slot, int M) {

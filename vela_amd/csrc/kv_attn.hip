@@ -6,9 +6,9 @@
 // span, and what goes from the first kernel to the join is 4 D bytes a span and query head beside the 512 D bytes of its 8-bit keys and values.
 //
 // A block of four waves takes a span of one sequence and key head with up to sixteen of its query heads, the columns of the 16x16x64 int8
-// matrix instruction. What bounds it is memory: two sequences of 131072 tokens (8 x 128 heads, 8 bits, 32 query heads) take 111 us, 4.8 TB/s of
-// cache, against 5.0 for a copy; a span alone is a chain of two loads and ~3.5 us of work, 5.6 us for a sequence of 500 tokens (16 x 64, 16 bits) without its
-// join.
+// matrix instruction. What bounds it is memory: two sequences of 131072 tokens (8 x 128 heads, 8 bits, 32 query heads) take 112 us, 4.8 TB/s of
+// cache, against 5.0 for a copy; a span alone is a chain of two loads and ~3.5 us of work: a sequence of 500 tokens (16 x 64, 16 bits), two spans side by side and
+// their join in one launch, takes 7.8 us.
 //   * Scores: wave w has the positions [64 w, 64 w + 64). The keys are the A operand; row i of subtile ks is position 16 (i / 4) + 4 ks + i % 4, so that
 //     lane (fg, query) ends with the scores of the 16 positions from 16 fg on, in order. Quarters of four tokens
 //     lie together in a page (vgemm_kv.h), so a load touches four runs of 256 bytes.
@@ -146,7 +146,7 @@ __device__ __forceinline__ void store_words(void* p, const T (&w)[N]) {
 
 // EXACT: D == 64 NS, so that the loads' offsets are constants. F: up to 16 / F query heads share a key head; each stands in F columns, whose
 // lanes take a F-th of its scores, weights and results (the matrix instructions give all of them in every column): 780 vector instructions a wave and
-// span for 128 values in 8 bits with F = 1, about 450 with 4; four queries a key, 32 x 8192 tokens of 64 values 82 -> 73 us, of 128 89 % of the time.
+// span for 128 values in 8 bits with F = 1, about 450 with 4; four queries a key, 32 x 8192 tokens of 64 values 78 -> 68 us, of 128 133 -> 127; eight, F = 2, 82 -> 75 and 140 -> 135.
 // chunks > 0: blocks take runs of spans of one sequence and key head, as even as the lengths allow, so that there are about `chunks` runs
 // a head over all sequences; every block counts them from the lengths. chunks = 0: a block has one span, or each gridDim.z-th.
 // SHORT: a block of eight waves takes a sequence of at most SHORT_SPANS spans, two at a time, each by four waves as elsewhere, and joins them itself.
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(SHORT ? 512 : 256, SHORT ? 2 : kv_held(64 * NS
 
 // ---------------------------------------------------------------- the join
 
-constexpr int JOIN_ONE = 64;       // spans that one wave joins, a lane each for their weights: 8 spans 13.0 us a pass so and 19.2 with eight waves, 64 of 32 sequences 242 and 244
+constexpr int JOIN_ONE = 64;       // spans that one wave joins, a lane each for their weights: 8 spans 12.0 us a pass so and 19.3 with eight waves, 64 of 32 sequences 241 and 244
 constexpr int JOIN_WAVES = 8;      // waves of a query head where there are more
 constexpr int JOIN_CHUNK = 64 * JOIN_WAVES;   // spans whose weights stand in LDS at a time
 
@@ -818,16 +818,16 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     const int heads = a.c.heads * a.qtiles;
     const int spans = a.window > 0 ? std::min(a.spans, a.window / KV_SPAN + 2) : a.spans;   // that a sequence may have
     const int held = 256 * kv_held(a.c.D, a.c.planes);   // blocks the card holds at a time
-    // Few spans a sequence, and a CU for each sequence and head: one launch (500 tokens of 16 heads 9.4 us a pass, 13 with the join's launch; 32 x 1000 of 8 heads
-    // 17.5 and 21.1). With twice as many, sequences of unequal length wait for the longest twice (64 ragged ones up to 1000: 21.9 and 16.3).
+    // Few spans a sequence, and a CU for each sequence and head: one launch (500 tokens of 16 heads 9.2 us a pass, 11.0 with the join's launch; 32 x 1000 of 8 heads
+    // 17.4 and 21.0). With twice as many, sequences of unequal length wait for the longest twice (64 ragged ones up to 1000: 21.7 and 15.2).
     if (spans > 1 && spans <= SHORT_SPANS && kv_short(a.c.D, a.c.planes) && i64(heads) * a.rows <= 256) {
         launch_spans(st, a, dim3(heads, a.rows), -1);
         return hipGetLastError();
     }
     if (a.rows <= DEAL_ROWS && i64(heads) * a.rows * spans > 2 * held) {
-        // Blocks with more than two spans each take them as dealt (32 x 4096 tokens 80.6 us a pass, 85.7 with a block a span; 16 x 2000, 1.3 spans a block,
-        // 29.3 and 28.0). Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
-        // of max_len (a run costs its spans and START more; 64 x 8192 tokens in two runs a block 256 us, in one 282), and at least two where the sequences alone are more than the
+        // Blocks with more than two spans each take them as dealt (256 ragged sequences up to 8000 tokens 136 us a pass, 193 with a block a span; 2 x 131072 129 and
+        // 133; 32 x 4096 67.1 and 67.7; 16 x 2000, 1.3 spans a block, 21.0 and 21.2). Runs of a length that gives each of these blocks one, two, three or four: the one whose rounds of blocks would take least if all sequences were
+        // of max_len (a run costs its spans and START more; 64 x 8192 tokens in two runs a block 237 us, in one 252), and at least two where the sequences alone are more than the
         // blocks: then the longest are what is waited for.
         const float START = 1.5f;
         const i64 all = i64(a.rows) * spans;
@@ -852,7 +852,7 @@ hipError_t launch_kv_attention(hipStream_t st, const KvAttnArgs& a) {
     if (spans <= JOIN_ONE) {
         kv_join_kernel<1><<<dim3((a.Hq + 3) / 4, a.rows), 256, 0, st>>>(a, a.c.D);
     } else {
-        const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;   // 64 heads of 128: 10.4 us so, 16.4 with a block a head
+        const int dims = a.rows * a.Hq >= 256 ? a.c.D : 32;   // 2 x 131072, 64 heads of 128: 129 us so, 135 with a block a head; 128 heads 131 and 129
         kv_join_kernel<JOIN_WAVES><<<dim3(a.Hq * ((a.c.D + dims - 1) / dims), a.rows), 64 * JOIN_WAVES, 0, st>>>(a, dims);
     }
     return hipGetLastError();
